@@ -32,7 +32,9 @@ __device__ __forceinline__ float head_sum(float v, int hl) {
   return v;
 }
 
+// (four products, three sums, unfused: the roundings that the layers' recorded results hold)
 __device__ __forceinline__ float dot4(const f32x4& a, const f32x4& b) {
+#pragma clang fp contract(off)
   return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
 }
 
