@@ -52,6 +52,10 @@ extern "C" {
  * (reference utils/ops.py:524-548: mode_1 -> divisor 100, mode_3 -> divisor 200) */
 #define SAMBLE_TEMP_FIXED 0
 #define SAMBLE_TEMP_COUNT 1
+/* element types of the entry points that take more than fp32 */
+#define SAMBLE_TYPE_F32 0
+#define SAMBLE_TYPE_F16 1
+#define SAMBLE_TYPE_BF16 2
 
 const char* samble_version(void);
 const char* samble_last_error(void);
@@ -717,6 +721,27 @@ size_t samble_amax_bwd_workspace_bytes(int B, int N, int O);
 int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const int32_t* arg, const float* gy, const float* W,
                         int O, float* dx_inout, int64_t dx_bs, float* dW, void* ws, size_t ws_bytes, void* stream);
 
+/* Layer normalisation over the middle axis of (outer, C, inner): inner = 1 for rows of C contiguous values (a row every x_os
+   elements; x_cs unused), otherwise channel-major slices as this library's layers hold them, (B, C, N) with channel stride
+   x_cs and contiguous columns.  type / w_type: SAMBLE_TYPE_* of the tensors / of weight and bias (w_type = type or F32; either
+   pointer may be null: 1 / 0).
+     samble_layer_norm_fwd   s = x [+ residual, rounded to `type` and written to `sum` (outer, C, inner) contiguous];
+                             y = (s - mean) rstd weight + bias, contiguous; biased variance; mean / rstd (outer, inner) fp32 for
+                             the backward (both may be null)
+     samble_layer_norm_bwd   x: the normalised tensor (x, or `sum`); dx = rstd (g - mean(g) - xhat mean(g xhat)) with
+                             g = dy weight, plus `extra` (may be null: the gradient that reaches the sum from elsewhere),
+                             contiguous; dweight / dbias (both or neither null) of type w_type, sums in fp32 in a fixed order.
+                             workspace: samble_layer_norm_workspace_bytes, needed for dweight / dbias only
+   outputs do not overlap inputs, except dx = dy or dx = extra where those are contiguous */
+size_t samble_layer_norm_workspace_bytes(int type, int C, int64_t outer, int64_t inner);
+int samble_layer_norm_fwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* residual, int64_t r_os,
+                          int64_t r_cs, const void* weight, const void* bias, int64_t outer, int C, int64_t inner, float eps,
+                          void* y, void* sum, float* mean, float* rstd, void* stream);
+int samble_layer_norm_bwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* dy, int64_t dy_os,
+                          int64_t dy_cs, const void* extra, int64_t e_os, int64_t e_cs, const void* weight, const float* mean,
+                          const float* rstd, int64_t outer, int C, int64_t inner, void* dx, void* dweight, void* dbias, void* ws,
+                          size_t ws_bytes, void* stream);
+
 /* ---- measurement hook (bench.py; the only entry points that are not part of the path) ------------------
  * The library records HIP events around its own launches of the selected kernels, on the stream each is
  * launched on.  samble_timing_select(mask): bit SAMBLE_T_x set = time kernel x (0 = off; resets the samples);
@@ -763,6 +788,10 @@ int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const
 #define SAMBLE_T_BN_FWD 37       /* bn_stats + bn_apply: BatchNorm1d training forward */
 #define SAMBLE_T_LIN_CHAIN 38    /* lin_chain: a feed-forward layer's two convolutions in one sweep */
 #define SAMBLE_T_BN_BWD 39       /* bn_bwd_reduce + bn_bwd_apply: BatchNorm1d training backward */
+#define SAMBLE_T_LN_FWD 40       /* layer normalisation, forward */
+#define SAMBLE_T_LN_BWD 41       /* layer normalisation, backward (+ the weight gradients' reduction) */
+#define SAMBLE_T_DIFF_FWD 42     /* differential attention, forward (+ the join of its splits) */
+#define SAMBLE_T_DIFF_BWD 43     /* differential attention, backward (both launches) */
 int samble_timing_select(uint64_t kernel_mask);
 int samble_timing_read(int kernel_id, float* mean_ms, float* median_ms, int* launches);
 

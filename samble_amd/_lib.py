@@ -121,6 +121,12 @@ _SIGNATURES = {
                                              c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
     "samble_bn_train_bwd_apply_f32": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                               c_void_p, c_void_p, c_void_p, c_float, c_void_p]),
+    "samble_layer_norm_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64]),
+    "samble_layer_norm_fwd": (c_int, [c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                      c_int64, c_int, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "samble_layer_norm_bwd": (c_int, [c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                      c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int64, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_size_t, c_void_p]),
     "samble_amax_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "samble_amax_bwd_f32": (c_int, [c_void_p, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                     c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
@@ -268,6 +274,7 @@ TIMED_KERNELS = {
     "alloc_counts": 16, "bin_select": 17, "bwd_prep": 18, "gather": 19, "bwd_rows_f32": 22, "nn_prepare": 23,
     "edge_fwd": 24, "edge_bwd": 25, "n2p_fwd": 26, "n2p_bwd": 27, "inv_nn": 28, "seg_sum": 29, "edge_sums": 30,
     "knn_small": 31, "lin_fwd": 32, "lin_dx": 33, "lin_dw": 34, "lin_amax": 35, "lin_amax_bwd": 36, "bn_fwd": 37, "lin_chain": 38, "bn_bwd": 39,
+    "ln_fwd": 40, "ln_bwd": 41, "diff_fwd": 42, "diff_bwd": 43,
 }
 
 

@@ -1384,3 +1384,58 @@ SAMBLE_API int samble_n2p_attn_bwd_f32(const float* qkv, int64_t bs, int64_t rs,
                                     dbs, drs, (float*)ws, heads, inv_order, inv_offsets, (hipStream_t)stream),
               "samble_n2p_attn_bwd_f32");
 }
+
+/* ---- layer normalisation (csrc/layernorm.hip) -------------------------------------------------------------------------- */
+extern "C" {
+size_t samble_ln_ws_bytes(int, int, long, long);
+int samble_launch_ln_fwd(int, int, const void*, long, long, const void*, long, long, const void*, const void*, long, int, long,
+                         float, void*, void*, float*, float*, hipStream_t);
+int samble_launch_ln_bwd(int, int, const void*, long, long, const void*, long, long, const void*, long, long, const void*,
+                         const float*, const float*, long, int, long, void*, void*, void*, float*, hipStream_t);
+}
+
+static bool type_ok(int type) { return type >= SAMBLE_TYPE_F32 && type <= SAMBLE_TYPE_BF16; }
+static bool aligned_for(int type, const void* p) { return (reinterpret_cast<uintptr_t>(p) & (type == SAMBLE_TYPE_F32 ? 3 : 1)) == 0; }
+
+static int ln_args_ok(const char* who, int type, int w_type, const void* x, const void* w, int64_t outer, int C, int64_t inner) {
+  if (!type_ok(type) || (w_type != type && w_type != SAMBLE_TYPE_F32)) return fail(SAMBLE_E_INVALID, who);
+  if (outer <= 0 || inner <= 0 || C <= 0 || outer > (int64_t)1 << 40 || inner > (int64_t)1 << 40) return fail(SAMBLE_E_INVALID, who);
+  if (!x || !aligned_for(type, x) || !aligned_for(w_type, w)) return fail(SAMBLE_E_INVALID, who);
+  return 0;
+}
+
+SAMBLE_API size_t samble_layer_norm_workspace_bytes(int type, int C, int64_t outer, int64_t inner) {
+  return (type_ok(type) && C > 0 && outer > 0 && inner > 0) ? samble_ln_ws_bytes(type, C, outer, inner) : 0;
+}
+
+SAMBLE_API int samble_layer_norm_fwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* residual,
+                                     int64_t r_os, int64_t r_cs, const void* weight, const void* bias, int64_t outer, int C,
+                                     int64_t inner, float eps, void* y, void* sum, float* mean, float* rstd, void* stream) {
+  if (int rc = ln_args_ok("samble_layer_norm_fwd: need a known type (weights: the same or fp32), outer, C, inner > 0 and "
+                          "element-aligned tensors", type, w_type, x, weight, outer, C, inner))
+    return rc;
+  if (!y || (!mean) != (!rstd) || (residual && !sum) || !aligned_for(type, y) || !aligned_for(type, residual) ||
+      !aligned_for(type, sum) || !aligned_for(w_type, bias))
+    return fail(SAMBLE_E_INVALID, "samble_layer_norm_fwd: y, mean with rstd, and sum with residual are needed, element-aligned");
+  return done(samble_launch_ln_fwd(type, w_type == SAMBLE_TYPE_F32, x, x_os, x_cs, residual, r_os, r_cs, weight, bias, outer, C,
+                                   inner, eps, y, sum, mean, rstd, (hipStream_t)stream),
+              "samble_layer_norm_fwd");
+}
+
+SAMBLE_API int samble_layer_norm_bwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* dy,
+                                     int64_t dy_os, int64_t dy_cs, const void* extra, int64_t e_os, int64_t e_cs,
+                                     const void* weight, const float* mean, const float* rstd, int64_t outer, int C,
+                                     int64_t inner, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
+                                     void* stream) {
+  if (int rc = ln_args_ok("samble_layer_norm_bwd: need a known type (weights: the same or fp32), outer, C, inner > 0 and "
+                          "element-aligned tensors", type, w_type, x, weight, outer, C, inner))
+    return rc;
+  if (!dy || !mean || !rstd || !dx || !aligned_for(type, dy) || !aligned_for(type, dx) || !aligned_for(type, extra) ||
+      (!dweight) != (!dbias) || !aligned_for(w_type, dweight) || !aligned_for(w_type, dbias))
+    return fail(SAMBLE_E_INVALID, "samble_layer_norm_bwd: dy, mean, rstd, dx, and dweight with dbias or neither, element-aligned");
+  if (dweight && (!ws || ws_bytes < samble_ln_ws_bytes(type, C, outer, inner)))
+    return fail(SAMBLE_E_WORKSPACE, "samble_layer_norm_bwd: workspace too small (samble_layer_norm_workspace_bytes)");
+  return done(samble_launch_ln_bwd(type, w_type == SAMBLE_TYPE_F32, x, x_os, x_cs, dy, dy_os, dy_cs, extra, e_os, e_cs, weight,
+                                   mean, rstd, outer, C, inner, dx, dweight, dbias, (float*)ws, (hipStream_t)stream),
+              "samble_layer_norm_bwd");
+}
