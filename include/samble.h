@@ -721,6 +721,30 @@ size_t samble_amax_bwd_workspace_bytes(int B, int N, int O);
 int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const int32_t* arg, const float* gy, const float* W,
                         int O, float* dx_inout, int64_t dx_bs, float* dW, void* ws, size_t ws_bytes, void* stream);
 
+/* Differential attention: per query head h two softmax maps over the keys,
+       P_m = softmax_j(scale <q[b,i,h,m], k[b,j,hk,m]>),  m = 0, 1,   hk = h / (H / Hkv)
+       out[b,i,h] = sum_j (P_0 - lam[h] P_1)_ij v[b,j,hk]              (2 d values)
+   type: SAMBLE_TYPE_* of q, k, v, out and the gradients; lam_type = type or F32 (lam, dlam).
+     shape   (host) B, Nq, Nk, H, Hkv, d          H a multiple of Hkv; d a multiple of 8, at most 128 (fp32: 64)
+     strides (host) q: batch, row, head, map; k: batch, row, head, map; v: batch, row, head; key_mask: batch; and for the
+                    backward dout: batch, row, head.  The last axes are contiguous; every row starts on 16 bytes
+     lengths (B) or null: item b has that many keys (taken into 0 .. Nk); key_mask (B, Nk) or null: 0 = the key does not exist
+     causal          query i sees the keys up to position q_start[b] + i; q_start null: Nk - Nq
+   A row that sees no key gives zeros and takes no part in the gradients.  Values of keys that do not exist are never used.
+     samble_diff_attn_fwd   out (B, Nq, H, 2 d) contiguous; out2 (sum_j P_1 v, same shape) and lse (B, H, 2, Nq) for the
+                            backward, both or neither null; workspace: samble_diff_attn_fwd_workspace_bytes (may be 0)
+     samble_diff_attn_bwd   dq (B, Nq, H, 2, d), dk (B, Nk, Hkv, 2, d), dv (B, Nk, Hkv, 2 d), dlam (H), contiguous, every
+                            element written; workspace: samble_diff_attn_bwd_workspace_bytes.  No atomics */
+size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* shape);
+int samble_diff_attn_fwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                         const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                         const uint8_t* key_mask, int causal, float scale, void* out, void* out2, float* lse, void* ws,
+                         size_t ws_bytes, void* stream);
+size_t samble_diff_attn_bwd_workspace_bytes(int type, const int64_t* shape);
+int samble_diff_attn_bwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                         const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                         const uint8_t* key_mask, int causal, float scale, const void* out, const void* out2, const float* lse,
+                         const void* dout, void* dq, void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
 /* Layer normalisation over the middle axis of (outer, C, inner): inner = 1 for rows of C contiguous values (a row every x_os
    elements; x_cs unused), otherwise channel-major slices as this library's layers hold them, (B, C, N) with channel stride
    x_cs and contiguous columns.  type / w_type: SAMBLE_TYPE_* of the tensors / of weight and bias (w_type = type or F32; either

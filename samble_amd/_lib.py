@@ -121,6 +121,13 @@ _SIGNATURES = {
                                              c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
     "samble_bn_train_bwd_apply_f32": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                               c_void_p, c_void_p, c_void_p, c_float, c_void_p]),
+    "samble_diff_attn_fwd_workspace_bytes": (c_size_t, [c_int, c_void_p]),
+    "samble_diff_attn_fwd": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "samble_diff_attn_bwd_workspace_bytes": (c_size_t, [c_int, c_void_p]),
+    "samble_diff_attn_bwd": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "samble_layer_norm_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64]),
     "samble_layer_norm_fwd": (c_int, [c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                       c_int64, c_int, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),

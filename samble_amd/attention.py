@@ -20,6 +20,7 @@ import torch
 from torch import nn
 
 from . import linear, ops
+from .norm import LayerNorm
 
 
 def _attention_from_projection(qkv, nn_idx, heads: int, diff: bool):
@@ -530,6 +531,152 @@ def _p2p_attention_in_torch(self, x):
 
 
 Point2PointAttention._attention_in_torch = _p2p_attention_in_torch
+
+
+class _DiffAttn(torch.autograd.Function):
+    @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
+    def forward(ctx, q, k, v, lam, scale, causal, lengths, q_start, key_mask):
+        out, out2, lse = ops.stage_diff_attn_fwd(q, k, v, lam, scale, causal, lengths, q_start, key_mask, for_backward=True)
+        ctx.save_for_backward(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse)
+        ctx.cfg = (scale, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @torch.amp.custom_bwd(device_type="cuda")
+    def backward(ctx, g):
+        q, k, v, lam, lengths, q_start, key_mask, out, out2, lse = ctx.saved_tensors
+        grads = ops.stage_diff_attn_bwd(q, k, v, lam, *ctx.cfg, lengths, q_start, key_mask, out, out2, lse, g.to(q.dtype))
+        return tuple(d if need else None for d, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
+
+
+def _per_item(name: str, t, B: int, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.shape != (B,) or t.dtype not in (torch.int32, torch.int64) or t.device != device:
+        raise ValueError(f"differential_attention: {name} must be a ({B},) int32 or int64 tensor on {device}")
+    if t.dtype == torch.int64:      # (beyond int32: the nearest, which stands for the same keys)
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t.contiguous()
+
+
+def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam, *, scale=None, causal: bool = False,
+                           lengths=None, q_start=None, key_mask=None) -> torch.Tensor:
+    """Attention by the difference of two softmax maps: out = (softmax(scale q_1 k_1^T) - lam softmax(scale q_2 k_2^T)) v,
+    differentiable in q, k, v and lam.
+
+    q (B, Nq, H, 2, d), k (B, Nk, Hkv, 2, d): two maps per head; v (B, Nk, Hkv, 2 d) -> (B, Nq, H, 2 d).  fp32, fp16 or
+    bf16, one type, softmax statistics and sums in fp32; Hkv divides H (query head h reads key head h // (H // Hkv)); d a
+    multiple of 8 up to 128 (fp32: 64).  Any strides (copied unless rows start on 16 bytes and the last axis is contiguous).
+    lam: (H,) or one value, of q's type or fp32.  scale: 1 / sqrt(d) unless given, positive.
+    lengths (B,): item b has that many keys (out of 0 .. Nk: the nearest); key_mask (B, Nk) bool: False = the key does not
+    exist.  Whatever stands at keys that do not exist, NaN included, is not used and gets gradient 0.
+    causal: query i sees the keys up to position q_start[b] + i; q_start (B,) is Nk - Nq unless given (the queries are the
+    last ones).  Keys that only the causal order hides must be finite.
+    A row that sees no key gives zeros and gets no gradient.  The calls Nq = 1 over a long cache split the keys over the GPU."""
+    for name, t, n in (("q", q, 5), ("k", k, 5), ("v", v, 4)):
+        if not isinstance(t, torch.Tensor) or t.dim() != n:
+            raise ValueError(f"differential_attention: {name} must be a tensor with {n} axes")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("differential_attention: q, k and v must share one type and device")
+    if q.dtype not in ops.ELEMENT_TYPES:
+        raise ValueError(f"differential_attention: float32, float16 or bfloat16, got {q.dtype}")
+    B, Nq, H, two, d = q.shape
+    Nk, Hkv = k.shape[1:3]
+    if two != 2 or k.shape != (B, Nk, Hkv, 2, d) or v.shape != (B, Nk, Hkv, 2 * d):
+        raise ValueError(f"differential_attention: q (B,Nq,H,2,d), k (B,Nk,Hkv,2,d), v (B,Nk,Hkv,2d); got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise ValueError(f"differential_attention: {H} query heads do not share {Hkv} key heads evenly")
+    most = 64 if q.dtype == torch.float32 else 128
+    if d < 8 or d % 8 or d > most:
+        raise ValueError(f"differential_attention: d = {d} must be a multiple of 8 up to {most} for {q.dtype}")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"differential_attention: scale must be positive, got {scale}")
+    if not isinstance(lam, torch.Tensor):
+        lam = torch.full((H,), float(lam), dtype=torch.float32, device=q.device)
+    if lam.dtype not in (q.dtype, torch.float32) or lam.device != q.device or lam.shape not in ((H,), (1,), ()):
+        raise ValueError(f"differential_attention: lam must be ({H},) or one value, of type {q.dtype} or float32 on {q.device}")
+    lengths = _per_item("lengths", lengths, B, q.device)
+    if q_start is not None and not causal:
+        raise ValueError("differential_attention: q_start goes with causal=True")
+    q_start = _per_item("q_start", q_start, B, q.device)
+    if key_mask is not None:
+        if key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool or key_mask.device != q.device:
+            raise ValueError(f"differential_attention: key_mask must be a ({B}, {Nk}) bool tensor on {q.device}")
+        if Nk > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    ops._need_gpu(q, k, v, lam, lengths, q_start, key_mask)
+    if B == 0 or Nq == 0 or Nk == 0:      # nothing to sum over: zeros that still hang on the inputs
+        tie = q.sum() * 0 + k.sum() * 0 + v.sum() * 0 + lam.sum().to(q.dtype) * 0
+        return torch.zeros((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device) + torch.nan_to_num(tie)
+    lam = lam.expand(H).contiguous()
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
+        return _DiffAttn.apply(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)
+    return ops.stage_diff_attn_fwd(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)[0]
+
+
+class DifferentialAttention(nn.Module):
+    """Point2PointAttention's layer with differential attention and layer normalisation: global self-attention over the points
+    of (B, C, N) tensors whose heads subtract a second softmax map, lam = exp(lambda_q1 . lambda_k1) - exp(lambda_q2 .
+    lambda_k2) + lambda_init per head, each head's output normalised over its own channels and scaled by 1 - lambda_init:
+
+        x = norm1(x + heads(x));  x = norm2(x + ff(x))
+
+    Constructor fields as Point2PointAttention's (q_in .. v_out equal, C = 2 d H with d a multiple of 8 up to 64), plus an
+    optional `lambda_init` list (default 0.8 - 0.6 exp(-0.3 layer)).  forward(x, lengths=None, key_mask=None): ragged clouds
+    padded to N points -- the points that do not exist are seen by nobody (their own outputs mean nothing)."""
+
+    def __init__(self, config_attention, layer):
+        super().__init__()
+        cfg = config_attention
+        widths = {getattr(cfg, n)[layer] for n in ("q_in", "q_out", "k_in", "k_out", "v_in", "v_out")}
+        if len(widths) != 1:
+            raise ValueError(f"DifferentialAttention: q_in .. v_out must be equal, got {sorted(widths)}")
+        C, H = widths.pop(), cfg.num_heads[layer]
+        if C % (2 * H) or (C // (2 * H)) % 8 or C // (2 * H) > 64:
+            raise ValueError(f"DifferentialAttention: {C} channels in {H} heads: a map's depth C / 2H must be a multiple of 8 up to 64")
+        self.num_heads, self.depth = H, C // (2 * H)
+        self.lambda_init = (cfg.lambda_init[layer] if hasattr(cfg, "lambda_init") else 0.8 - 0.6 * math.exp(-0.3 * layer))
+        self.q_conv = nn.Conv1d(C, C, 1, bias=False)
+        self.k_conv = nn.Conv1d(C, C, 1, bias=False)
+        self.v_conv = nn.Conv1d(C, C, 1, bias=False)
+        for name in ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2"):
+            setattr(self, name, nn.Parameter(0.1 * torch.randn(H, self.depth)))
+        self.head_norm = LayerNorm(2 * self.depth)
+        self.ff = nn.Sequential(
+            nn.Conv1d(cfg.ff_conv1_channels_in[layer], cfg.ff_conv1_channels_out[layer], 1, bias=False),
+            nn.LeakyReLU(negative_slope=0.2),
+            nn.Conv1d(cfg.ff_conv2_channels_in[layer], cfg.ff_conv2_channels_out[layer], 1, bias=False),
+        )
+        self.norm1 = LayerNorm(C, dim=1)
+        self.norm2 = LayerNorm(C, dim=1)
+
+    def lam(self) -> torch.Tensor:
+        return (torch.exp((self.lambda_q1 * self.lambda_k1).sum(-1)) - torch.exp((self.lambda_q2 * self.lambda_k2).sum(-1))
+                + self.lambda_init)
+
+    def forward(self, x, lengths=None, key_mask=None):
+        if not x.is_cuda:
+            raise ops._lib.SambleError("samble_amd.DifferentialAttention runs on the GPU only (no CPU fallback)")
+        B, C, N = x.shape
+        H, d = self.num_heads, self.depth
+        if C == 128:
+            from .downsample import _Projection
+            no_tokens = self.q_conv.weight.new_zeros((1, C, 0))
+            qkv = _Projection.apply(x, no_tokens, self.q_conv.weight, self.k_conv.weight, self.v_conv.weight)
+        else:      # (the projection kernels are built for 128 channels)
+            w = torch.cat((self.q_conv.weight, self.k_conv.weight, self.v_conv.weight)).reshape(3 * C, C)
+            qkv = torch.matmul(x.transpose(1, 2), w.t())
+        q, k, v = qkv.split(C, dim=2)          # rows [Q | K | V]: read where they stand
+        out = differential_attention(q.view(B, N, H, 2, d), k.view(B, N, H, 2, d), v.view(B, N, H, 2 * d), self.lam(),
+                                     lengths=lengths, key_mask=key_mask)
+        out = self.head_norm(out) * (1.0 - self.lambda_init)
+        x, _ = self.norm1(out.reshape(B, N, C).transpose(1, 2).contiguous(), residual=x)
+        x, _ = self.norm2(_feed_forward(self.ff, x), residual=x)
+        return x
 
 
 def attention_config(preset: str = "cls"):

@@ -1439,3 +1439,98 @@ SAMBLE_API int samble_layer_norm_bwd(int type, int w_type, const void* x, int64_
                                    mean, rstd, outer, C, inner, dx, dweight, dbias, (float*)ws, (hipStream_t)stream),
               "samble_layer_norm_bwd");
 }
+
+/* ---- differential attention (csrc/diff_attn_fwd.hip, csrc/diff_attn_bwd.hip) ------------------------------------------- */
+#include "diff_args.h"
+extern "C" {
+size_t samble_diff_fwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d);
+int samble_launch_diff_fwd(int, const samble::DaArgs*, hipStream_t);
+int samble_launch_diff_bwd(int, const samble::DaArgs*, hipStream_t);
+}
+
+static bool diff_shape_ok(int type, const int64_t* n) {
+  if (!n || !type_ok(type)) return false;
+  const int64_t most = (int64_t)1 << 30;
+  for (int i = 0; i < 6; ++i)
+    if (n[i] <= 0 || n[i] > most) return false;
+  return n[3] % n[4] == 0 && n[5] % 8 == 0 && n[5] <= (type == SAMBLE_TYPE_F32 ? 64 : 128) && n[0] <= (1 << 24) && n[3] <= (1 << 20);
+}
+static bool rows16(int type, const void* p, const int64_t* strides, int n) {   // rows on 16 bytes
+  const int64_t unit = type == SAMBLE_TYPE_F32 ? 4 : 8;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % unit || strides[i] < 0) return false;
+  return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+static int diff_args(const char* who, int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                     const int64_t* n, const int64_t* st, const int32_t* lengths, const int32_t* q_start, const uint8_t* key_mask,
+                     int causal, float scale, samble::DaArgs* A) {
+  if (!diff_shape_ok(type, n) || !st || (lam_type != type && lam_type != SAMBLE_TYPE_F32)) return fail(SAMBLE_E_INVALID, who);
+  if (!rows16(type, q, st, 4) || !rows16(type, k, st + 4, 4) || !rows16(type, v, st + 8, 3) || !lam || !aligned_for(lam_type, lam))
+    return fail(SAMBLE_E_INVALID, who);
+  if (!(scale > 0.f) || !(scale < 1e30f) || (q_start && !causal) || st[11] < 0) return fail(SAMBLE_E_INVALID, who);
+  *A = samble::DaArgs{};
+  A->q = q; A->k = k; A->v = v; A->lam = lam;
+  A->q_bs = st[0]; A->q_rs = st[1]; A->q_hs = st[2]; A->q_ms = st[3];
+  A->k_bs = st[4]; A->k_rs = st[5]; A->k_hs = st[6]; A->k_ms = st[7];
+  A->v_bs = st[8]; A->v_rs = st[9]; A->v_hs = st[10]; A->km_bs = st[11];
+  A->lengths = lengths; A->q_start = q_start; A->key_mask = key_mask;
+  A->B = (int)n[0]; A->Nq = (int)n[1]; A->Nk = (int)n[2]; A->H = (int)n[3]; A->Hkv = (int)n[4]; A->G = (int)(n[3] / n[4]);
+  A->d = (int)n[5]; A->causal = causal != 0; A->lam_f32 = lam_type == SAMBLE_TYPE_F32; A->splits = 1; A->scale = scale;
+  return 0;
+}
+#define SAMBLE_DIFF_NEEDS                                                                                                   \
+  ": needs a known type (lam: the same or fp32), positive sizes, H a multiple of Hkv, d a multiple of 8 up to 128 (fp32: 64), " \
+  "rows on 16 bytes, 0 < scale < 1e30, q_start with causal only"
+
+SAMBLE_API size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* n) {
+  return diff_shape_ok(type, n) ? samble_diff_fwd_ws_bytes(type, (int)n[0], (int)n[1], (int)n[2], (int)n[3], (int)n[4], (int)n[5]) : 0;
+}
+
+SAMBLE_API int samble_diff_attn_fwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                                    const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                                    const uint8_t* key_mask, int causal, float scale, void* out, void* out2, float* lse, void* ws,
+                                    size_t ws_bytes, void* stream) {
+  samble::DaArgs A;
+  if (int rc = diff_args("samble_diff_attn_fwd" SAMBLE_DIFF_NEEDS, type, lam_type, q, k, v, lam, shape, strides, lengths, q_start,
+                         key_mask, causal, scale, &A))
+    return rc;
+  const int64_t none = 0;
+  if (!rows16(type, out, &none, 1) || (out2 && !rows16(type, out2, &none, 1)) || (!out2) != (!lse))
+    return fail(SAMBLE_E_INVALID, "samble_diff_attn_fwd: out on 16 bytes, out2 with lse or neither");
+  const size_t need = samble_diff_attn_fwd_workspace_bytes(type, shape);
+  if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)))
+    return fail(SAMBLE_E_WORKSPACE, "samble_diff_attn_fwd: workspace too small (samble_diff_attn_fwd_workspace_bytes)");
+  A.out = out; A.out2 = out2; A.lse = lse; A.part = (float*)ws;
+  const int rc = samble_launch_diff_fwd(type, &A, (hipStream_t)stream);
+  if (rc == -22) return fail(SAMBLE_E_INVALID, "samble_diff_attn_fwd: more rows and heads than one launch holds");
+  return done(rc, "samble_diff_attn_fwd");
+}
+
+SAMBLE_API size_t samble_diff_attn_bwd_workspace_bytes(int type, const int64_t* n) {
+  return diff_shape_ok(type, n) ? (size_t)n[0] * n[3] * 2 * n[1] * sizeof(float) : 0;
+}
+
+SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                                    const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                                    const uint8_t* key_mask, int causal, float scale, const void* out, const void* out2,
+                                    const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* ws,
+                                    size_t ws_bytes, void* stream) {
+  samble::DaArgs A;
+  if (int rc = diff_args("samble_diff_attn_bwd" SAMBLE_DIFF_NEEDS, type, lam_type, q, k, v, lam, shape, strides, lengths, q_start,
+                         key_mask, causal, scale, &A))
+    return rc;
+  const int64_t none = 0;
+  if (!rows16(type, out, &none, 1) || !rows16(type, out2, &none, 1) || !rows16(type, dout, strides + 12, 3) ||
+      !rows16(type, dq, &none, 1) || !rows16(type, dk, &none, 1) || !rows16(type, dv, &none, 1) || !lse || !dlam ||
+      !aligned_for(lam_type, dlam))
+    return fail(SAMBLE_E_INVALID, "samble_diff_attn_bwd: out, out2, lse, dout, dq, dk, dv, dlam are needed, rows on 16 bytes");
+  if (!ws || ws_bytes < samble_diff_attn_bwd_workspace_bytes(type, shape))
+    return fail(SAMBLE_E_WORKSPACE, "samble_diff_attn_bwd: workspace too small (samble_diff_attn_bwd_workspace_bytes)");
+  A.out = const_cast<void*>(out); A.out2 = const_cast<void*>(out2); A.lse = const_cast<float*>(lse); A.dout = dout;
+  A.g_bs = strides[12]; A.g_rs = strides[13]; A.g_hs = strides[14];
+  A.dq = dq; A.dk = dk; A.dv = dv; A.dlam = dlam; A.delta = (float*)ws;
+  const int rc = samble_launch_diff_bwd(type, &A, (hipStream_t)stream);
+  if (rc == -22) return fail(SAMBLE_E_INVALID, "samble_diff_attn_bwd: more rows and heads than one launch holds");
+  return done(rc, "samble_diff_attn_bwd");
+}

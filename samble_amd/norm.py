@@ -10,9 +10,8 @@ import torch
 from torch import nn
 
 from . import _lib
+from .ops import ELEMENT_TYPES as TYPES
 from .ops import _need_gpu, _p, _stream
-
-TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # include/samble.h SAMBLE_TYPE_*
 
 
 def _slices(t: torch.Tensor, dim: int):

@@ -1,0 +1,495 @@
+"""Differential attention (samble_amd.attention.differential_attention, csrc/diff_attn_*.hip) against its formulas in float64.
+
+Tolerances are sums of the roundings that the kernels are allowed, per element:
+  * U = 2^-24 arithmetic.  A dot product of n terms in fp32 is off by at most (n + 32) U times the sum of magnitudes (fp32
+    tensors: the three bf16 planes and six products lose a few U of the same sum, inside the 32).  With L the largest such sum
+    over a row's logits, a probability is off by the factor 2 * ((d + 32) U L + 16 U); sums over n keys or rows by n U.
+  * h = eps / 2 of the tensors' type: P, P_1 - lam P_2 and dS enter the second products rounded once (fp16 / bf16 only; fp32
+    enters whole), saved outputs and results are rounded once.  fp16 adds half a subnormal step, 2^-25, where values are small.
+"""
+import math
+
+import pytest
+import torch
+
+from samble_amd import _lib
+
+U = 2.0 ** -24
+DEV = "cuda"
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _visible(B, Nq, Nk, causal, lengths, q_start, key_mask, device):
+    j = torch.arange(Nk, device=device)
+    ok = torch.ones((B, Nq, Nk), dtype=torch.bool, device=device)
+    if lengths is not None:
+        ok &= (j < lengths[:, None])[:, None, :]
+    if key_mask is not None:
+        ok &= key_mask[:, None, :]
+    if causal:
+        start = torch.full((B,), Nk - Nq, device=device) if q_start is None else q_start
+        ok &= j <= (torch.arange(Nq, device=device)[None, :, None] + start[:, None, None])
+    return ok
+
+
+def _check(q, k, v, lam, g, got, scale, causal, lengths, q_start, key_mask):
+    """got = (out[, dq, dk, dv, dlam]) against float64 within the derived bounds; one (batch item, key head) at a time."""
+    B, Nq, H, _, d = q.shape
+    Nk, Hkv = k.shape[1:3]
+    G = H // Hkv
+    dt = q.dtype
+    half = torch.finfo(dt).eps / 2
+    hp = 0.0 if dt == torch.float32 else half       # P and dS as operands
+    sub = 2.0 ** -25 if dt == torch.float16 else 0.0
+    ok_all = _visible(B, Nq, Nk, causal, lengths, q_start, key_mask, q.device)
+    lam_err = torch.zeros(H, dtype=torch.float64, device=q.device)
+    lam_ref = torch.zeros(H, dtype=torch.float64, device=q.device)
+
+    def held(x, ref, tol, what):
+        tol = tol * (1 + 1e-3) + half * ref.abs() + sub + 1e-30
+        err = (x.double() - ref).abs()
+        bad = (err - tol).max().item() if err.numel() else 0.0
+        assert bool(torch.isfinite(x).all()), f"{what}: not finite"
+        assert bad <= 0, f"{what}: {bad:.3e} over the bound (worst error {err.max():.3e}, largest value {ref.abs().max():.3e})"
+
+    for b in range(B):
+        seen_key = ok_all[b].any(0)
+        for hk in range(Hkv):
+            # keys that do not exist may hold anything
+            kk = torch.where(seen_key[:, None, None], k[b, :, hk].double(), 0.0)       # (Nk, 2, d)
+            vv = torch.where(seen_key[:, None], v[b, :, hk].double(), 0.0)             # (Nk, 2d)
+            dk_ref, dk_tol = torch.zeros_like(kk), torch.zeros_like(kk)
+            dv_ref, dv_tol = torch.zeros_like(vv), torch.zeros_like(vv)
+            ok = ok_all[b]
+            for hq in range(hk * G, hk * G + G):
+                qq, lm = q[b, :, hq].double(), float(lam[hq].double())
+                P, dP = [], []
+                for m in range(2):
+                    s = qq[:, m] @ kk[:, m].T * scale
+                    s = torch.where(ok, s, -math.inf)
+                    top = s.amax(-1, keepdim=True)
+                    p = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+                    tot = p.sum(-1, keepdim=True)
+                    P.append(p / torch.where(tot == 0, 1.0, tot))
+                    L = torch.where(ok, qq[:, m].abs() @ kk[:, m].abs().T * scale, 0.0).amax(-1, keepdim=True)
+                    dP.append(2 * ((d + 32) * U * L + 16 * U) + Nk * U)                # relative error of the map, per row
+                o1, o2 = P[0] @ vv, P[1] @ vv
+                av = vv.abs()
+                e1 = (P[0] * (dP[0] + hp)) @ av + sub * (ok.double() @ av)             # error of o1, o2 before rounding
+                e2 = (P[1] * (dP[1] + hp)) @ av + sub * (ok.double() @ av)
+                ref = o1 - lm * o2
+                held(got[0][b, :, hq], ref, e1 + abs(lm) * e2 + 4 * U * (o1.abs() + abs(lm) * o2.abs()), f"out b{b} h{hq}")
+                if g is None:
+                    continue
+                gg = g[b, :, hq].double()
+                A = P[0] - lm * P[1]
+                eA = P[0] * dP[0] + abs(lm) * P[1] * dP[1] + hp * A.abs() + sub * ok
+                dv_ref += A.T @ gg
+                dv_tol += eA.T @ gg.abs() + Nq * G * U * (A.abs().T @ gg.abs())
+                dA = gg @ vv.T
+                edA = (2 * d + 32) * U * (gg.abs() @ av.T)
+                t2 = (P[1] * dA).sum(-1, keepdim=True)
+                t1 = (P[0] * dA).sum(-1, keepdim=True)
+                out_err = e1 + abs(lm) * e2 + half * ref.abs() + sub
+                out2_err = e2 + half * o2.abs() + sub
+                n = (2 * d + 32) * U
+                et2 = (gg.abs() * (out2_err + n * o2.abs())).sum(-1, keepdim=True)
+                et1 = (gg.abs() * (out_err + n * ref.abs())).sum(-1, keepdim=True) + abs(lm) * et2
+                lam_ref[hq] += -t2.sum()
+                lam_err[hq] += et2.sum() + Nq * B * U * t2.abs().sum()
+                for m, (t, et, sign) in enumerate(((t1, et1, 1.0), (t2, et2, -lm))):
+                    dS = sign * P[m] * (dA - t)
+                    edS = abs(sign) * P[m] * (edA + et + (dP[m] + 4 * U) * (dA - t).abs()) + hp * dS.abs() + sub * ok
+                    dq_ref = scale * dS @ kk[:, m]
+                    dq_tol = scale * (edS + Nk * U * dS.abs()) @ kk[:, m].abs()
+                    held(got[1][b, :, hq, m], dq_ref, dq_tol, f"dq b{b} h{hq} m{m}")
+                    dk_ref[:, m] += scale * dS.T @ qq[:, m]
+                    dk_tol[:, m] += scale * (edS + Nq * G * U * dS.abs()).T @ qq[:, m].abs()
+            if g is not None:
+                held(got[2][b, :, hk], dk_ref, dk_tol, f"dk b{b} hk{hk}")
+                held(got[3][b, :, hk], dv_ref, dv_tol, f"dv b{b} hk{hk}")
+    if g is not None:
+        held(got[4], lam_ref, lam_err + (torch.finfo(got[4].dtype).eps / 2) * lam_ref.abs(), "dlam")
+
+
+def _inputs(B, Nq, Nk, H, Hkv, d, dtype, seed, packed=False, spread=1.4):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=gen, device=DEV)  # noqa: E731
+    if packed:      # rows [Q | K | V] of one projection
+        assert Nq == Nk and H == Hkv
+        qkv = (spread * rnd(B, Nk, 3 * H * 2 * d)).to(dtype)
+        q, k, v = qkv.split(H * 2 * d, 2)
+        q, k, v = q.view(B, Nq, H, 2, d), k.view(B, Nk, H, 2, d), v.view(B, Nk, H, 2 * d)
+    else:
+        q, k = (spread * rnd(B, Nq, H, 2, d)).to(dtype), (spread * rnd(B, Nk, Hkv, 2, d)).to(dtype)
+        v = rnd(B, Nk, Hkv, 2 * d).to(dtype)
+    lam = (0.2 + 0.6 * torch.rand(H, generator=gen, device=DEV)).to(dtype if seed % 2 else torch.float32)
+    g = rnd(B, Nq, H, 2 * d).to(dtype)
+    return q, k, v, lam, g, gen
+
+
+def _masks(kind, B, Nq, Nk, gen):
+    lengths = q_start = key_mask = None
+    causal = "causal" in kind
+    if "lengths" in kind:
+        lengths = torch.randint(0, Nk + 1, (B,), generator=gen, device=DEV, dtype=torch.int32)
+        lengths[0] = Nk
+        if B > 1:
+            lengths[1] = 0
+        if causal:
+            q_start = lengths - Nq
+    if "keys" in kind:
+        key_mask = torch.rand((B, Nk), generator=gen, device=DEV) > 0.3
+        key_mask[-1, : Nk // 2] = False
+    return causal, lengths, q_start, key_mask
+
+
+# B, Nq, Nk, H, Hkv, d, masks
+CASES = [
+    (1, 1, 1, 1, 1, 8, ""), (2, 1, 33, 4, 4, 16, "lengths"), (3, 5, 7, 2, 1, 24, "keys"), (2, 33, 31, 3, 3, 16, "causal"),
+    (2, 31, 65, 4, 2, 32, "causal"), (1, 64, 64, 2, 2, 64, "causal"), (2, 129, 127, 2, 1, 64, "causal lengths"),
+    (3, 100, 300, 4, 4, 40, "lengths keys"), (2, 257, 130, 6, 2, 8, "causal keys"), (1, 200, 200, 5, 1, 48, "causal"),
+    (2, 96, 515, 2, 2, 56, "lengths"), (1, 1, 700, 8, 1, 64, ""), (4, 3, 2100, 8, 2, 32, "lengths causal"),
+    (1, 7, 1500, 40, 8, 16, "keys"), (1, 300, 2600, 2, 2, 16, "causal"), (2, 70, 1, 2, 2, 16, ""),
+]
+WIDE = [(1, 1, 600, 4, 2, 128, "lengths"), (2, 65, 130, 2, 1, 128, "causal"), (2, 150, 70, 2, 2, 96, "keys"),
+        (1, 200, 2100, 1, 1, 72, "causal"), (1, 1, 5000, 4, 1, 128, "")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES + WIDE, ids=lambda c: "-".join(str(x).replace(" ", "+") or "full" for x in c))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_forward_and_gradients(case, dtype):
+    from samble_amd.attention import differential_attention
+    B, Nq, Nk, H, Hkv, d, kind = case
+    if dtype == "fp32" and d > 64:
+        pytest.skip("fp32: d up to 64")
+    q, k, v, lam, g, gen = _inputs(B, Nq, Nk, H, Hkv, d, TYPES[dtype], sum(case[:6]))
+    causal, lengths, q_start, key_mask = _masks(kind, B, Nq, Nk, gen)
+    kw = dict(causal=causal, lengths=lengths, q_start=q_start, key_mask=key_mask)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, **kw)
+    grads = torch.autograd.grad(out, leaves, g)
+    _check(q.detach(), k.detach(), v.detach(), lam.detach(), g, (out.detach(),) + grads, d ** -0.5, causal, lengths, q_start, key_mask)
+    with torch.no_grad():
+        assert torch.equal(differential_attention(q, k, v, lam, **kw), out)
+    again = torch.autograd.grad(differential_attention(*leaves, **kw), leaves, g)
+    assert all(torch.equal(a, b) for a, b in zip(again, grads)), "not the same run to run"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_long_cache_single_token(dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, _, gen = _inputs(2, 1, 20011, 8, 2, 64, TYPES[dtype], 4)
+    lengths = torch.tensor([20011, 9001], dtype=torch.int64, device=DEV)
+    out = differential_attention(q, k, v, lam, lengths=lengths)
+    _check(q, k, v, lam, None, (out,), 0.125, False, lengths, None, None)
+    # the cache as a model holds it: heads before positions, longer than what is filled
+    cache_k = torch.full((2, 2, 20100, 2, 64), float("nan"), dtype=TYPES[dtype], device=DEV)
+    cache_v = torch.full((2, 2, 20100, 128), float("nan"), dtype=TYPES[dtype], device=DEV)
+    cache_k[:, :, :20011], cache_v[:, :, :20011] = k.transpose(1, 2), v.transpose(1, 2)
+    cache_k[1, :, 9001:], cache_v[1, :, 9001:] = float("nan"), float("inf")
+    held = differential_attention(q, cache_k.transpose(1, 2), cache_v.transpose(1, 2), lam, lengths=lengths)
+    _check(q, k, v, lam, None, (held,), 0.125, False, lengths, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_strided_operands_scale_and_one_lam(dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, _ = _inputs(2, 150, 150, 4, 4, 16, TYPES[dtype], 11, packed=True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    one = torch.tensor(0.35, device=DEV, requires_grad=True)
+    out = differential_attention(*leaves, one, scale=0.4)
+    grads = torch.autograd.grad(out, leaves + [one], g)
+    full = torch.full((4,), 0.35, device=DEV)
+    split = torch.autograd.grad(differential_attention(*leaves, full.requires_grad_(True), scale=0.4), leaves + [full], g)
+    assert all(torch.equal(a, b) for a, b in zip(grads[:3], split[:3]))
+    torch.testing.assert_close(grads[3], split[3].sum(), rtol=1e-5, atol=1e-5)
+    _check(q, k, v, full.detach(), g, (out.detach(),) + split, 0.4, False, None, None, None)
+    # rows that do not start on 16 bytes, a gradient that is an expanded value, a transposed output gradient
+    odd = [torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape).copy_(t.detach()) for t in leaves]
+    assert torch.equal(differential_attention(*odd, 0.35, scale=0.4), out)
+    ones = torch.autograd.grad(differential_attention(*leaves, 0.35, scale=0.4).sum(), leaves)
+    same = torch.autograd.grad(differential_attention(*leaves, 0.35, scale=0.4), leaves, torch.ones_like(out))
+    assert all(torch.equal(a, b) for a, b in zip(ones, same))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_nothing_of_missing_keys_is_used(dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, gen = _inputs(3, 40, 90, 2, 2, 32, TYPES[dtype], 21)
+    lengths = torch.tensor([90, 0, 50], dtype=torch.int32, device=DEV)
+    mask = torch.rand((3, 90), generator=gen, device=DEV) > 0.4
+    gone = ~(mask & (torch.arange(90, device=DEV) < lengths[:, None]))
+    res = []
+    for filler in (0.0, float("nan"), float("inf"), torch.finfo(TYPES[dtype]).min):
+        kk, vv = k.clone(), v.clone()
+        kk[gone], vv[gone] = filler, -filler if filler == filler else filler
+        leaves = [t.detach().requires_grad_(True) for t in (q, kk, vv, lam)]
+        out = differential_attention(*leaves, lengths=lengths, key_mask=mask)
+        res.append((out.detach(),) + torch.autograd.grad(out, leaves, g))
+    for other in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], other))
+    out, dq, dk, dv, _ = res[0]
+    assert not out[1].any() and not dq[1].any()
+    assert not dk[gone].any() and not dv[gone].any()
+
+
+@pytest.mark.gpu
+def test_lengths_and_starts_out_of_range_are_taken_to_the_nearest():
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, _, _ = _inputs(4, 6, 20, 2, 2, 16, torch.float32, 3)
+    wild = torch.tensor([-5, 1000, 2 ** 40, -(2 ** 40)], device=DEV)
+    tame = torch.tensor([0, 20, 20, 0], device=DEV)
+    assert torch.equal(differential_attention(q, k, v, lam, lengths=wild), differential_attention(q, k, v, lam, lengths=tame))
+    starts = torch.tensor([-100, 2 ** 31 - 1, -2, 3], device=DEV, dtype=torch.int64)
+    out = differential_attention(q, k, v, lam, causal=True, q_start=starts)
+    assert not out[0].any() and not out[2, :2].any() and out[2, 2].any()
+    assert torch.equal(out[1], differential_attention(q, k, v, lam)[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_extreme_logits_and_infinities_stay_in_their_rows(dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, _ = _inputs(1, 70, 200, 1, 1, 16, TYPES[dtype], 6, spread=12.0)     # logits of several hundred
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    out = differential_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, g)
+    _check(q.detach(), k.detach(), v.detach(), lam.detach(), g, (out.detach(),) + grads, 0.25, False, None, None, None)
+    bad = q.detach().clone()
+    bad[0, 13] = float("nan")
+    bad[0, 44, 0, 0, 3] = float("inf")
+    with torch.no_grad():
+        res = differential_attention(bad, k, v, lam)
+    rows = torch.ones(70, dtype=torch.bool, device=DEV)
+    rows[[13, 44]] = False
+    assert torch.equal(res[0, rows], out[0, rows]) and torch.isnan(res[0, 13]).all() and not torch.isfinite(res[0, 44]).all()
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """central differences of a scalar of the output in float64 arithmetic of the formula, at a few coordinates"""
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, _ = _inputs(1, 20, 24, 2, 1, 8, torch.float32, 2)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    grads = torch.autograd.grad(differential_attention(*leaves, causal=True), leaves, g)
+
+    def value(q, k, v, lam):
+        ok = _visible(1, 20, 24, True, None, None, None, DEV)[0]
+        total = 0.0
+        for h in range(2):
+            p = [torch.softmax((q[0, :, h, m] @ k[0, :, 0, m].T / math.sqrt(8)).masked_fill(~ok, -math.inf), -1) for m in range(2)]
+            total += (((p[0] - lam[h] * p[1]) @ v[0, :, 0]) * g[0, :, h].double()).sum()
+        return float(total)
+
+    base = [t.detach().double() for t in leaves]
+    for n, t in enumerate(base):
+        for at in (0, t.numel() // 3, t.numel() - 1):
+            for step in (1e-5,):
+                lo, hi = t.clone(), t.clone()
+                lo.view(-1)[at] -= step
+                hi.view(-1)[at] += step
+                diff = (value(*base[:n], hi, *base[n + 1:]) - value(*base[:n], lo, *base[n + 1:])) / (2 * step)
+                assert abs(diff - grads[n].reshape(-1)[at].item()) <= 1e-5 * (1 + abs(diff)), (n, at)
+
+
+@pytest.mark.gpu
+def test_empty_sizes_and_frozen_inputs():
+    from samble_amd.attention import differential_attention
+    for B, Nq, Nk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):
+        q, k, v, lam, _, _ = _inputs(B, Nq, Nk, 2, 1, 16, torch.bfloat16, 1)
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        out = differential_attention(*leaves)
+        assert out.shape == (B, Nq, 2, 32) and not out.any()
+        assert all(not t.any() for t in torch.autograd.grad(out.sum(), leaves))
+    q, k, v, lam, g, _ = _inputs(1, 9, 9, 2, 2, 16, torch.float32, 1)
+    both = torch.autograd.grad(differential_attention(q.requires_grad_(True), k, v.requires_grad_(True), lam), (q, v), g)
+    (only,) = torch.autograd.grad(differential_attention(q, k, v.detach(), lam), q, g)
+    assert torch.equal(both[0], only)
+
+
+@pytest.mark.gpu
+def test_other_stream_and_graph_replay():
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, gen = _inputs(2, 200, 200, 4, 2, 32, torch.bfloat16, 8)
+    tok = q[:, :1]
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+
+    def step():
+        out = differential_attention(*leaves, causal=True)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, g)
+
+    def serve():
+        with torch.no_grad():
+            return differential_attention(tok, long_k, long_v, lam, lengths=lengths)
+
+    long_k, long_v = (torch.randn(s, generator=gen, device=DEV).bfloat16() for s in ((2, 4000, 2, 2, 32), (2, 4000, 2, 64)))
+    lengths = torch.tensor([4000, 77], dtype=torch.int32, device=DEV)
+    eager, answer = step(), serve()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other, there = step(), serve()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(eager, other)) and torch.equal(answer, there)
+    graph, graph2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.cuda.graph(graph2):
+        held2 = serve()
+    for n in (3999, 1, 0, 2500):
+        with torch.no_grad():
+            q.copy_(torch.randn(q.shape, generator=gen, device=DEV))
+            lengths[0] = n
+        graph.replay()
+        graph2.replay()
+        eager, answer = step(), serve()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, held)) and torch.equal(answer, held2), n
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """a cache whose last item starts behind 2^31 elements"""
+    from samble_amd.attention import differential_attention
+    B, Nk, d = 3, 70000, 64
+    k = torch.empty((B, Nk, 64, 2, d), dtype=torch.bfloat16, device=DEV)      # 2^29 elements an item: 1.7e9 in all, with v 3.4e9 bytes each
+    v = torch.empty((B, Nk, 64, 2 * d), dtype=torch.bfloat16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    for t in (k, v):
+        t[2, :, 63] = torch.randn(t[2, :, 63].shape, generator=gen, device=DEV).bfloat16()
+        t[0, :, 0] = torch.randn(t[0, :, 0].shape, generator=gen, device=DEV).bfloat16()
+    big = torch.as_strided(k, (2, Nk, 2, 2, d), (2 * k.stride(0), k.stride(1), 63 * k.stride(2), d, 1))
+    bigv = torch.as_strided(v, (2, Nk, 2, 2 * d), (2 * v.stride(0), v.stride(1), 63 * v.stride(2), 1))
+    big[0, :, 1], big[1, :, 0], bigv[0, :, 1], bigv[1, :, 0] = 0.5, 0.25, 1.0, 2.0
+    q = torch.randn((2, 1, 2, 2, d), generator=gen, device=DEV).bfloat16()
+    lam = torch.tensor([0.3, 0.6], device=DEV)
+    out = differential_attention(q, big, bigv, lam)
+    copy = differential_attention(q, big.contiguous(), bigv.contiguous(), lam)
+    assert torch.equal(out, copy)
+    _check(q, big.contiguous(), bigv.contiguous(), lam, None, (out,), d ** -0.5, False, None, None, None)
+
+
+# ---- the layer ------------------------------------------------------------------------------------------------------------
+def _layer_config(C, H, ff):
+    from samble_amd.config import to_attr
+    one = lambda v: [v]  # noqa: E731
+    return to_attr(dict(q_in=one(C), q_out=one(C), k_in=one(C), k_out=one(C), v_in=one(C), v_out=one(C), num_heads=one(H),
+                        ff_conv1_channels_in=one(C), ff_conv1_channels_out=one(ff), ff_conv2_channels_in=one(ff),
+                        ff_conv2_channels_out=one(C)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H,ff,N", [(128, 4, 512, 257), (128, 1, 512, 100), (64, 2, 96, 65)])
+def test_layer_against_float64(C, H, ff, N):
+    """The whole layer, forward and every gradient, with ragged clouds.  Tolerance: the layer chains some ten fp32 stages of
+    at most 512-term sums on values of order one; 512 U = 3e-5 per stage, taken against the largest value of each tensor."""
+    from samble_amd.attention import DifferentialAttention
+    torch.manual_seed(C + H)
+    layer = DifferentialAttention(_layer_config(C, H, ff), 0).to(DEV)
+    with torch.no_grad():
+        for p in (layer.head_norm, layer.norm1, layer.norm2):
+            p.weight.add_(0.1 * torch.randn_like(p.weight))
+            p.bias.add_(0.1 * torch.randn_like(p.bias))
+    B, d = 3, C // (2 * H)
+    x = torch.randn(B, C, N, device=DEV, requires_grad=True)
+    lengths = torch.tensor([N, N // 2, N - 1], dtype=torch.int32, device=DEV)
+    g = torch.randn(B, C, N, device=DEV)
+    y = layer(x, lengths=lengths)
+    params = dict(layer.named_parameters())
+    got = torch.autograd.grad(y, [x, *params.values()], g)
+
+    w = {n: p.detach().double().requires_grad_(True) for n, p in params.items()}
+    xd = x.detach().double().requires_grad_(True)
+
+    def norm(t, name, dim):
+        r = t.movedim(dim, -1)
+        var, mean = torch.var_mean(r, -1, correction=0, keepdim=True)
+        return ((r - mean) / torch.sqrt(var + 1e-5) * w[name + ".weight"] + w[name + ".bias"]).movedim(-1, dim)
+
+    def conv(t, name):
+        return torch.matmul(w[name + ".weight"][:, :, 0], t)
+
+    q, k, v = (conv(xd, n).transpose(1, 2) for n in ("q_conv", "k_conv", "v_conv"))
+    lam = (torch.exp((w["lambda_q1"] * w["lambda_k1"]).sum(-1)) - torch.exp((w["lambda_q2"] * w["lambda_k2"]).sum(-1)) + layer.lambda_init)
+    ok = torch.arange(N, device=DEV) < lengths[:, None]
+    q, k = (t.reshape(B, N, H, 2, d).permute(0, 2, 3, 1, 4) for t in (q, k))
+    v = v.reshape(B, N, H, 2 * d).permute(0, 2, 1, 3)
+    p = torch.softmax((torch.matmul(q, k.transpose(-1, -2)) / math.sqrt(d)).masked_fill(~ok[:, None, None, None, :], -math.inf), -1)
+    o = torch.matmul(p[:, :, 0] - lam[None, :, None, None] * p[:, :, 1], v).transpose(1, 2)       # (B, N, H, 2d)
+    o = norm(o, "head_norm", -1) * (1 - layer.lambda_init)
+    z = norm(xd + o.reshape(B, N, C).transpose(1, 2), "norm1", 1)
+    ref = norm(z + conv(torch.nn.functional.leaky_relu(conv(z, "ff.0"), 0.2), "ff.2"), "norm2", 1)
+    want = torch.autograd.grad(ref, [xd, *w.values()], g.double())
+    for name, a, b in zip(["y", "x", *params], (y, *got), (ref, *want)):
+        err = ((a.double() - b).abs().max() / b.abs().max()).item()
+        assert err <= 10 * 512 * U, f"{name}: {err:.2e}"
+
+
+def test_layer_refusals():
+    from samble_amd.attention import DifferentialAttention
+    for C, H in ((128, 3), (128, 16), (256, 1)):
+        with pytest.raises(ValueError, match="DifferentialAttention"):
+            DifferentialAttention(_layer_config(C, H, 64), 0)
+    bad = _layer_config(128, 4, 512)
+    bad["v_out"] = [64]
+    with pytest.raises(ValueError, match="equal"):
+        DifferentialAttention(bad, 0)
+    layer = DifferentialAttention(_layer_config(128, 4, 512), 0)
+    with pytest.raises(_lib.SambleError, match="GPU"):
+        layer(torch.zeros(1, 128, 8))
+
+
+def test_refusals():
+    from samble_amd.attention import differential_attention
+    q, k, v, lam = torch.zeros(2, 3, 4, 2, 16), torch.zeros(2, 5, 2, 2, 16), torch.zeros(2, 5, 2, 32), torch.zeros(4)
+    good = dict(q=q, k=k, v=v, lam=lam)
+    bad = [dict(q=q[0]), dict(k=k.half()), dict(v=v[:, :4]), dict(v=v[..., :16]), dict(k=k[:, :, :, :1]), dict(q=q[:, :, :3]),
+           dict(q=q.double(), k=k.double(), v=v.double()), dict(lam=torch.zeros(3)), dict(lam=torch.zeros(4).half()),
+           dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+           dict(lengths=torch.zeros(3, dtype=torch.int32)), dict(lengths=torch.zeros(2)), dict(lengths=[5, 5]),
+           dict(q_start=torch.zeros(2, dtype=torch.int32)), dict(causal=True, q_start=torch.zeros(1, dtype=torch.int32)),
+           dict(key_mask=torch.ones(2, 5)), dict(key_mask=torch.ones(2, 4, dtype=torch.bool)),
+           dict(q=q[..., :12], k=k[..., :12], v=v[..., :24]), dict(q=q[..., :0], k=k[..., :0], v=v[..., :0]),
+           dict(q=torch.zeros(1, 1, 1, 2, 72), k=torch.zeros(1, 1, 1, 2, 72), v=torch.zeros(1, 1, 1, 144), lam=torch.zeros(1)),
+           dict(q=torch.zeros(1, 1, 1, 2, 136).half(), k=torch.zeros(1, 1, 1, 2, 136).half(), v=torch.zeros(1, 1, 1, 272).half(),
+                lam=torch.zeros(1))]
+    for change in bad:
+        with pytest.raises(ValueError, match="differential_attention"):
+            differential_attention(**{**good, **change})
+    with pytest.raises(_lib.SambleError, match="GPU"):
+        differential_attention(**good)
+
+
+def test_c_entries_refuse_bad_arguments():
+    import ctypes
+    ok = dict(type=2, lt=2, q=256, k=256, v=256, lam=256, shape=(1, 2, 3, 4, 2, 16),
+              st=(256, 128, 32, 16, 192, 64, 32, 16, 192, 64, 32, 0, 256, 128, 32), len=None, qs=None, km=None, causal=0, scale=0.25)
+
+    def call(name, tail, **change):
+        a = {**ok, **change}
+        args = [(ctypes.c_int64 * len(x))(*x) if isinstance(x, tuple) else x for x in a.values()]
+        _lib.call(name, *args, *tail)
+
+    fwd_tail = (256, None, None, None, 0, None)
+    bwd_tail = (256, 256, 256, 256, 256, 256, 256, 256, 256, 1 << 20, None)
+    bad = [dict(type=4), dict(type=2, lt=1), dict(q=None), dict(k=8), dict(v=257), dict(lam=None), dict(lam=257),
+           dict(shape=(0, 2, 3, 4, 2, 16)), dict(shape=(1, 2, 3, 4, 3, 16)), dict(shape=(1, 2, 3, 4, 2, 12)),
+           dict(shape=(1, 2, 3, 4, 2, 136)), dict(type=0, lt=0, shape=(1, 2, 3, 4, 2, 72)), dict(shape=(1, 2, 1 << 31, 4, 2, 16)),
+           dict(st=(256, 129) + ok["st"][2:]), dict(st=(-256,) + ok["st"][1:]), dict(scale=0.0), dict(scale=float("nan")), dict(qs=256)]
+    for change in bad:
+        for name, tail in (("samble_diff_attn_fwd", fwd_tail), ("samble_diff_attn_bwd", bwd_tail)):
+            with pytest.raises(_lib.SambleError, match=name):
+                call(name, tail, **change)
+    with pytest.raises(_lib.SambleError, match="out2 with lse"):
+        call("samble_diff_attn_fwd", (256, 256, None, None, 0, None))
+    with pytest.raises(_lib.SambleError, match="workspace"):
+        call("samble_diff_attn_bwd", bwd_tail[:-2] + (8, None))
+    with pytest.raises(_lib.SambleError, match="workspace"):
+        call("samble_diff_attn_fwd", fwd_tail, shape=(1, 1, 60000, 4, 2, 16))
+    assert _lib.query("samble_diff_attn_fwd_workspace_bytes", 2, (ctypes.c_int64 * 6)(1, 1, 60000, 4, 2, 16)) > 0
+    assert _lib.query("samble_diff_attn_fwd_workspace_bytes", 2, None) == 0
