@@ -534,8 +534,8 @@ Point2PointAttention._attention_in_torch = _p2p_attention_in_torch
 
 
 class _DiffAttn(torch.autograd.Function):
+    # (no autocast decorators: no torch arithmetic runs in either direction, the kernels take the types they are given)
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, q, k, v, lam, scale, causal, lengths, q_start, key_mask):
         out, out2, lse = ops.stage_diff_attn_fwd(q, k, v, lam, scale, causal, lengths, q_start, key_mask, for_backward=True)
         ctx.save_for_backward(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse)
@@ -544,7 +544,6 @@ class _DiffAttn(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    @torch.amp.custom_bwd(device_type="cuda")
     def backward(ctx, g):
         q, k, v, lam, lengths, q_start, key_mask, out, out2, lse = ctx.saved_tensors
         grads = ops.stage_diff_attn_bwd(q, k, v, lam, *ctx.cfg, lengths, q_start, key_mask, out, out2, lse, g.to(q.dtype))
@@ -612,7 +611,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     if B == 0 or Nq == 0 or Nk == 0:      # nothing to sum over: zeros that still hang on the inputs
         tie = q.sum() * 0 + k.sum() * 0 + v.sum() * 0 + lam.sum().to(q.dtype) * 0
         return torch.zeros((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device) + torch.nan_to_num(tie)
-    lam = lam.expand(H).contiguous()
+    if lam.shape != (H,) or lam.stride(0) != 1:
+        lam = lam.expand(H).contiguous()
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
         return _DiffAttn.apply(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)
     return ops.stage_diff_attn_fwd(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)[0]

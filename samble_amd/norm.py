@@ -11,12 +11,17 @@ from torch import nn
 
 from . import _lib
 from .ops import ELEMENT_TYPES as TYPES
-from .ops import _need_gpu, _p, _stream
+from .ops import _need_gpu, _on, _p
 
 
 def _slices(t: torch.Tensor, dim: int):
     """(outer, C, inner) view of t around axis `dim` -> (tensor, outer stride, channel stride); copied where the leading axes do
     not collapse into one stride, or the axes behind (rows: the axis itself) are not contiguous."""
+    if t.is_contiguous():
+        inner = 1
+        for n in t.shape[dim + 1:]:
+            inner *= n
+        return t, t.shape[dim] * inner, inner
     C = t.shape[dim]
     inner = 1
     for n in t.shape[dim + 1:]:
@@ -58,7 +63,7 @@ def stage_layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, dim: int, re
     (None unless `stats`)."""
     _need_gpu(x, weight, bias, residual)
     outer, C, inner = _extent(x, dim)
-    with torch.cuda.device(x.device):
+    with _on(x.device) as stream:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         s = torch.empty_like(y) if residual is not None else x
         n = outer * inner
@@ -68,7 +73,7 @@ def stage_layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, dim: int, re
             rv, r_os, r_cs = _slices(residual, dim) if residual is not None else (None, 0, 0)
             _lib.call("samble_layer_norm_fwd", TYPES[x.dtype], _weight_type(x, weight, bias), xv.data_ptr(), x_os, x_cs, _p(rv),
                       r_os, r_cs, _p(weight), _p(bias), outer, C, inner, float(eps), y.data_ptr(),
-                      _p(s) if residual is not None else None, _p(mean), _p(rstd), _stream())
+                      _p(s) if residual is not None else None, _p(mean), _p(rstd), stream)
     return y, s, mean, rstd
 
 
@@ -78,7 +83,7 @@ def stage_layer_norm_bwd(s: torch.Tensor, dy: torch.Tensor, weight, mean: torch.
     _need_gpu(s, dy, weight, mean, rstd, extra)
     outer, C, inner = _extent(s, dim)
     w_dtype = weight.dtype if weight is not None else (w_dtype or s.dtype)
-    with torch.cuda.device(s.device):
+    with _on(s.device) as stream:
         ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
         if outer * inner == 0:
             zero = lambda: torch.zeros(C, dtype=w_dtype, device=s.device) if want_weight_grads else None  # noqa: E731
@@ -91,13 +96,13 @@ def stage_layer_norm_bwd(s: torch.Tensor, dy: torch.Tensor, weight, mean: torch.
         ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device) if want_weight_grads else None
         _lib.call("samble_layer_norm_bwd", TYPES[s.dtype], TYPES[w_dtype], sv.data_ptr(), s_os, s_cs, gv.data_ptr(), g_os, g_cs,
                   _p(ev), e_os, e_cs, _p(weight), mean.data_ptr(), rstd.data_ptr(), outer, C, inner, ds.data_ptr(), _p(dw),
-                  _p(db), _p(ws), nbytes, _stream())
+                  _p(db), _p(ws), nbytes, stream)
     return ds, dw, db
 
 
 class _LayerNorm(torch.autograd.Function):
+    # (no autocast decorators: no torch arithmetic runs in either direction, the kernels take the types they are given)
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias, residual, eps, dim):
         y, s, mean, rstd = stage_layer_norm_fwd(x, weight, bias, eps, dim, residual)
         ctx.save_for_backward(s, weight, mean, rstd)
@@ -108,7 +113,6 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    @torch.amp.custom_bwd(device_type="cuda")
     def backward(ctx, dy, extra=None):
         s, weight, mean, rstd = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]

@@ -27,6 +27,27 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+class _on:
+    """`with _on(device) as stream`: device current (switched only where it is not), its current stream's handle -- the short
+    form of torch.cuda.device + current_stream for calls that take a few microseconds themselves."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, device):
+        self.index = device.index
+        self.guard = None
+
+    def __enter__(self):
+        if torch._C._cuda_getDevice() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
 def _need_gpu(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
@@ -407,28 +428,26 @@ def stage_attn_heads_bwd(qkv: torch.Tensor, heads: int, out: torch.Tensor, lse: 
 ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # include/samble.h SAMBLE_TYPE_*
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t with a contiguous last axis and every row on 16 bytes (a copy where it is not so)."""
+def _rows16(t: torch.Tensor):
+    """(t, its strides but the last; 0 for axes of one): every row on 16 bytes and contiguous, a copy where it is not so."""
     unit = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _strides(t: torch.Tensor):
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)]
+    for copy in (False, True):
+        if copy:
+            t = t.clone(memory_format=torch.contiguous_format)
+        st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+        last = st.pop()
+        if copy or (last == 1 and t.data_ptr() % 16 == 0 and not any([s % unit for s in st])):
+            return t, st
 
 
 def _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask):
-    """(tensors kept alive, leading arguments of samble_diff_attn_*, shape array, strides)"""
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    """(tensors kept alive, leading arguments of samble_diff_attn_*, shape array, strides, mask arguments)"""
+    (q, qs), (k, ks), (v, vs) = _rows16(q), _rows16(k), _rows16(v)
     B, Nq, H, _, d = q.shape
     shape = (ctypes.c_int64 * 6)(B, Nq, k.shape[1], H, k.shape[2], d)
-    strides = _strides(q) + _strides(k) + _strides(v) + [key_mask.stride(0) if key_mask is not None and B > 1 else 0]
+    strides = qs + ks + vs + [key_mask.stride(0) if key_mask is not None and B > 1 else 0]
     head = [ELEMENT_TYPES[q.dtype], ELEMENT_TYPES[lam.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), shape]
-    masks = [_p(lengths), _p(q_start), _p(key_mask)]
-    return (q, k, v), head, shape, strides, masks
+    return (q, k, v), head, shape, strides, [_p(lengths), _p(q_start), _p(key_mask)]
 
 
 def stage_diff_attn_fwd(q, k, v, lam, scale: float, causal: bool, lengths=None, q_start=None, key_mask=None, for_backward=False):
@@ -436,30 +455,30 @@ def stage_diff_attn_fwd(q, k, v, lam, scale: float, causal: bool, lengths=None, 
     out2 (the second map's output) and lse (B,H,2,Nq) are what the backward needs (None unless for_backward)."""
     _need_gpu(q, k, v, lam, lengths, q_start, key_mask)
     B, Nq, H, _, d = q.shape
-    with torch.cuda.device(q.device):
+    with _on(q.device) as stream:
         out = torch.empty((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device)
         out2 = torch.empty_like(out) if for_backward else None
         lse = torch.empty((B, H, 2, Nq), dtype=torch.float32, device=q.device) if for_backward else None
         keep, head, shape, strides, masks = _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask)
         nbytes = _lib.query("samble_diff_attn_fwd_workspace_bytes", head[0], shape)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _lib.call("samble_diff_attn_fwd", *head, (ctypes.c_int64 * 12)(*strides), *masks, int(causal), scale, out.data_ptr(),
-                  _p(out2), _p(lse), _p(ws), nbytes, _stream())
+        _lib.call("samble_diff_attn_fwd", *head, (ctypes.c_int64 * 12)(*strides), *masks, causal, scale, out.data_ptr(), _p(out2),
+                  _p(lse), _p(ws), nbytes, stream)
     return out, out2, lse
 
 
 def stage_diff_attn_bwd(q, k, v, lam, scale: float, causal: bool, lengths, q_start, key_mask, out, out2, lse, g):
     """-> (dq, dk, dv, dlam), contiguous, in the shapes and types of q, k, v, lam: csrc/diff_attn_bwd.hip."""
     _need_gpu(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, g)
-    with torch.cuda.device(q.device):
-        dq, dk, dv, dlam = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, lam))
+    with _on(q.device) as stream:
+        dq, dk, dv, dlam = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, lam)]
         keep, head, shape, strides, masks = _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask)
-        g = _rows16(g)
+        g, gs = _rows16(g)
         nbytes = _lib.query("samble_diff_attn_bwd_workspace_bytes", head[0], shape)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.call("samble_diff_attn_bwd", *head, (ctypes.c_int64 * 15)(*strides, *_strides(g)), *masks, int(causal), scale,
-                  out.data_ptr(), out2.data_ptr(), lse.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                  dlam.data_ptr(), ws.data_ptr(), nbytes, _stream())
+        _lib.call("samble_diff_attn_bwd", *head, (ctypes.c_int64 * 15)(*strides, *gs), *masks, causal, scale, out.data_ptr(),
+                  out2.data_ptr(), lse.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(),
+                  ws.data_ptr(), nbytes, stream)
     return dq, dk, dv, dlam
 
 
