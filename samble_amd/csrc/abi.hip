@@ -1453,7 +1453,8 @@ static bool diff_shape_ok(int type, const int64_t* n) {
   const int64_t most = (int64_t)1 << 30;
   for (int i = 0; i < 6; ++i)
     if (n[i] <= 0 || n[i] > most) return false;
-  return n[3] % n[4] == 0 && n[5] % 8 == 0 && n[5] <= (type == SAMBLE_TYPE_F32 ? 64 : 128) && n[0] <= (1 << 24) && n[3] <= (1 << 20);
+  return n[3] % n[4] == 0 && n[5] % 8 == 0 && n[5] <= (type == SAMBLE_TYPE_F32 ? 64 : 128) && n[0] <= (1 << 24) && n[3] <= (1 << 20) &&
+         n[1] * (n[3] / n[4]) <= most;      // rows of a key head
 }
 static bool rows16(int type, const void* p, const int64_t* strides, int n) {   // rows on 16 bytes
   const int64_t unit = type == SAMBLE_TYPE_F32 ? 4 : 8;

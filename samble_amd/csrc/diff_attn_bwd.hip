@@ -12,50 +12,53 @@
 
 namespace samble {
 
+// MW waves along the maps (each forms dA for itself): where both maps' operands and gradients would leave no registers for a
+// second wave on the SIMD
 template <typename T, int DP>
 struct DqCfg {
-  static constexpr int SUB = (DaT<T>::NP == 1 || DP <= 32) ? 2 : 1, KT = 32 * SUB;
-  typedef Tile<T, DP, KT> Tl;
+  static constexpr int MW = DP == 128 || (DaT<T>::NP == 3 && DP == 64) ? 2 : 1, MPW = 2 / MW, RW = 4, NW = RW * MW, NT = 64 * NW;
+  static constexpr int SUB = (DaT<T>::NP == 1 ? DP <= 64 : DP <= 32) ? 2 : 1, KT = 32 * SUB;
+  typedef Feed<T, DP, KT, NT> Fd;
   static constexpr int DT = DP < 32 ? 1 : DP / 32;     // 32-column pieces of a map's gradient (16 columns: both maps on one)
-  static constexpr int kLds = Tl::kBytes + KT / 8;
+  static constexpr int kLds = Fd::kLds;
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void diff_dq_kernel(DaArgs A) {
+__global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A) {
   typedef DqCfg<T, DP> Cfg;
-  typedef typename Cfg::Tl Tl;
-  constexpr int KS = DP / 16, DT = Cfg::DT, RW = 4;
+  typedef typename Cfg::Fd Fd;
+  typedef typename Fd::Tl Tl;
+  constexpr int KS = DP / 16, DT = Cfg::DT, RW = Cfg::RW, MPW = Cfg::MPW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  unsigned* words = reinterpret_cast<unsigned*>(smem + Tl::kBytes);
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-  const int rw = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const long rows = (long)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW), units = blocks * A.B * A.Hkv;
-  const long unit = da_unit(units);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, mw = wave / RW;
+  const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
+  const long units = (long)blocks * A.B * A.Hkv, unit = da_unit(units);
   if (unit >= units) return;
-  const long blk = blocks - 1 - unit % blocks;
+  const unsigned blk = blocks - 1 - (unsigned)(unit % blocks);
   const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
   const int len = da_len(A, b);
   const long start = da_start(A, b);
-  const long r = blk * 32 * RW + 32 * rw + (lane & 31);
+  const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
   const bool live = r < rows;
-  const int qi = live ? (int)(r / A.G) : 0, head = hk * A.G + (live ? (int)(r % A.G) : 0);
+  const int qi = live ? (int)(r / (unsigned)A.G) : 0, head = hk * A.G + (live ? (int)(r % (unsigned)A.G) : 0);
   const int limit = live ? da_limit(A, len, start, qi) : 0;
-  const long last = blk * 32 * RW + 32 * RW - 1;
-  const int kmax = da_limit(A, len, start, (int)((last < rows ? last : rows - 1) / A.G));
-  const long first = blk * 32 * RW + 32 * rw;
-  const int kmin = first + 31 < rows ? da_limit(A, len, start, (int)(first / A.G)) : 0;
+  const unsigned last = blk * 32 * RW + 32 * RW - 1;
+  const int kmax = da_limit(A, len, start, (int)((last < rows ? last : rows - 1) / (unsigned)A.G));
+  const int kmin = first + 31 < rows ? da_limit(A, len, start, (int)(first / (unsigned)A.G)) : 0;
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
 
-  const T* kb = (const T*)A.k + b * A.k_bs + hk * A.k_hs;
-  const T* vb = (const T*)A.v + b * A.v_bs + hk * A.v_hs;
-  const unsigned char* km = A.key_mask ? A.key_mask + b * A.km_bs : nullptr;
+  const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_rs, A.k_ms, A.v_rs,
+                        len, A.d, A.key_mask ? A.key_mask + b * A.km_bs : nullptr};
+  Fd feed(smem, tid);
+  if (tiles) feed.issue(keys, 0);
 
-  Frag<T> qf[2][KS], gf[2 * KS];
+  Frag<T> qf[MPW][KS], gf[2 * KS];
   {
-    const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs;
+    const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs + mw * A.q_ms;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MPW; ++m)
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int o = 16 * s + 8 * h;
@@ -65,7 +68,7 @@ __global__ __launch_bounds__(256, 1) void diff_dq_kernel(DaArgs A) {
       }
   }
   const float lam = da_lam<T>(A, head);
-  float t1 = 0.f, t2 = 0.f;
+  float dot[2] = {0.f, 0.f};      // t_1, t_2
   {
     const T* gp = (const T*)A.dout + b * A.g_bs + qi * A.g_rs + head * A.g_hs;
     const long at = (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
@@ -84,103 +87,85 @@ __global__ __launch_bounds__(256, 1) void diff_dq_kernel(DaArgs A) {
       o2.widen(w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        t1 = fmaf(g[e], u[e], t1);
-        t2 = fmaf(g[e], w[e], t2);
+        dot[0] = fmaf(g[e], u[e], dot[0]);
+        dot[1] = fmaf(g[e], w[e], dot[1]);
       }
     }
-    t1 = da_xor32_sum(t1);
-    t2 = da_xor32_sum(t2);
-    t1 = fmaf(lam, t2, t1);
+    dot[0] = da_xor32_sum(dot[0]);
+    dot[1] = da_xor32_sum(dot[1]);
+    dot[0] = fmaf(lam, dot[1], dot[0]);
   }
-  const float* ls = A.lse + ((long)b * A.H + head) * 2 * A.Nq + qi;
-  const float lse0 = live ? ls[0] : __builtin_huge_valf(), lse1 = live ? ls[A.Nq] : __builtin_huge_valf();
-  if (live && h == 0) {
-    float* dl = A.delta + ((long)b * A.H + head) * 2 * A.Nq + qi;
-    dl[0] = t1;
-    dl[A.Nq] = t2;
+  float lse[MPW], tm[MPW];
+#pragma unroll
+  for (int m = 0; m < MPW; ++m) {
+    const long at = (((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi;
+    lse[m] = live ? A.lse[at] : __builtin_huge_valf();
+    tm[m] = MPW == 2 ? dot[m] : mw ? dot[1] : dot[0];
+    if (live && h == 0) A.delta[at] = tm[m];
   }
 
-  f32x16 acc[2][DT];
+  f32x16 acc[MPW][DT];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MPW; ++m)
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[m][t] = zero16();
   const float c = A.scale * kLog2e;
 
-  Stage<T, DP, Cfg::KT, 256> st;
-  bool bit = false;
-  auto load_tile = [&](int t) {
-    const int k0 = t * Cfg::KT;
-    st.load(tid, A.d, A.k_ms, [&](int row, const T*& px, const T*& py) {
-      const long key = k0 + row;
-      const bool ok = key < len && (!km || km[key]);
-      px = kb + (ok ? key : 0) * A.k_rs;
-      py = vb + (ok ? key : 0) * A.v_rs;
-      return ok;
-    });
-    if (tid < Cfg::KT) bit = k0 + tid < len && (!km || km[k0 + tid]);
-  };
-  if (tiles) load_tile(0);
   for (int t = 0; t < tiles; ++t) {
-    __syncthreads();
-    st.store(smem, tid);
-    if (tid < Cfg::KT) {
-      const unsigned long long w = __ballot(bit);
-      if ((lane & 31) == 0) words[tid >> 5] = (unsigned)(w >> (lane & 32));
-    }
-    __syncthreads();
-    if (t + 1 < tiles) load_tile(t + 1);
+    const char* tile = feed.next();
+    if (t + 1 < tiles) feed.issue(keys, (t + 1) * Cfg::KT);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
       const int row0 = 32 * sub, k0 = t * Cfg::KT + row0;
       if (k0 >= kmax) continue;
-      f32x16 s[2] = {zero16(), zero16()}, da = zero16();
+      const unsigned word = Fd::word(tile, row0);
+      const bool masked = __builtin_amdgcn_readfirstlane(word) != 0xffffffffu || k0 + 32 > kmin;
+      f32x16 da = zero16();
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), gf[ks], da);
+      Frag<T> ds[MPW][2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[m] = da_mma<T>(Tl::rows(smem, 0, row0, m * KS + ks, lane), qf[m][ks], s[m]);
+      for (int m = 0; m < MPW; ++m) {
+        f32x16 s = zero16();
 #pragma unroll
-      for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(smem, 1, row0, ks, lane), gf[ks], da);
+        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(tile, 0, row0, (m + mw) * KS + ks, lane), qf[m][ks], s);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[0][e] = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, -lse0));
-        s[1][e] = __builtin_amdgcn_exp2f(fmaf(s[1][e], c, -lse1));
-      }
-      const unsigned word = words[row0 >> 5];
-      if (word != 0xffffffffu || k0 + 32 > kmin) {
-        const unsigned w = word >> (4 * h);
-        const int left = limit - k0 - 4 * h;
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse[m]));
+        if (masked) {
+          const unsigned w = word >> (4 * h);
+          const int left = limit - k0 - 4 * h;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int j = crow(e, 0);
-          const bool see = ((w >> j) & 1) && j < left;
-          s[0][e] = see ? s[0][e] : 0.f;
-          s[1][e] = see ? s[1][e] : 0.f;
+          for (int e = 0; e < 16; ++e) {
+            const int j = crow(e, 0);
+            s[e] = ((w >> j) & 1) && j < left ? s[e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e] * (da[8 * u + e] - tm[m]);
+          ds[m][u] = da_pack<T>(p);
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float d1[8], d2[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d1[e] = s[0][8 * u + e] * (da[8 * u + e] - t1);
-          d2[e] = -lam * s[1][8 * u + e] * (da[8 * u + e] - t2);
-        }
-        const Frag<T> f1 = da_pack<T>(d1), f2 = da_pack<T>(d2);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const Frag<T> k1 = Tl::cols(smem, 0, row0, u, 32 * dt, lane);
-          acc[0][dt] = da_mma<T>(k1, f1, acc[0][dt]);
-          const Frag<T> k2 = DP < 32 ? k1 : Tl::cols(smem, 0, row0, u, DP + 32 * dt, lane);
-          acc[1][dt] = da_mma<T>(k2, f2, acc[1][dt]);
+          Frag<T> kf;
+#pragma unroll
+          for (int m = 0; m < MPW; ++m) {
+            if (DP >= 32 || m == 0) kf = Tl::cols(tile, 0, row0, u, DP < 32 ? 0 : (m + mw) * DP + 32 * dt, lane);
+            acc[m][dt] = da_mma<T>(kf, ds[m][u], acc[m][dt]);
+          }
         }
-      }
     }
   }
   if (!live) return;
-  T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
+  T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d + mw * A.d;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MPW; ++m) {
+    const float f = A.scale * (m + mw ? -lam : 1.f);      // dS_2 = -lam P_2 (dA - t_2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -190,65 +175,107 @@ __global__ __launch_bounds__(256, 1) void diff_dq_kernel(DaArgs A) {
         typedef T vec __attribute__((ext_vector_type(4)));
         vec v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(A.scale * acc[m][dt][reg + e]);
+        for (int e = 0; e < 4; ++e) v[e] = (T)(f * acc[m][dt][reg + e]);
         *reinterpret_cast<vec*>(dq + m * A.d + col) = v;
       }
+  }
 }
 
-template <typename T, int DP>
+// KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  VL: the values, a stationary operand like
+// the keys, stay in LDS instead of registers (64-deep heads: room for a second wave on the SIMD; 128-deep: room at all).
+template <typename T, int DP, int KBW, int RWW>
 struct DkvCfg {
-  static constexpr int NW = DP == 128 ? 2 : 4;
-  static constexpr int SUB = (DaT<T>::NP == 1 || DP <= 32) ? (DP == 128 ? 1 : 2) : 1, RT = 32 * SUB;   // rows of a tile
-  typedef Tile<T, DP, RT> Tl;
+  static constexpr int NW = KBW * RWW, NT = 64 * NW, KB = 32 * KBW;
+  static constexpr bool VL = DaT<T>::NP == 1 && DP >= 64;
+  static constexpr int WPS = DP == 128 || (DaT<T>::NP == 3 && DP == 64) ? 1 : 2;      // waves per SIMD the registers allow
+  static constexpr int SUB = RWW == 1 && DP <= 32 ? 2 : 1, RT = 32 * RWW * SUB;       // rows of a tile
+  typedef Feed<T, DP, RT, NT> Fd;
+  typedef Tile<T, DP, KB> Vt;
   static constexpr int DT = DP < 32 ? 1 : DP / 32, DVT = 2 * DP / 32;
-  static constexpr int kLds = Tl::kBytes + 6 * RT * 4;
+  static constexpr int kStat = 6 * RT;       // lse_1, lse_2, t_1, t_2, limit (int), spare: floats per tile
+  static constexpr int kVal = VL ? Vt::kPlane : 0;
+  static constexpr int kState = (2 * DT + DVT) * 16 * 64;
+  static constexpr int kMerge = RWW > 1 ? kState * 4 * KBW : 0;      // one wave's sums per key block at a time
+  static constexpr int kBody = Fd::kLds + 2 * kStat * 4;
+  static constexpr int kLds = (kBody > kMerge ? kBody : kMerge) + kVal;
 };
 
-template <typename T, int DP>
-__global__ __launch_bounds__((DkvCfg<T, DP>::NW * 64), 1) void diff_dkv_kernel(DaArgs A, unsigned main_grid) {
-  typedef DkvCfg<T, DP> Cfg;
-  typedef typename Cfg::Tl Tl;
-  constexpr int KS = DP / 16, DT = Cfg::DT, DVT = Cfg::DVT, NW = Cfg::NW, NT = 64 * NW, RT = Cfg::RT;
+template <typename T, int DP, int KBW, int RWW>
+__global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, RWW>::WPS)) void diff_dkv_kernel(DaArgs A,
+                                                                                                               unsigned main_grid) {
+  typedef DkvCfg<T, DP, KBW, RWW> Cfg;
+  typedef typename Cfg::Fd Fd;
+  typedef typename Fd::Tl Tl;
+  constexpr int KS = DP / 16, DT = Cfg::DT, DVT = Cfg::DVT, NT = Cfg::NT, RT = Cfg::RT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* stat = reinterpret_cast<float*>(smem + Tl::kBytes);   // lse_1, lse_2, t_1, t_2, lam [RT], limit (int) [RT]
+  char* val = smem + Cfg::kLds - Cfg::kVal;
+  float* stats = reinterpret_cast<float*>(smem + Fd::kLds);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
 
   if (blockIdx.x >= main_grid) {      // dlam of one head: - sum of t_2 over batch and queries
     const int head = blockIdx.x - main_grid;
     float sum = 0.f;
-    const long n = (long)A.B * A.Nq;
-    for (long i = tid; i < n; i += NT) sum += A.delta[((i / A.Nq) * A.H + head) * 2 * A.Nq + A.Nq + i % A.Nq];
+    for (int bb = 0; bb < A.B; ++bb) {
+      const float* t2 = A.delta + (((long)bb * A.H + head) * 2 + 1) * A.Nq;
+      for (int i = tid; i < A.Nq; i += NT) sum += t2[i];
+    }
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) stat[tid >> 6] = sum;
+    if (lane == 0) stats[tid >> 6] = sum;
     __syncthreads();
     if (tid == 0) {
       sum = 0.f;
-      for (int w = 0; w < NW; ++w) sum += stat[w];
+      for (int w = 0; w < Cfg::NW; ++w) sum += stats[w];
       if (A.lam_f32) ((float*)A.dlam)[head] = -sum;
       else ((T*)A.dlam)[head] = (T)(-sum);
     }
     return;
   }
 
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const long rows = (long)A.Nq * A.G;
-  const long blocks = ((long)A.Nk + 32 * NW - 1) / (32 * NW), units = blocks * A.B * A.Hkv;
-  const long per = main_grid / 8, unit = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = wave % KBW, rww = wave / KBW;
+  const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
+  const long units = (long)blocks * A.B * A.Hkv;
+  const long unit = (long)(blockIdx.x & 7) * (main_grid / 8) + (blockIdx.x >> 3);
   if (unit >= units) return;
   const int blk = (int)(unit % blocks);           // (under a causal mask the keys that most rows see first)
   const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
   const int len = da_len(A, b);
   const long start = da_start(A, b);
-  const int key0 = blk * 32 * NW, kw0 = key0 + 32 * wave, key = kw0 + (lane & 31);
+  const int key0 = blk * Cfg::KB, kw0 = key0 + 32 * kb, key = kw0 + (lane & 31);
   const unsigned char* km = A.key_mask ? A.key_mask + b * A.km_bs : nullptr;
   const bool valid = key < len && (!km || km[key]);
   const bool all_valid = __all(valid);
 
-  Frag<T> kf[2][KS], vf[2 * KS];
+  // rows that see any key of the workgroup: all behind the first such query
+  const long i0 = A.causal && key0 > start ? key0 - start : 0;
+  const int per_head = (A.Nq + RT - 1) / RT;                            // tiles of a head
+  const int tile0 = key0 >= len || i0 >= A.Nq ? per_head : (int)(i0 / RT);
+  Rows<T> src = {nullptr, nullptr, A.q_rs, A.q_ms, A.g_rs, A.Nq, A.d, nullptr};
+  const T* qb = (const T*)A.q + b * A.q_bs + (long)hk * A.G * A.q_hs;
+  const T* gb = (const T*)A.dout + b * A.g_bs + (long)hk * A.G * A.g_hs;
+  Fd feed(smem, tid);
+  float sv[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  auto issue = [&](int g, int t) {
+    src.x = qb + g * A.q_hs;
+    src.y = gb + g * A.g_hs;
+    feed.issue(src, t * RT);
+    if (tid < RT) {
+      const int i = t * RT + tid;
+      const bool ok = i < A.Nq;
+      const long at = ((long)b * A.H + hk * A.G + g) * 2 * A.Nq + (ok ? i : 0);
+      sv[0] = ok ? A.lse[at] : __builtin_huge_valf();     // (rows behind the last: P = 0)
+      sv[1] = ok ? A.lse[at + A.Nq] : __builtin_huge_valf();
+      sv[2] = ok ? A.delta[at] : 0.f;
+      sv[3] = ok ? A.delta[at + A.Nq] : 0.f;
+      sv[4] = __int_as_float(ok ? da_limit(A, len, start, i) : 0);
+    }
+  };
+  if (tile0 < per_head) issue(0, tile0);
+
+  Frag<T> kf[2][KS], vf[Cfg::VL ? 1 : 2 * KS];
   {
     const T* kp = (const T*)A.k + b * A.k_bs + hk * A.k_hs + (long)(valid ? key : 0) * A.k_rs;
-    const T* vp = (const T*)A.v + b * A.v_bs + hk * A.v_hs + (long)(valid ? key : 0) * A.v_rs;
+    const T* vp = (const T*)A.v + b * A.v_bs + hk * A.v_hs;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -258,12 +285,21 @@ __global__ __launch_bounds__((DkvCfg<T, DP>::NW * 64), 1) void diff_dkv_kernel(D
         raw.load(kp + m * A.k_ms + o, valid && o < A.d);
         kf[m][s] = raw.frag();
       }
+    if constexpr (Cfg::VL) {
+      for (int e = tid; e < Cfg::KB * DP / 4; e += NT) {
+        const int row = e / (DP / 4), pc = e % (DP / 4), kk = key0 + row;
+        Raw8<T> raw;
+        raw.load(vp + kk * A.v_rs + pc * 8, kk < len && (!km || km[kk]) && pc * 8 < 2 * A.d);
+        *reinterpret_cast<vec8<typename Tl::E>*>(val + da_off<DP>(row, pc)) = raw.frag().p[0];
+      }
+    } else {
 #pragma unroll
-    for (int s = 0; s < 2 * KS; ++s) {
-      const int o = 16 * s + 8 * h;
-      Raw8<T> raw;
-      raw.load(vp + o, valid && o < 2 * A.d);
-      vf[s] = raw.frag();
+      for (int s = 0; s < 2 * KS; ++s) {
+        const int o = 16 * s + 8 * h;
+        Raw8<T> raw;
+        raw.load(vp + (long)(valid ? key : 0) * A.v_rs + o, valid && o < 2 * A.d);
+        vf[s] = raw.frag();
+      }
     }
   }
   f32x16 dk[2][DT], dv[DVT];
@@ -273,95 +309,113 @@ __global__ __launch_bounds__((DkvCfg<T, DP>::NW * 64), 1) void diff_dkv_kernel(D
   for (int t = 0; t < DVT; ++t) dv[t] = zero16();
   const float c = A.scale * kLog2e;
 
-  // rows that see any key of the workgroup: all behind the first such query
-  const long i0 = A.causal ? (key0 - start > 0 ? key0 - start : 0) : 0;
-  const long tiles = key0 >= len || i0 >= A.Nq ? 0 : (rows + RT - 1) / RT;
-  const long tile0 = tiles ? i0 * A.G / RT : 0;
-
-  Stage<T, DP, RT, NT> st;
-  float sv[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto load_tile = [&](long t) {
-    st.load(tid, A.d, A.q_ms, [&](int row, const T*& px, const T*& py) {
-      const long r = t * RT + row;
-      const bool ok = r < rows;
-      const long i = ok ? r / A.G : 0, hd = hk * A.G + (ok ? r % A.G : 0);
-      px = (const T*)A.q + b * A.q_bs + i * A.q_rs + hd * A.q_hs;
-      py = (const T*)A.dout + b * A.g_bs + i * A.g_rs + hd * A.g_hs;
-      return ok;
-    });
-    if (tid < RT) {
-      const long r = t * RT + tid;
-      const bool ok = r < rows;
-      const int i = ok ? (int)(r / A.G) : 0, hd = hk * A.G + (ok ? (int)(r % A.G) : 0);
-      const long at = ((long)b * A.H + hd) * 2 * A.Nq + i;
-      sv[0] = ok ? A.lse[at] : __builtin_huge_valf();     // (rows behind the last: P = 0)
-      sv[1] = ok ? A.lse[at + A.Nq] : __builtin_huge_valf();
-      sv[2] = ok ? A.delta[at] : 0.f;
-      sv[3] = ok ? A.delta[at + A.Nq] : 0.f;
-      sv[4] = da_lam<T>(A, hd);
-      sv[5] = __int_as_float(ok ? da_limit(A, len, start, i) : 0);
-    }
-  };
-  if (tile0 < tiles) load_tile(tile0);
-  for (long t = tile0; t < tiles; ++t) {
-    __syncthreads();
-    st.store(smem, tid);
-    if (tid < RT) {
+  int buf = 0;
+  for (int g = 0; g < A.G; ++g) {
+    const float lam = da_lam<T>(A, hk * A.G + g);
+    for (int t = tile0; t < per_head; ++t) {
+      float* stat = stats + buf * Cfg::kStat;
+      buf ^= 1;
+      if (tid < RT) {
 #pragma unroll
-      for (int e = 0; e < 6; ++e) stat[e * RT + tid] = sv[e];
-    }
-    __syncthreads();
-    if (t + 1 < tiles) load_tile(t + 1);
+        for (int e = 0; e < 5; ++e) stat[e * RT + tid] = sv[e];
+      }
+      const char* tile = feed.next();
+      if (t + 1 < per_head) issue(g, t + 1);
+      else if (g + 1 < A.G) issue(g + 1, tile0);
 #pragma unroll
-    for (int sub = 0; sub < Cfg::SUB; ++sub) {
-      const int row0 = 32 * sub;
-      f32x16 s[2] = {zero16(), zero16()}, da = zero16();
+      for (int sub = 0; sub < Cfg::SUB; ++sub) {
+        const int row0 = 32 * (rww + sub);
+        f32x16 da = zero16();
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+        for (int ks = 0; ks < 2 * KS; ++ks) {
+          if constexpr (Cfg::VL) da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), Cfg::Vt::rows(val, 0, 32 * kb, ks, lane), da);
+          else da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), vf[ks], da);
+        }
+        const int fewest = __builtin_amdgcn_readfirstlane(__float_as_int(stat[4 * RT + row0]));   // (limits rise with the row)
+        const bool masked = !all_valid || kw0 + 32 > fewest;
+        f32x16 p1;
+        Frag<T> f[2][2], af[2];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[m] = da_mma<T>(Tl::rows(smem, 0, row0, m * KS + ks, lane), kf[m][ks], s[m]);
+        for (int m = 0; m < 2; ++m) {
+          f32x16 s = zero16();
 #pragma unroll
-      for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(smem, 1, row0, ks, lane), vf[ks], da);
-      const int fewest = __builtin_amdgcn_readfirstlane(__float_as_int(stat[5 * RT + row0]));   // (limits rise with the row)
-      const bool masked = !all_valid || kw0 + 32 > fewest;
+          for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(tile, 0, row0, m * KS + ks, lane), kf[m][ks], s);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float a[8], d1[8], d2[8];
+          for (int u = 0; u < 2; ++u) {
+            float d[8], a[8];
 #pragma unroll
-        for (int q4 = 0; q4 < 2; ++q4) {
-          const int at = row0 + 16 * u + 8 * q4 + 4 * h;
-          const f32x4 l1 = *reinterpret_cast<const f32x4*>(stat + at), l2 = *reinterpret_cast<const f32x4*>(stat + RT + at);
-          const f32x4 t1 = *reinterpret_cast<const f32x4*>(stat + 2 * RT + at);
-          const f32x4 t2 = *reinterpret_cast<const f32x4*>(stat + 3 * RT + at);
-          const f32x4 lm = *reinterpret_cast<const f32x4*>(stat + 4 * RT + at);
-          const f32x4 lt = *reinterpret_cast<const f32x4*>(stat + 5 * RT + at);
+            for (int q4 = 0; q4 < 2; ++q4) {
+              const int at = row0 + 16 * u + 8 * q4 + 4 * h;
+              const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + m * RT + at);
+              const f32x4 tt = *reinterpret_cast<const f32x4*>(stat + (2 + m) * RT + at);
+              const f32x4 lt = *reinterpret_cast<const f32x4*>(stat + 4 * RT + at);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 8 * u + 4 * q4 + e;
-            float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], c, -l1[e])), p2 = __builtin_amdgcn_exp2f(fmaf(s[1][i], c, -l2[e]));
-            if (masked) {
-              const bool see = valid && key < __float_as_int(lt[e]);
-              p1 = see ? p1 : 0.f;
-              p2 = see ? p2 : 0.f;
+              for (int e = 0; e < 4; ++e) {
+                const int i = 8 * u + 4 * q4 + e;
+                float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ls[e]));
+                if (masked) p = valid && key < __float_as_int(lt[e]) ? p : 0.f;
+                if (m == 0) {
+                  p1[i] = p;
+                  d[4 * q4 + e] = p * (da[i] - tt[e]);
+                } else {
+                  p *= lam;
+                  a[4 * q4 + e] = p1[i] - p;
+                  d[4 * q4 + e] = p * (tt[e] - da[i]);
+                }
+              }
             }
-            p2 *= lm[e];
-            a[4 * q4 + e] = p1 - p2;
-            d1[4 * q4 + e] = p1 * (da[i] - t1[e]);
-            d2[4 * q4 + e] = -p2 * (da[i] - t2[e]);
+            f[m][u] = da_pack<T>(d);
+            if (m == 1) af[u] = da_pack<T>(a);
           }
         }
-        const Frag<T> af = da_pack<T>(a), f1 = da_pack<T>(d1), f2 = da_pack<T>(d2);
 #pragma unroll
-        for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(smem, 1, row0, u, 32 * dt, lane), af, dv[dt]);
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const Frag<T> q1 = Tl::cols(smem, 0, row0, u, 32 * dt, lane);
-          dk[0][dt] = da_mma<T>(q1, f1, dk[0][dt]);
-          const Frag<T> q2 = DP < 32 ? q1 : Tl::cols(smem, 0, row0, u, DP + 32 * dt, lane);
-          dk[1][dt] = da_mma<T>(q2, f2, dk[1][dt]);
+          for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(tile, 1, row0, u, 32 * dt, lane), af[u], dv[dt]);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            const Frag<T> q1 = Tl::cols(tile, 0, row0, u, 32 * dt, lane);
+            dk[0][dt] = da_mma<T>(q1, f[0][u], dk[0][dt]);
+            const Frag<T> q2 = DP < 32 ? q1 : Tl::cols(tile, 0, row0, u, DP + 32 * dt, lane);
+            dk[1][dt] = da_mma<T>(q2, f[1][u], dk[1][dt]);
+          }
         }
       }
     }
+  }
+  if constexpr (RWW > 1) {      // the waves along the rows: one after the other onto the first
+    float* w = reinterpret_cast<float*>(smem) + kb * Cfg::kState + lane;
+    for (int from = 1; from < RWW; ++from) {
+      __syncthreads();
+      if (rww == from) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            w[(dt * 16 + e) * 64] = dk[0][dt][e];
+            w[((DT + dt) * 16 + e) * 64] = dk[1][dt][e];
+          }
+#pragma unroll
+        for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[((2 * DT + dt) * 16 + e) * 64] = dv[dt][e];
+      }
+      __syncthreads();
+      if (rww == 0) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            dk[0][dt][e] += w[(dt * 16 + e) * 64];
+            dk[1][dt][e] += w[((DT + dt) * 16 + e) * 64];
+          }
+#pragma unroll
+        for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dv[dt][e] += w[((2 * DT + dt) * 16 + e) * 64];
+      }
+    }
+    if (rww) return;
   }
   if (key >= A.Nk) return;
   typedef T vec __attribute__((ext_vector_type(4)));
@@ -393,29 +447,39 @@ __global__ __launch_bounds__((DkvCfg<T, DP>::NW * 64), 1) void diff_dkv_kernel(D
     }
 }
 
+template <typename K>
+static int big_lds(K kernel, int bytes) {
+  if (bytes <= 64 * 1024) return 0;
+  return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int DP, int KBW, int RWW>
+static int dkv_go(const DaArgs& A, hipStream_t s) {
+  typedef DkvCfg<T, DP, KBW, RWW> K;
+  const long grid = (((long)A.Nk + K::KB - 1) / K::KB * A.B * A.Hkv + 7) / 8 * 8;
+  if ((grid + A.H) * K::NT >= (1ll << 32)) return -22;
+  if (const int rc = big_lds(diff_dkv_kernel<T, DP, KBW, RWW>, K::kLds)) return rc;
+  hipLaunchKernelGGL((diff_dkv_kernel<T, DP, KBW, RWW>), dim3((unsigned)(grid + A.H)), dim3(K::NT), K::kLds, s, A, (unsigned)grid);
+  return (int)hipGetLastError();
+}
+
+// Few key blocks (fewer than two workgroups of 128 keys per CU): half the keys, four waves along the rows
 template <typename T, int DP>
 static int bwd_go(const DaArgs& A, hipStream_t s) {
   typedef DqCfg<T, DP> Q;
-  typedef DkvCfg<T, DP> K;
   const long rows = (long)A.Nq * A.G, pairs = (long)A.B * A.Hkv;
-  const long gq = ((rows + 127) / 128 * pairs + 7) / 8 * 8;
-  const long gk = (((long)A.Nk + 32 * K::NW - 1) / (32 * K::NW) * pairs + 7) / 8 * 8;
-  if (gq * 256 >= (1ll << 32) || (gk + A.H) * 256 >= (1ll << 32)) return -22;
-  if (Q::kLds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(diff_dq_kernel<T, DP>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, Q::kLds);
-    if (e != hipSuccess) return (int)e;
-  }
-  if (K::kLds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(diff_dkv_kernel<T, DP>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, K::kLds);
-    if (e != hipSuccess) return (int)e;
-  }
-  hipLaunchKernelGGL((diff_dq_kernel<T, DP>), dim3((unsigned)gq), dim3(256), Q::kLds, s, A);
+  const long grid = ((rows + 127) / 128 * pairs + 7) / 8 * 8;
+  if (grid * Q::NT >= (1ll << 32)) return -22;
+  if (const int rc = big_lds(diff_dq_kernel<T, DP>, Q::kLds)) return rc;
+  hipLaunchKernelGGL((diff_dq_kernel<T, DP>), dim3((unsigned)grid), dim3(Q::NT), Q::kLds, s, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL((diff_dkv_kernel<T, DP>), dim3((unsigned)(gk + A.H)), dim3(64 * K::NW), K::kLds, s, A, (unsigned)gk);
-  return (int)hipGetLastError();
+  if constexpr (DP == 128 || (DaT<T>::NP == 3 && DP == 64)) {
+    return dkv_go<T, DP, 4, 1>(A, s);
+  } else {
+    const long blocks = ((long)A.Nk + 127) / 128 * pairs;
+    return blocks < 512 ? dkv_go<T, DP, 2, 4>(A, s) : dkv_go<T, DP, 4, 1>(A, s);
+  }
 }
 
 template <typename T>

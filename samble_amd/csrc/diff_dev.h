@@ -168,43 +168,132 @@ struct Tile {
   }
 };
 
-// one thread's pieces of a tile on their way from memory to LDS
+// sixteen zero bytes that pieces of rows which do not exist are copied from
+__device__ __attribute__((aligned(16))) const unsigned da_zero[4] = {0, 0, 0, 0};
+
+// rows r of the matrices X and Y, r in 0 .. n - 1 where mask (if any) is not 0; other rows are zero
+template <typename T>
+struct Rows {
+  const T *x, *y;
+  long x_rs, x_ms, y_rs;
+  int n, d;
+  const unsigned char* mask;
+};
+
+// Tiles on their way from memory to LDS, NT threads together.
+//   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), two tiles: while one is computed on, the next
+//   lands.  The 64 pieces of a wave's copy stand one behind the other in LDS, so the lane picks the piece that belongs there.
+//   fp32: through registers, where the values are split into planes; one tile.
+// use:  feed.issue(first, row0);  for each tile: { const char* t = feed.next();  [feed.issue(following, row0)];  compute }
+// next() is a barrier of the workgroup.
 template <typename T, int DP, int KT, int NT>
-struct Stage {
+struct Feed {
+  typedef Tile<T, DP, KT> Tl;
+  static constexpr bool DMA = Tl::NP == 1;
   static constexpr int kPieces = KT * DP / 4;                    // of X, and of Y
   static constexpr int kPer = (kPieces + NT - 1) / NT;
-  Raw8<T> x[kPer], y[kPer];
+  static constexpr int kTile = Tl::kBytes + 16 * ((KT / 8 + 15) / 16);   // the tile and its visible rows, a bit each
+  static constexpr int kLds = kTile * (DMA ? 2 : 1);
+  static_assert(!DMA || kPieces % 64 == 0, "whole waves copy");
+  static_assert(NT * 4 / DP % 8 == 0 || kPer == 1, "a thread's pieces stand at one place of their rows");
 
-  // row_of(row, px, py) sets the row's base pointers and says whether the row counts (otherwise zeros); d: live elements of a
-  // map, ms: stride between the maps of X
-  template <typename RowOf>
-  __device__ __forceinline__ void load(int tid, int d, long ms, RowOf row_of) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid + NT * i;
-      if (kPieces % NT && e >= kPieces) break;
-      const int row = e / (DP / 4), c = e % (DP / 4);
-      const T *px, *py;
-      const bool ok = row_of(row, px, py);
-      const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
-      x[i].load(px + map * ms + o, ok && o < d);
-      y[i].load(py + c * 8, ok && c * 8 < 2 * d);
+  char* lds;
+  int tid, wave, cur;       // cur: the buffer that next() returns
+  bool bit;
+  Raw8<T> x[DMA ? 1 : kPer], y[DMA ? 1 : kPer];
+
+  __device__ __forceinline__ Feed(char* l, int t) : lds(l), tid(t), wave(__builtin_amdgcn_readfirstlane(t >> 6)), cur(0), bit(false) {}
+
+  // piece e of a matrix of the tile -> its row and column piece
+  static __device__ __forceinline__ void place(int e, int& row, int& c) {
+    if constexpr (DP == 16) {
+      const int line = e >> 3, q = (e & 7) ^ (((line & 1) << 1) | ((line >> 1) & 1));
+      row = line * 2 + (q >> 2);
+      c = q & 3;
+    } else {
+      row = e / (DP / 4);
+      c = (e % (DP / 4)) ^ (((row & 3) << 1) | ((row >> 2) & 1));
     }
   }
-  __device__ __forceinline__ void store(char* lds, int tid) const {
-    typedef Tile<T, DP, KT> Tl;
+  static __device__ __forceinline__ void words(char* tile, int tid, bool bit) {
+    if (tid < KT) {
+      const unsigned long long w = __ballot(bit);
+      if ((tid & 31) == 0) reinterpret_cast<unsigned*>(tile + Tl::kBytes)[tid >> 5] = (unsigned)(w >> (tid & 32));
+    }
+  }
+  static __device__ __forceinline__ void copy16(const void* g, char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                     (__attribute__((address_space(3))) void*)l, 16, 0, 0);
+  }
+
+  __device__ __forceinline__ void issue(const Rows<T>& R, int row0) {
+    bit = tid < KT && row0 + tid < R.n && (!R.mask || R.mask[row0 + tid]);
+    if constexpr (DMA) {
+      char* tile = lds + (cur ^ 1) * kTile;
+      int row, c;
+      place(tid, row, c);
+      const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
+      const bool all = R.d == DP && row0 + KT <= R.n && !R.mask;      // uniform
+      const long xo = (long)row * R.x_rs + map * R.x_ms + o, yo = (long)row * R.y_rs + c * 8;
+      const T* xt = R.x + row0 * R.x_rs;
+      const T* yt = R.y + row0 * R.y_rs;
+      constexpr int kRows = NT * 4 / DP;       // rows between a thread's pieces
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid + NT * i;
-      if (kPieces % NT && e >= kPieces) break;
-      const int o = da_off<DP>(e / (DP / 4), e % (DP / 4));
-      const Frag<T> fx = x[i].frag(), fy = y[i].frag();
+      for (int i = 0; i < kPer; ++i) {
+        if (kPieces % NT && 64 * wave + NT * i >= kPieces) break;
+        char* l = tile + (64 * wave + NT * i) * 16;
+        const T *px = xt + xo + i * kRows * R.x_rs, *py = yt + yo + i * kRows * R.y_rs;
+        if (!all) {
+          const int r = row0 + row + i * kRows;
+          const bool ok = r < R.n && (!R.mask || R.mask[r]);
+          px = ok && o < R.d ? px : (const T*)da_zero;
+          py = ok && c * 8 < 2 * R.d ? py : (const T*)da_zero;
+        }
+        copy16(px, l);
+        copy16(py, l + Tl::kPlane);
+      }
+      words(tile, tid, bit);
+    } else {
 #pragma unroll
-      for (int p = 0; p < Tl::NP; ++p) {
-        *reinterpret_cast<vec8<typename Tl::E>*>(lds + p * Tl::kPlane + o) = fx.p[p];
-        *reinterpret_cast<vec8<typename Tl::E>*>(lds + (Tl::NP + p) * Tl::kPlane + o) = fy.p[p];
+      for (int i = 0; i < kPer; ++i) {
+        const int e = tid + NT * i;
+        if (kPieces % NT && e >= kPieces) break;
+        const int row = e / (DP / 4), c = e % (DP / 4);
+        const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
+        const long r = row0 + row;
+        const bool ok = r < R.n && (!R.mask || R.mask[r]);
+        x[i].load(R.x + r * R.x_rs + map * R.x_ms + o, ok && o < R.d);
+        y[i].load(R.y + r * R.y_rs + c * 8, ok && c * 8 < 2 * R.d);
       }
     }
+  }
+  // the tile issued last, in LDS for every wave; every wave is done with the tile before it
+  __device__ __forceinline__ const char* next() {
+    if constexpr (DMA) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      cur ^= 1;
+      return lds + cur * kTile;
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int e = tid + NT * i;
+        if (kPieces % NT && e >= kPieces) break;
+        const int o = da_off<DP>(e / (DP / 4), e % (DP / 4));
+        const Frag<T> fx = x[i].frag(), fy = y[i].frag();
+#pragma unroll
+        for (int p = 0; p < Tl::NP; ++p) {
+          *reinterpret_cast<vec8<typename Tl::E>*>(lds + p * Tl::kPlane + o) = fx.p[p];
+          *reinterpret_cast<vec8<typename Tl::E>*>(lds + (Tl::NP + p) * Tl::kPlane + o) = fy.p[p];
+        }
+      }
+      words(lds, tid, bit);
+      __syncthreads();
+      return lds;
+    }
+  }
+  static __device__ __forceinline__ unsigned word(const char* tile, int row0) {
+    return reinterpret_cast<const unsigned*>(tile + Tl::kBytes)[row0 >> 5];
   }
 };
 
