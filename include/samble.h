@@ -727,7 +727,8 @@ int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const
    type: SAMBLE_TYPE_* of q, k, v, out and the gradients; lam_type = type or F32 (lam, dlam).
      shape   (host) B, Nq, Nk, H, Hkv, d          H a multiple of Hkv; d a multiple of 8, at most 128 (fp32: 64)
      strides (host) q: batch, row, head, map; k: batch, row, head, map; v: batch, row, head; key_mask: batch; and for the
-                    backward dout: batch, row, head.  The last axes are contiguous; every row starts on 16 bytes
+                    backward dout: batch, row, head.  The last axes are contiguous; every row starts on 16 bytes; rows at
+                    most 2^23, maps at most 2^28 elements apart
      lengths (B) or null: item b has that many keys (taken into 0 .. Nk); key_mask (B, Nk) or null: 0 = the key does not exist
      causal          query i sees the keys up to position q_start[b] + i; q_start null: Nk - Nq
    A row that sees no key gives zeros and takes no part in the gradients.  Values of keys that do not exist are never used.

@@ -1460,6 +1460,8 @@ static bool rows16(int type, const void* p, const int64_t* strides, int n) {   /
   const int64_t unit = type == SAMBLE_TYPE_F32 ? 4 : 8;
   for (int i = 0; i < n; ++i)
     if (strides[i] % unit || strides[i] < 0) return false;
+  if (n >= 3 && strides[1] > 1 << 23) return false;               // rows of a tile within 32-bit offsets
+  if (n == 4 && strides[3] > 1 << 28) return false;               // and the two maps of a row
   return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
@@ -1482,7 +1484,7 @@ static int diff_args(const char* who, int type, int lam_type, const void* q, con
 }
 #define SAMBLE_DIFF_NEEDS                                                                                                   \
   ": needs a known type (lam: the same or fp32), positive sizes, H a multiple of Hkv, d a multiple of 8 up to 128 (fp32: 64), " \
-  "rows on 16 bytes, 0 < scale < 1e30, q_start with causal only"
+  "rows on 16 bytes and at most 2^23 elements apart (maps 2^28), 0 < scale < 1e30, q_start with causal only"
 
 SAMBLE_API size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* n) {
   return diff_shape_ok(type, n) ? samble_diff_fwd_ws_bytes(type, (int)n[0], (int)n[1], (int)n[2], (int)n[3], (int)n[4], (int)n[5]) : 0;
@@ -1509,7 +1511,7 @@ SAMBLE_API int samble_diff_attn_fwd(int type, int lam_type, const void* q, const
 }
 
 SAMBLE_API size_t samble_diff_attn_bwd_workspace_bytes(int type, const int64_t* n) {
-  return diff_shape_ok(type, n) ? (size_t)n[0] * n[3] * 2 * n[1] * sizeof(float) : 0;
+  return diff_shape_ok(type, n) ? (size_t)n[0] * n[3] * 3 * n[1] * sizeof(float) : 0;
 }
 
 SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,

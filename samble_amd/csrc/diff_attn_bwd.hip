@@ -16,8 +16,8 @@ namespace samble {
 // second wave on the SIMD
 template <typename T, int DP>
 struct DqCfg {
-  static constexpr int MW = DP == 128 || (DaT<T>::NP == 3 && DP == 64) ? 2 : 1, MPW = 2 / MW, RW = 4, NW = RW * MW, NT = 64 * NW;
-  static constexpr int SUB = (DaT<T>::NP == 1 ? DP <= 64 : DP <= 32) ? 2 : 1, KT = 32 * SUB;
+  static constexpr int MW = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 2 : 1, MPW = 2 / MW, RW = 4, NW = RW * MW, NT = 64 * NW;
+  static constexpr int SUB = DP <= 64 ? 2 : 1, KT = 32 * SUB;
   typedef Feed<T, DP, KT, NT> Fd;
   static constexpr int DT = DP < 32 ? 1 : DP / 32;     // 32-column pieces of a map's gradient (16 columns: both maps on one)
   static constexpr int kLds = Fd::kLds;
@@ -32,14 +32,14 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, mw = wave / RW;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, mw = Cfg::MW > 1 ? wave / RW : 0;
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = (long)blocks * A.B * A.Hkv, unit = da_unit(units);
   if (unit >= units) return;
   const unsigned blk = blocks - 1 - (unsigned)(unit % blocks);
   const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
   const int len = da_len(A, b);
-  const long start = da_start(A, b);
+  const int start = da_start(A, b);
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
   const bool live = r < rows;
   const int qi = live ? (int)(r / (unsigned)A.G) : 0, head = hk * A.G + (live ? (int)(r % (unsigned)A.G) : 0);
@@ -49,29 +49,25 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   const int kmin = first + 31 < rows ? da_limit(A, len, start, (int)(first / (unsigned)A.G)) : 0;
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
 
-  const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_rs, A.k_ms, A.v_rs,
+  const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_ms, (int)A.k_rs, (int)A.v_rs,
                         len, A.d, A.key_mask ? A.key_mask + b * A.km_bs : nullptr};
   Fd feed(smem, tid);
   if (tiles) feed.issue(keys, 0);
 
+  Lane<DP> L(lane, 0);
   Frag<T> qf[MPW][KS], gf[2 * KS];
+  float c[MPW], gscale;
   {
     const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs + mw * A.q_ms;
 #pragma unroll
-    for (int m = 0; m < MPW; ++m)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int o = 16 * s + 8 * h;
-        Raw8<T> raw;
-        raw.load(qp + m * A.q_ms + o, live && o < A.d);
-        qf[m][s] = raw.frag();
-      }
+    for (int m = 0; m < MPW; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
   }
   const float lam = da_lam<T>(A, head);
-  float dot[2] = {0.f, 0.f};      // t_1, t_2
+  float dot[2] = {0.f, 0.f}, norm = 0.f;      // t_1, t_2, |g|^2
   {
     const T* gp = (const T*)A.dout + b * A.g_bs + qi * A.g_rs + head * A.g_hs;
     const long at = (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
+    gscale = da_row<T, 2 * KS>(gp, 2 * A.d, live, h, gf);
 #pragma unroll
     for (int s = 0; s < 2 * KS; ++s) {
       const int o = 16 * s + 8 * h;
@@ -80,7 +76,6 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
       raw.load(gp + o, ok);
       o1.load((const T*)A.out + at + o, ok);
       o2.load((const T*)A.out2 + at + o, ok);
-      gf[s] = raw.frag();
       float g[8], u[8], w[8];
       raw.widen(g);
       o1.widen(u);
@@ -89,11 +84,13 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
       for (int e = 0; e < 8; ++e) {
         dot[0] = fmaf(g[e], u[e], dot[0]);
         dot[1] = fmaf(g[e], w[e], dot[1]);
+        norm = fmaf(g[e], g[e], norm);
       }
     }
     dot[0] = da_xor32_sum(dot[0]);
     dot[1] = da_xor32_sum(dot[1]);
     dot[0] = fmaf(lam, dot[1], dot[0]);
+    if (DaT<T>::NP == 2) norm = da_xor32_sum(norm);
   }
   float lse[MPW], tm[MPW];
 #pragma unroll
@@ -103,37 +100,77 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
     tm[m] = MPW == 2 ? dot[m] : mw ? dot[1] : dot[0];
     if (live && h == 0) A.delta[at] = tm[m];
   }
+  if (DaT<T>::NP == 2 && live && h == 0 && mw == 0)
+    A.delta[2l * A.B * A.H * A.Nq + ((long)b * A.H + head) * A.Nq + qi] = sqrtf(norm);
 
   f32x16 acc[MPW][DT];
 #pragma unroll
   for (int m = 0; m < MPW; ++m)
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[m][t] = zero16();
-  const float c = A.scale * kLog2e;
+  // fp32: the scale of dS (this lane's row: from the largest dA - t so far) and of the keys in the sums
+  float fscale = 1.f, kscale = 1.f;
+  unsigned fbits = 0;
+  if (DaT<T>::NP == 2) {
+    for (int m = 0; m < MPW; ++m) fbits = da_max_bits(fbits, tm[m]);
+    fscale = 0.5f * da_scale(fbits);
+  }
 
   for (int t = 0; t < tiles; ++t) {
-    const char* tile = feed.next();
+    feed.next(L);
+    if (DaT<T>::NP == 2 && kscale != feed.sx) {       // uniform, rare
+      const float f = t == 0 ? 1.f : feed.sx / kscale;
+      kscale = feed.sx;
+#pragma unroll
+      for (int m = 0; m < MPW; ++m)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[m][dt][e] *= f;
+    }
     if (t + 1 < tiles) feed.issue(keys, (t + 1) * Cfg::KT);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
       const int row0 = 32 * sub, k0 = t * Cfg::KT + row0;
       if (k0 >= kmax) continue;
-      const unsigned word = Fd::word(tile, row0);
+      const unsigned word = feed.word(row0);
       const bool masked = __builtin_amdgcn_readfirstlane(word) != 0xffffffffu || k0 + 32 > kmin;
       f32x16 da = zero16();
 #pragma unroll
-      for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), gf[ks], da);
+      for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(L, 1, row0, ks), gf[ks], da);
+      float a1 = 1.f;
+      if (DaT<T>::NP == 2) {
+        a1 = 1.f / gscale / feed.sy;
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(da[e]));
+        const unsigned now = __float_as_uint(xor32_max(top) * a1);
+        if (__any(now > (fbits | 0x007fffffu))) {     // a larger power of two than so far
+          fbits = max(fbits, now);
+          const float n = 0.5f * da_scale(fbits), f = n / fscale;
+          fscale = n;
+#pragma unroll
+          for (int m = 0; m < MPW; ++m)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[m][dt][e] *= f;
+        }
+        a1 *= fscale;
+      }
       Frag<T> ds[MPW][2];
 #pragma unroll
       for (int m = 0; m < MPW; ++m) {
         f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(tile, 0, row0, (m + mw) * KS + ks, lane), qf[m][ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, row0, (m + mw) * KS + ks), qf[m][ks], s);
+        const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse[m]));
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cm, -lse[m]));
         if (masked) {
-          const unsigned w = word >> (4 * h);
-          const int left = limit - k0 - 4 * h;
+          unsigned w = word >> (4 * h);
+          int left = limit - k0 - 4 * h;
+          asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every tile, in front of the branch)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int j = crow(e, 0);
@@ -144,7 +181,8 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
         for (int u = 0; u < 2; ++u) {
           float p[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e] * (da[8 * u + e] - tm[m]);
+          for (int e = 0; e < 8; ++e)
+            p[e] = s[8 * u + e] * (DaT<T>::NP == 2 ? fmaf(da[8 * u + e], a1, -tm[m] * fscale) : da[8 * u + e] - tm[m]);
           ds[m][u] = da_pack<T>(p);
         }
       }
@@ -155,7 +193,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
           Frag<T> kf;
 #pragma unroll
           for (int m = 0; m < MPW; ++m) {
-            if (DP >= 32 || m == 0) kf = Tl::cols(tile, 0, row0, u, DP < 32 ? 0 : (m + mw) * DP + 32 * dt, lane);
+            if (DP >= 32 || m == 0) kf = Tl::cols(L, 0, row0, u, DP < 32 ? 0 : (m + mw) * DP + 32 * dt);
             acc[m][dt] = da_mma<T>(kf, ds[m][u], acc[m][dt]);
           }
         }
@@ -165,7 +203,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d + mw * A.d;
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    const float f = A.scale * (m + mw ? -lam : 1.f);      // dS_2 = -lam P_2 (dA - t_2)
+    const float f = A.scale * (m + mw ? -lam : 1.f) / fscale / kscale;      // dS_2 = -lam P_2 (dA - t_2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -186,14 +224,14 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
 template <typename T, int DP, int KBW, int RWW>
 struct DkvCfg {
   static constexpr int NW = KBW * RWW, NT = 64 * NW, KB = 32 * KBW;
-  static constexpr bool VL = DaT<T>::NP == 1 && DP >= 64;
-  static constexpr int WPS = DP == 128 || (DaT<T>::NP == 3 && DP == 64) ? 1 : 2;      // waves per SIMD the registers allow
+  static constexpr bool VL = DP >= 64;
+  static constexpr int WPS = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 1 : 2;      // waves per SIMD the registers allow
   static constexpr int SUB = RWW == 1 && DP <= 32 ? 2 : 1, RT = 32 * RWW * SUB;       // rows of a tile
   typedef Feed<T, DP, RT, NT> Fd;
   typedef Tile<T, DP, KB> Vt;
   static constexpr int DT = DP < 32 ? 1 : DP / 32, DVT = 2 * DP / 32;
   static constexpr int kStat = 6 * RT;       // lse_1, lse_2, t_1, t_2, limit (int), spare: floats per tile
-  static constexpr int kVal = VL ? Vt::kPlane : 0;
+  static constexpr int kVal = VL ? DaT<T>::NP * Vt::kPlane : 0;
   static constexpr int kState = (2 * DT + DVT) * 16 * 64;
   static constexpr int kMerge = RWW > 1 ? kState * 4 * KBW : 0;      // one wave's sums per key block at a time
   static constexpr int kBody = Fd::kLds + 2 * kStat * 4;
@@ -232,7 +270,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     return;
   }
 
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = wave % KBW, rww = wave / KBW;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = wave % KBW, rww = RWW > 1 ? wave / KBW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
   const long units = (long)blocks * A.B * A.Hkv;
   const long unit = (long)(blockIdx.x & 7) * (main_grid / 8) + (blockIdx.x >> 3);
@@ -240,21 +278,22 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const int blk = (int)(unit % blocks);           // (under a causal mask the keys that most rows see first)
   const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
   const int len = da_len(A, b);
-  const long start = da_start(A, b);
+  const int start = da_start(A, b);
   const int key0 = blk * Cfg::KB, kw0 = key0 + 32 * kb, key = kw0 + (lane & 31);
   const unsigned char* km = A.key_mask ? A.key_mask + b * A.km_bs : nullptr;
   const bool valid = key < len && (!km || km[key]);
   const bool all_valid = __all(valid);
 
   // rows that see any key of the workgroup: all behind the first such query
-  const long i0 = A.causal && key0 > start ? key0 - start : 0;
+  const long i0 = A.causal && key0 > start ? (long)key0 - start : 0;
   const int per_head = (A.Nq + RT - 1) / RT;                            // tiles of a head
   const int tile0 = key0 >= len || i0 >= A.Nq ? per_head : (int)(i0 / RT);
-  Rows<T> src = {nullptr, nullptr, A.q_rs, A.q_ms, A.g_rs, A.Nq, A.d, nullptr};
+  Rows<T> src = {nullptr, nullptr, A.q_ms, (int)A.q_rs, (int)A.g_rs, A.Nq, A.d, nullptr};
   const T* qb = (const T*)A.q + b * A.q_bs + (long)hk * A.G * A.q_hs;
   const T* gb = (const T*)A.dout + b * A.g_bs + (long)hk * A.G * A.g_hs;
   Fd feed(smem, tid);
-  float sv[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
+  Lane<DP> L(lane, 32 * rww);
+  float sv[5] = {0.f, 0.f, 0.f, 0.f, 0.f}, gn = 0.f;
   auto issue = [&](int g, int t) {
     src.x = qb + g * A.q_hs;
     src.y = gb + g * A.g_hs;
@@ -262,35 +301,68 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     if (tid < RT) {
       const int i = t * RT + tid;
       const bool ok = i < A.Nq;
-      const long at = ((long)b * A.H + hk * A.G + g) * 2 * A.Nq + (ok ? i : 0);
-      sv[0] = ok ? A.lse[at] : __builtin_huge_valf();     // (rows behind the last: P = 0)
-      sv[1] = ok ? A.lse[at + A.Nq] : __builtin_huge_valf();
-      sv[2] = ok ? A.delta[at] : 0.f;
-      sv[3] = ok ? A.delta[at + A.Nq] : 0.f;
+      const long hd = (long)b * A.H + hk * A.G + g;
+      const float *ls = A.lse + hd * 2 * A.Nq, *tt = A.delta + hd * 2 * A.Nq;
+      sv[0] = ok ? ls[i] : __builtin_huge_valf();     // (rows behind the last: P = 0)
+      sv[1] = ok ? (ls + A.Nq)[i] : __builtin_huge_valf();
+      sv[2] = ok ? tt[i] : 0.f;
+      sv[3] = ok ? (tt + A.Nq)[i] : 0.f;
       sv[4] = __int_as_float(ok ? da_limit(A, len, start, i) : 0);
+      if (DaT<T>::NP == 2) gn = ok ? A.delta[2l * A.B * A.H * A.Nq + hd * A.Nq + i] : 0.f;
     }
   };
   if (tile0 < per_head) issue(0, tile0);
 
   Frag<T> kf[2][KS], vf[Cfg::VL ? 1 : 2 * KS];
+  float c[2], vscale = 1.f;     // logits' base-2 exponents per unit of the products; scale of this lane's values
+  // fp32: the largest |v_j| of the workgroup's keys; scale 2^kA of the probabilities, which leaves room for P_1 - lam P_2
+  float vnorm = 0.f;
+  int kA = 0;
   {
     const T* kp = (const T*)A.k + b * A.k_bs + hk * A.k_hs + (long)(valid ? key : 0) * A.k_rs;
     const T* vp = (const T*)A.v + b * A.v_bs + hk * A.v_hs;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(kp + m * A.k_ms, A.d, valid, h, kf[m]);
+    if constexpr (DaT<T>::NP == 2) {
+      unsigned bits = 0;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
+      for (int s = 0; s < 2 * KS; ++s) {
         const int o = 16 * s + 8 * h;
         Raw8<T> raw;
-        raw.load(kp + m * A.k_ms + o, valid && o < A.d);
-        kf[m][s] = raw.frag();
+        raw.load(vp + (long)(valid ? key : 0) * A.v_rs + o, valid && o < 2 * A.d);
+        float w[8];
+        raw.widen(w);
+        bits = raw.bits(bits);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vnorm = fmaf(w[e], w[e], vnorm);
       }
+      vnorm = wave_max64(sqrtf(da_xor32_sum(vnorm)));
+      bits = da_wave_max(bits);
+      float* red = stats;      // (the waves' maxima meet here before the first tile's statistics)
+      if (lane == 0) {
+        red[2 * wave] = vnorm;
+        red[2 * wave + 1] = __uint_as_float(bits);
+      }
+      __syncthreads();
+      for (int w = 0; w < Cfg::NW; ++w) {
+        vnorm = fmaxf(vnorm, red[2 * w]);
+        bits = max(bits, __float_as_uint(red[2 * w + 1]));
+      }
+      __syncthreads();
+      vscale = da_scale(__builtin_amdgcn_readfirstlane(bits));
+      float lm = 0.f;
+      for (int g = 0; g < A.G; ++g) lm = fmaxf(lm, fabsf(da_lam<T>(A, hk * A.G + g)));
+      kA = 13 - min(max((int)((__float_as_uint(1.f + lm) >> 23) & 255) - 127, 0), 100);
+    }
     if constexpr (Cfg::VL) {
       for (int e = tid; e < Cfg::KB * DP / 4; e += NT) {
         const int row = e / (DP / 4), pc = e % (DP / 4), kk = key0 + row;
         Raw8<T> raw;
-        raw.load(vp + kk * A.v_rs + pc * 8, kk < len && (!km || km[kk]) && pc * 8 < 2 * A.d);
-        *reinterpret_cast<vec8<typename Tl::E>*>(val + da_off<DP>(row, pc)) = raw.frag().p[0];
+        raw.load(vp + (long)kk * A.v_rs + pc * 8, kk < len && (!km || km[kk]) && pc * 8 < 2 * A.d);
+        const Frag<T> f = raw.frag(vscale);
+#pragma unroll
+        for (int p = 0; p < Tl::NP; ++p)
+          *reinterpret_cast<vec8<typename Tl::E>*>(val + p * Cfg::Vt::kPlane + da_off<DP>(row, pc)) = f.p[p];
       }
     } else {
 #pragma unroll
@@ -298,7 +370,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         const int o = 16 * s + 8 * h;
         Raw8<T> raw;
         raw.load(vp + (long)(valid ? key : 0) * A.v_rs + o, valid && o < 2 * A.d);
-        vf[s] = raw.frag();
+        vf[s] = raw.frag(vscale);
       }
     }
   }
@@ -307,29 +379,63 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   for (int t = 0; t < DT; ++t) dk[0][t] = dk[1][t] = zero16();
 #pragma unroll
   for (int t = 0; t < DVT; ++t) dv[t] = zero16();
-  const float c = A.scale * kLog2e;
+  // fp32: scale of dA - t (|dA| and |t| are at most |g| |v|), of the queries in dk's sums and of the gradients in dv's
+  float fscale = 1.f, qscale = 1.f, gscale = 1.f;
+  bool fresh = true;
 
-  int buf = 0;
-  for (int g = 0; g < A.G; ++g) {
+  int buf = 0, g = 0, t = tile0;
+  while (t < per_head) {
     const float lam = da_lam<T>(A, hk * A.G + g);
-    for (int t = tile0; t < per_head; ++t) {
-      float* stat = stats + buf * Cfg::kStat;
-      buf ^= 1;
+    float* stat = stats + buf * Cfg::kStat;
+    buf ^= 1;
+    feed.next(L, __float_as_uint(gn), [&] {
+      if (DaT<T>::NP == 2) {
+        const float f = 0.5f * da_scale(__float_as_uint(__uint_as_float(feed.uz) * vnorm));
+        sv[0] -= (float)kA;
+        sv[1] -= (float)kA;
+        const float u = f * 0x1p-14f;        // |dA - t| u <= 1
+        if (u != fscale || feed.sx != qscale || feed.sy != gscale) {      // uniform, rare
+          const float a = fresh ? 1.f : (u / fscale) * (feed.sx / qscale), z = fresh ? 1.f : feed.sy / gscale;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              dk[0][dt][e] *= a;
+              dk[1][dt][e] *= a;
+            }
+#pragma unroll
+          for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dv[dt][e] *= z;
+          fscale = u;
+          qscale = feed.sx;
+          gscale = feed.sy;
+          fresh = false;
+        }
+        sv[2] *= fscale;
+        sv[3] *= fscale;
+      }
       if (tid < RT) {
 #pragma unroll
         for (int e = 0; e < 5; ++e) stat[e * RT + tid] = sv[e];
       }
-      const char* tile = feed.next();
-      if (t + 1 < per_head) issue(g, t + 1);
-      else if (g + 1 < A.G) issue(g + 1, tile0);
+    });
+    // the tile behind this one
+    if (++t == per_head && ++g < A.G) t = tile0;
+    if (t < per_head) issue(g, t);
+    const float a1 = DaT<T>::NP == 2 ? fscale / vscale / feed.sy : 1.f;
 #pragma unroll
-      for (int sub = 0; sub < Cfg::SUB; ++sub) {
+    for (int sub = 0; sub < Cfg::SUB; ++sub) {
         const int row0 = 32 * (rww + sub);
         f32x16 da = zero16();
 #pragma unroll
         for (int ks = 0; ks < 2 * KS; ++ks) {
-          if constexpr (Cfg::VL) da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), Cfg::Vt::rows(val, 0, 32 * kb, ks, lane), da);
-          else da = da_mma<T>(Tl::rows(tile, 1, row0, ks, lane), vf[ks], da);
+          if constexpr (Cfg::VL) {
+            const unsigned at = (L.r[ks & 3] & (unsigned)(Tl::kBytes - 1)) + (unsigned)(Cfg::kLds - Cfg::kVal + (32 * kb - 32 * rww) * 4 * DP);
+            da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), Cfg::Vt::rows_at(at, 0, 0, ks), da);
+          } else {
+            da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), vf[ks], da);
+          }
         }
         const int fewest = __builtin_amdgcn_readfirstlane(__float_as_int(stat[4 * RT + row0]));   // (limits rise with the row)
         const bool masked = !all_valid || kw0 + 32 > fewest;
@@ -339,7 +445,18 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         for (int m = 0; m < 2; ++m) {
           f32x16 s = zero16();
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(tile, 0, row0, m * KS + ks, lane), kf[m][ks], s);
+          for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, 32 * sub, m * KS + ks), kf[m][ks], s);
+          const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
+          if (masked) {       // (what a row does not see: exp2 gives 0)
+            int mine = valid ? key : 0x7fffffff;
+            asm volatile("" : "+v"(mine));
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const f32x4 lt = *reinterpret_cast<const f32x4*>(stat + 4 * RT + row0 + 8 * q4 + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[4 * q4 + e] = mine < __float_as_int(lt[e]) ? s[4 * q4 + e] : kNegInf;
+            }
+          }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             float d[8], a[8];
@@ -348,19 +465,18 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
               const int at = row0 + 16 * u + 8 * q4 + 4 * h;
               const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + m * RT + at);
               const f32x4 tt = *reinterpret_cast<const f32x4*>(stat + (2 + m) * RT + at);
-              const f32x4 lt = *reinterpret_cast<const f32x4*>(stat + 4 * RT + at);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int i = 8 * u + 4 * q4 + e;
-                float p = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ls[e]));
-                if (masked) p = valid && key < __float_as_int(lt[e]) ? p : 0.f;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i], cm, -ls[e]));
+                const float dt = DaT<T>::NP == 2 ? fmaf(da[i], a1, -tt[e]) : da[i] - tt[e];
                 if (m == 0) {
-                  p1[i] = p;
-                  d[4 * q4 + e] = p * (da[i] - tt[e]);
+                  p1[i] = p0;
+                  d[4 * q4 + e] = p0 * dt;
                 } else {
-                  p *= lam;
+                  const float p = p0 * lam;
                   a[4 * q4 + e] = p1[i] - p;
-                  d[4 * q4 + e] = p * (tt[e] - da[i]);
+                  d[4 * q4 + e] = -p * dt;
                 }
               }
             }
@@ -371,18 +487,19 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
-          for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(tile, 1, row0, u, 32 * dt, lane), af[u], dv[dt]);
+          for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(L, 1, 32 * sub, u, 32 * dt), af[u], dv[dt]);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const Frag<T> q1 = Tl::cols(tile, 0, row0, u, 32 * dt, lane);
+            const Frag<T> q1 = Tl::cols(L, 0, 32 * sub, u, 32 * dt);
             dk[0][dt] = da_mma<T>(q1, f[0][u], dk[0][dt]);
-            const Frag<T> q2 = DP < 32 ? q1 : Tl::cols(tile, 0, row0, u, DP + 32 * dt, lane);
+            const Frag<T> q2 = DP < 32 ? q1 : Tl::cols(L, 0, 32 * sub, u, DP + 32 * dt);
             dk[1][dt] = da_mma<T>(q2, f[1][u], dk[1][dt]);
           }
         }
-      }
     }
   }
+  const float back = DaT<T>::NP == 2 ? __uint_as_float((unsigned)(127 - kA) << 23) : 1.f;      // 2^-kA
+  const float kback = A.scale * back / fscale / qscale, vback = back / gscale;
   if constexpr (RWW > 1) {      // the waves along the rows: one after the other onto the first
     float* w = reinterpret_cast<float*>(smem) + kb * Cfg::kState + lane;
     for (int from = 1; from < RWW; ++from) {
@@ -431,7 +548,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         if (col >= A.d) continue;
         vec v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(A.scale * dk[m][dt][reg + e]);
+        for (int e = 0; e < 4; ++e) v[e] = (T)(kback * dk[m][dt][reg + e]);
         *reinterpret_cast<vec*>(dkp + m * A.d + col) = v;
       }
 #pragma unroll
@@ -442,7 +559,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       if (col >= 2 * A.d) continue;
       vec v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)dv[dt][4 * q4 + e];
+      for (int e = 0; e < 4; ++e) v[e] = (T)(vback * dv[dt][4 * q4 + e]);
       *reinterpret_cast<vec*>(dvp + col) = v;
     }
 }
@@ -474,7 +591,7 @@ static int bwd_go(const DaArgs& A, hipStream_t s) {
   hipLaunchKernelGGL((diff_dq_kernel<T, DP>), dim3((unsigned)grid), dim3(Q::NT), Q::kLds, s, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if constexpr (DP == 128 || (DaT<T>::NP == 3 && DP == 64)) {
+  if constexpr (DP == 128 || (DaT<T>::NP == 2 && DP == 64)) {
     return dkv_go<T, DP, 4, 1>(A, s);
   } else {
     const long blocks = ((long)A.Nk + 127) / 128 * pairs;

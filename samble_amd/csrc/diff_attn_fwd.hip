@@ -16,7 +16,7 @@ namespace samble {
 template <typename T, int DP, int RW, int KW, int MW>
 struct FwdCfg {
   static constexpr int NW = RW * KW * MW, NT = 64 * NW;
-  static constexpr int SUB = KW > 1 ? 1 : (DaT<T>::NP == 1 ? DP <= 64 : DP <= 32) ? 2 : 1;   // 32-key steps of a wave per tile
+  static constexpr int SUB = KW > 1 ? 1 : DP <= 64 ? 2 : 1;   // 32-key steps of a wave per tile
   static constexpr int KT = 32 * KW * SUB;
   static constexpr int DVT = 2 * DP / 32, MPW = 2 / MW;      // 32-column pieces of an output, maps of a wave
   typedef Feed<T, DP, KT, NT> Fd;
@@ -32,7 +32,9 @@ template <typename T, int DP> struct FwdWaves { static constexpr int value = 2; 
 // partial results of a split: per row (row order of the pair) m_1, l_1, m_2, l_2, then O_1, O_2 (2 d each)
 __device__ __forceinline__ long da_part_floats(int d) { return 4 + 4l * d; }
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }   // (0 for a row without keys, NaN stays)
-__device__ __forceinline__ float da_lse(float m, float l) { return l == 0.f ? __builtin_huge_valf() : m + __builtin_amdgcn_logf(l); }
+__device__ __forceinline__ float da_lse(float m, float l, int shift) {      // log2 of the row's sum
+  return l == 0.f ? __builtin_huge_valf() : m - (float)shift + __builtin_amdgcn_logf(l);
+}
 
 template <typename T, int DP, int RW, int KW, int MW>
 __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void diff_fwd_kernel(DaArgs A) {
@@ -44,7 +46,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rw = wave % RW, kw = (wave / RW) % KW, mw = wave / (RW * KW);
+  const int rw = wave % RW, kw = KW > 1 ? (wave / RW) % KW : 0, mw = MW > 1 ? wave / (RW * KW) : 0;
   const unsigned rows = (unsigned)A.Nq * A.G;
   const unsigned blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = (long)blocks * A.splits * A.B * A.Hkv;
@@ -55,7 +57,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   const int pair = (int)(rest / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
 
   const int len = da_len(A, b);
-  const long start = da_start(A, b);
+  const int start = da_start(A, b);
   // this lane's row
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
   const bool live = r < rows;
@@ -69,23 +71,18 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
   const int t0 = (int)((long)tiles * split / A.splits), t1 = (int)((long)tiles * (split + 1) / A.splits);
 
-  const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_rs, A.k_ms, A.v_rs,
+  const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_ms, (int)A.k_rs, (int)A.v_rs,
                         len, A.d, A.key_mask ? A.key_mask + b * A.km_bs : nullptr};
   Fd feed(smem, tid);
   if (t0 < t1) feed.issue(keys, t0 * Cfg::KT);
 
+  Lane<DP> L(lane, 32 * kw);
   Frag<T> qf[MPW][KS];
+  float c[MPW];             // logits' base-2 exponents per unit of the products
   {
     const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs + mw * A.q_ms;
 #pragma unroll
-    for (int m = 0; m < MPW; ++m)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int o = 16 * s + 8 * h;
-        Raw8<T> raw;
-        raw.load(qp + m * A.q_ms + o, live && o < A.d);
-        qf[m][s] = raw.frag();
-      }
+    for (int m = 0; m < MPW; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
   }
 
   f32x16 o[MPW][DVT];
@@ -97,26 +94,37 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
 #pragma unroll
     for (int t = 0; t < DVT; ++t) o[m][t] = zero16();
   }
-  const float c = A.scale * kLog2e;
+  float vscale = 1.f;       // scale of the outputs' sums (fp32: the values')
 
   for (int t = t0; t < t1; ++t) {
-    const char* tile = feed.next();
+    feed.next(L);
+    if (DaT<T>::NP == 2 && vscale != feed.sy) {       // uniform, rare
+      const float f = t == t0 ? 1.f : feed.sy / vscale;
+      vscale = feed.sy;
+#pragma unroll
+      for (int m = 0; m < MPW; ++m)
+#pragma unroll
+        for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[m][dt][e] *= f;
+    }
     if (t + 1 < t1) feed.issue(keys, (t + 1) * Cfg::KT);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
       const int row0 = 32 * (kw + sub), k0 = t * Cfg::KT + row0;
       if (k0 >= kmax) continue;   // (uniform; nothing of it is seen)
-      const unsigned word = Fd::word(tile, row0);
+      const unsigned word = feed.word(row0);
       const bool masked = __builtin_amdgcn_readfirstlane(word) != 0xffffffffu || k0 + 32 > kmin;
       Frag<T> pf[MPW][2];
 #pragma unroll
       for (int m = 0; m < MPW; ++m) {
         f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(tile, 0, row0, (m + mw) * KS + ks, lane), qf[m][ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, 32 * sub, (m + mw) * KS + ks), qf[m][ks], s);
         if (masked) {
-          const unsigned w = word >> (4 * h);
-          const int left = limit - k0 - 4 * h;
+          unsigned w = word >> (4 * h);
+          int left = limit - k0 - 4 * h;
+          asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every tile, in front of the branch)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int j = crow(e, 0);
@@ -126,7 +134,8 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        top = xor32_max(top) * c;
+        const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
+        top = xor32_max(top) * cm;
         // the reference of the exponentials follows the maximum only when that has grown by more than 8 (a factor of 256 in
         // the sums): any reference gives the same quotients, and the outputs are rescaled in few of the steps
         if (__any(top > mx[m] + 8.f)) {
@@ -139,13 +148,13 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
             for (int e = 0; e < 16; ++e) o[m][dt][e] *= al;
           mx[m] = nm;
         }
-        const float ref = mx[m] == kNegInf ? 0.f : mx[m];
+        const float ref = (mx[m] == kNegInf ? 0.f : mx[m]) - (float)DaT<T>::kP;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float p[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + e], c, -ref));
+            p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + e], cm, -ref));
             l[m] += p[e];
           }
           pf[m][u] = da_pack<T>(p);
@@ -155,7 +164,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
       for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const Frag<T> vf = Tl::cols(tile, 1, row0, u, 32 * dt, lane);
+          const Frag<T> vf = Tl::cols(L, 1, 32 * sub, u, 32 * dt);
 #pragma unroll
           for (int m = 0; m < MPW; ++m) o[m][dt] = da_mma<T>(vf, pf[m][u], o[m][dt]);
         }
@@ -201,6 +210,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
     }
   }
 
+  if (DaT<T>::NP == 2) vscale = 1.f / vscale;
   if (A.splits > 1) {
     if (kw || !live) return;
     float* w = A.part + (((long)split * A.B * A.Hkv + pair) * rows + r) * da_part_floats(A.d);
@@ -216,7 +226,8 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
         for (int q4 = 0; q4 < 4; ++q4) {
           const int col = 32 * dt + 8 * q4 + 4 * h;
           if (col < 2 * A.d) {
-            const f32x4 v = {o[m][dt][4 * q4], o[m][dt][4 * q4 + 1], o[m][dt][4 * q4 + 2], o[m][dt][4 * q4 + 3]};
+            f32x4 v = {o[m][dt][4 * q4], o[m][dt][4 * q4 + 1], o[m][dt][4 * q4 + 2], o[m][dt][4 * q4 + 3]};
+            if (DaT<T>::NP == 2) v *= vscale;
             *reinterpret_cast<f32x4*>(w + 4 + 2 * (m + mw) * A.d + col) = v;
           }
         }
@@ -225,12 +236,12 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   }
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    const float inv = da_inv(l[m]);
+    const float inv = da_inv(l[m]) * (DaT<T>::NP == 2 ? vscale : 1.f);
 #pragma unroll
     for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[m][dt][e] *= inv;
-    if (A.lse && live && kw == 0 && h == 0) A.lse[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = da_lse(mx[m], l[m]);
+    if (A.lse && live && kw == 0 && h == 0) A.lse[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = da_lse(mx[m], l[m], DaT<T>::kP);
   }
   const float* f = reinterpret_cast<const float*>(smem) + rw * DVT * 16 * 64 + lane;   // two waves: the second map's output
   if constexpr (MW > 1) {
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DaArgs A) {
     for (int k = 0; k < 2; ++k) {
       l[k] = (red[0][k][256] + red[1][k][256]) + (red[2][k][256] + red[3][k][256]);
       v[k] = ((red[0][k][c] + red[1][k][c]) + (red[2][k][c] + red[3][k][c])) * da_inv(l[k]);
-      if (A.lse && c == 0) A.lse[(((long)b * A.H + head) * 2 + k) * A.Nq + qi] = da_lse(m[k], l[k]);
+      if (A.lse && c == 0) A.lse[(((long)b * A.H + head) * 2 + k) * A.Nq + qi] = da_lse(m[k], l[k], DaT<T>::kP);
     }
     if (c < cols) {
       const long o = (((long)b * A.Nq + qi) * A.H + head) * cols + c;
@@ -373,7 +384,7 @@ template <typename T>
 static int fwd_type(DaArgs& A, hipStream_t s) {
   const FwdPlan p = fwd_plan(A.B, A.Nq, A.Nk, A.H, A.Hkv);
   A.splits = p.splits;
-  constexpr bool F = DaT<T>::NP == 3;
+  constexpr bool F = DaT<T>::NP == 2;
   int rc = -22;
   if (A.d <= 16) rc = p.few ? fwd_go<T, 16, 1, 4, 1>(A, s) : fwd_go<T, 16, 4, 1, 1>(A, s);
   else if (A.d <= 32) rc = p.few ? fwd_go<T, 32, 1, 4, 1>(A, s) : fwd_go<T, 32, 4, 1, 1>(A, s);

@@ -7,8 +7,11 @@
 // gradients are ordinary sums over rows.
 //
 // Products.  v_mfma_f32_32x32x16 on fp16 or bf16 operands, fp32 sums.  fp16 / bf16 tensors are operands as they are; an fp32
-// tensor is split into three bf16 planes (x = h + m + l, 24 bits; bf16 has fp32's range, so no scale is needed) and a product
-// takes the six partial products down to 2^-16 of the first: the error of an fp32 product.  Lane l holds
+// tensor is split into two fp16 planes of its scaled values (x s = h + l, 22 bits) and a product takes three partial products.
+// The scales are powers of two: one per row where a row is a lane's own, one for the whole tile (the largest value so far over
+// a workgroup's tiles) where rows stream through LDS; sums are rescaled in the few steps where that one changes.  What is 2^15
+// below the largest value of the tiles loses bits below 2^-37 of that value.
+// Lane l holds
 //     A: A[row = l & 31][k = 8 (l >> 5) + e],  B: B[k = 8 (l >> 5) + e][col = l & 31],  e = 0 .. 7
 //     D: register r: D[row = crow(r, l >> 5)][col = l & 31]
 // The reduced index of a second product stands on the first one's ROW axis: registers 8 t .. 8 t + 7 of a softmax tile are
@@ -32,13 +35,15 @@ typedef __bf16 bf16;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-template <typename T> struct DaT;
-template <> struct DaT<float> { typedef bf16 E; static constexpr int NP = 3; };
-template <> struct DaT<f16> { typedef f16 E; static constexpr int NP = 1; };
-template <> struct DaT<bf16> { typedef bf16 E; static constexpr int NP = 1; };
+template <typename T> struct DaT;      // operand type, planes; kP: the probabilities' scale 2^kP (fp16 operands: off the subnormals)
+template <> struct DaT<float> { typedef f16 E; static constexpr int NP = 2, kP = 6; };
+template <> struct DaT<f16> { typedef f16 E; static constexpr int NP = 1, kP = 6; };
+template <> struct DaT<bf16> { typedef bf16 E; static constexpr int NP = 1, kP = 0; };
 
 template <typename E> using vec8 = E __attribute__((ext_vector_type(8)));
 template <typename E> using vec4 = E __attribute__((ext_vector_type(4)));
+template <typename E> using vec2 = E __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16 da_mfma(vec8<bf16> a, vec8<bf16> b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -55,9 +60,6 @@ __device__ __forceinline__ f32x16 da_mma(const Frag<T>& a, const Frag<T>& b, f32
   if constexpr (DaT<T>::NP == 1) {
     return da_mfma(a.p[0], b.p[0], c);
   } else {   // the small products first
-    c = da_mfma(a.p[2], b.p[0], c);
-    c = da_mfma(a.p[0], b.p[2], c);
-    c = da_mfma(a.p[1], b.p[1], c);
     c = da_mfma(a.p[1], b.p[0], c);
     c = da_mfma(a.p[0], b.p[1], c);
     return da_mfma(a.p[0], b.p[0], c);
@@ -65,28 +67,40 @@ __device__ __forceinline__ f32x16 da_mma(const Frag<T>& a, const Frag<T>& b, f32
 }
 
 // eight fp32 values as an operand.  fp16 / bf16: one rounding to the tensors' own type (half a step of the value; the sums
-// that these factors enter stay in fp32); fp32: three planes, no bit lost.
+// that these factors enter stay in fp32); fp32 (values scaled into fp16's range): two planes, 22 bits.
 template <typename T>
 __device__ __forceinline__ Frag<T> da_pack(const float (&v)[8]) {
   typedef typename DaT<T>::E E;
   Frag<T> f;
-  if constexpr (DaT<T>::NP == 1) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.p[0][e] = (E)v[e];
-  } else {
-    float r[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f.p[0][e] = (E)v[e];
-      r[e] = v[e] - (float)f.p[0][e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f.p[1][e] = (E)r[e];
-      f.p[2][e] = (E)(r[e] - (float)f.p[1][e]);
+  for (int e = 0; e < 8; e += 2) {
+    const f32x2 x = {v[e], v[e + 1]};
+    const vec2<E> h = __builtin_convertvector(x, vec2<E>);
+    f.p[0][e] = h[0];
+    f.p[0][e + 1] = h[1];
+    if constexpr (DaT<T>::NP == 2) {
+      const f32x2 r = {fmaf((float)h[0], -1.f, v[e]), fmaf((float)h[1], -1.f, v[e + 1])};
+      const vec2<E> l = __builtin_convertvector(r, vec2<E>);
+      f.p[1][e] = l[0];
+      f.p[1][e + 1] = l[1];
     }
   }
   return f;
+}
+
+// the power of two that takes a value with these absolute bits to 2^13 .. 2^14 (0: left alone as far as it goes; infinities
+// and NaN stay what they are)
+__device__ __forceinline__ float da_scale(unsigned abs_bits) {
+  const unsigned e = max(abs_bits >> 23, 14u);
+  return __uint_as_float((267u - e) << 23);
+}
+// c / scale, never 0: what is masked stands for minus infinity times it
+__device__ __forceinline__ float da_per(float c, float scale) { return fmaxf(c / scale, 0x1p-126f); }
+__device__ __forceinline__ unsigned da_max_bits(unsigned a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
+__device__ __forceinline__ unsigned da_wave_max(unsigned x) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, o, 64));
+  return x;
 }
 
 // eight contiguous values of a tensor, as they are read (held across a tile's computation); ok = false: zeros
@@ -98,13 +112,18 @@ template <> struct Raw8<float> {
     v[0] = ok ? *reinterpret_cast<const f32x4*>(p) : z;
     v[1] = ok ? *reinterpret_cast<const f32x4*>(p + 4) : z;
   }
-  __device__ __forceinline__ Frag<float> frag() const {
-    const float t[8] = {v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+  __device__ __forceinline__ Frag<float> frag(float s) const {
+    const float t[8] = {v[0][0] * s, v[0][1] * s, v[0][2] * s, v[0][3] * s, v[1][0] * s, v[1][1] * s, v[1][2] * s, v[1][3] * s};
     return da_pack<float>(t);
   }
   __device__ __forceinline__ void widen(float (&t)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = v[e >> 2][e & 3];
+  }
+  __device__ __forceinline__ unsigned bits(unsigned a) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = da_max_bits(a, v[e >> 2][e & 3]);
+    return a;
   }
 };
 template <typename T> struct Raw8 {
@@ -113,12 +132,31 @@ template <typename T> struct Raw8 {
     const u32x4 z = {0, 0, 0, 0};
     v = __builtin_bit_cast(vec8<T>, ok ? *reinterpret_cast<const u32x4*>(p) : z);
   }
-  __device__ __forceinline__ Frag<T> frag() const { return Frag<T>{{v}}; }
+  __device__ __forceinline__ Frag<T> frag(float) const { return Frag<T>{{v}}; }
   __device__ __forceinline__ void widen(float (&t)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (float)v[e];
   }
+  __device__ __forceinline__ unsigned bits(unsigned a) const { return a; }
 };
+
+// a lane's own row as KS operands (elements 16 s + 8 h .. of a row of n live ones) and the scale they carry: the row's own
+// power of two for fp32, 1 otherwise
+template <typename T, int KS>
+__device__ __forceinline__ float da_row(const T* p, int n, bool live, int h, Frag<T> (&f)[KS]) {
+  Raw8<T> raw[KS];
+  unsigned bits = 0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    raw[s].load(p + 16 * s + 8 * h, live && 16 * s + 8 * h < n);
+    bits = raw[s].bits(bits);
+  }
+  float sc = 1.f;
+  if constexpr (DaT<T>::NP == 2) sc = da_scale(max(bits, (unsigned)__shfl_xor((int)bits, 32, 64)));
+#pragma unroll
+  for (int s = 0; s < KS; ++s) f[s] = raw[s].frag(sc);
+  return sc;
+}
 
 // byte offset of piece c of a row of 2 DP 16-bit elements
 template <int DP>
@@ -131,38 +169,60 @@ __device__ __forceinline__ int da_off(int row, int c) {
   }
 }
 
+// The LDS addresses a lane reads a tile's operands at: few registers, everything else is an offset of the instruction.
+template <int DP>
+struct Lane {
+  unsigned r[DP == 16 ? 2 : 4], c[DP == 16 ? 1 : 2];
+  // row0: the wave's first row of every tile (a multiple of 32)
+  __device__ __forceinline__ Lane(int lane, int row0) {
+    const int h = lane >> 5, i = lane & 15;
+#pragma unroll
+    for (int k = 0; k < (DP == 16 ? 2 : 4); ++k) r[k] = da_off<DP>(lane & 31, 2 * k + h) + row0 * (4 * DP);
+#pragma unroll
+    for (int v = 0; v < (DP == 16 ? 1 : 2); ++v)
+      c[v] = da_off<DP>(4 * h + (i >> 2), 4 * v + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) + 8 * (i & 1) + row0 * (4 * DP);
+  }
+  __device__ __forceinline__ void flip(unsigned bit) {
+#pragma unroll
+    for (int k = 0; k < (DP == 16 ? 2 : 4); ++k) r[k] ^= bit;
+#pragma unroll
+    for (int v = 0; v < (DP == 16 ? 1 : 2); ++v) c[v] ^= bit;
+  }
+};
+
 template <typename T, int DP, int KT>
 struct Tile {
   static constexpr int NP = DaT<T>::NP;
   static constexpr int kPlane = KT * 4 * DP;          // bytes of one plane of X or Y
   static constexpr int kBytes = 2 * NP * kPlane;      // X planes, then Y planes
   typedef typename DaT<T>::E E;
+  typedef __attribute__((address_space(3))) const vec8<E> lds_vec8;
 
-  // A operand, 32 rows row0 .. row0 + 31 (a multiple of 32), step ks of the 16-deep steps along the row (X: map m starts at
+  // A operand, 32 rows row0 .. row0 + 31 of the wave's (a multiple of 32), step ks of the 16-deep steps along the row (X: map m starts at
   // step m DP / 16)
-  static __device__ __forceinline__ Frag<T> rows(const char* lds, int which, int row0, int ks, int lane) {
+  static __device__ __forceinline__ Frag<T> rows(const Lane<DP>& L, int which, int row0, int ks) {
+    return rows_at(L.r[DP == 16 ? ks : ks & 3], which * NP, row0, ks);
+  }
+  static __device__ __forceinline__ Frag<T> rows_at(unsigned at, int plane, int row0, int ks) {
     Frag<T> f;
-    const int o = da_off<DP>(row0 + (lane & 31), 2 * ks + (lane >> 5));
+    const int o = row0 * (4 * DP) + (DP == 16 ? 0 : (ks >> 2) * 128);
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-      f.p[p] = *reinterpret_cast<const vec8<E>*>(lds + (which * NP + p) * kPlane + o);
+    for (int p = 0; p < NP; ++p) f.p[p] = *(lds_vec8*)(at + (unsigned)((plane + p) * kPlane + o));
     return f;
   }
   // A operand of the transposed tile: 32 columns col0 .. (a multiple of 32), reduced rows row0 + 16 t + {4 h + 0..3,
   // 8 + 4 h + 0..3}
-  static __device__ __forceinline__ Frag<T> cols(const char* lds, int which, int row0, int t, int col0, int lane) {
+  static __device__ __forceinline__ Frag<T> cols(const Lane<DP>& L, int which, int row0, int t, int col0) {
     Frag<T> f;
-    const int i = lane & 15, h = lane >> 5;
-    const int row = row0 + 16 * t + 4 * h + (i >> 2);
-    const int c = col0 / 8 + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-    const int o0 = da_off<DP>(row, c) + 8 * (i & 1), o1 = da_off<DP>(row + 8, c) + 8 * (i & 1);
+    const unsigned at = L.c[DP == 16 ? 0 : (col0 >> 5) & 1];
+    const int o = (row0 + 16 * t) * (4 * DP) + (col0 >> 6) * 128;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const char* b = lds + (which * NP + p) * kPlane;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(b + o0));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(b + o1));
-      const vec4<E> a = __builtin_bit_cast(vec4<E>, lo), z = __builtin_bit_cast(vec4<E>, hi);
-      f.p[p] = __builtin_shufflevector(a, z, 0, 1, 2, 3, 4, 5, 6, 7);
+      const unsigned b = at + (unsigned)((which * NP + p) * kPlane + o);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(b + 8 * 4 * DP));
+      const vec4<E> x = __builtin_bit_cast(vec4<E>, lo), z = __builtin_bit_cast(vec4<E>, hi);
+      f.p[p] = __builtin_shufflevector(x, z, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     return f;
   }
@@ -175,34 +235,38 @@ __device__ __attribute__((aligned(16))) const unsigned da_zero[4] = {0, 0, 0, 0}
 template <typename T>
 struct Rows {
   const T *x, *y;
-  long x_rs, x_ms, y_rs;
-  int n, d;
+  long x_ms;
+  int x_rs, y_rs, n, d;
   const unsigned char* mask;
 };
 
-// Tiles on their way from memory to LDS, NT threads together.
+// Tiles on their way from memory to LDS, NT threads together, at LDS address 0.
 //   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), two tiles: while one is computed on, the next
 //   lands.  The 64 pieces of a wave's copy stand one behind the other in LDS, so the lane picks the piece that belongs there.
-//   fp32: through registers, where the values are split into planes; one tile.
-// use:  feed.issue(first, row0);  for each tile: { const char* t = feed.next();  [feed.issue(following, row0)];  compute }
+//   fp32: through registers, where the values are scaled and split into planes; one tile.
+// use:  feed.issue(first, row0);  for each tile: { feed.next(L);  [feed.issue(following, row0)];  compute }
 // next() is a barrier of the workgroup.
 template <typename T, int DP, int KT, int NT>
 struct Feed {
   typedef Tile<T, DP, KT> Tl;
   static constexpr bool DMA = Tl::NP == 1;
   static constexpr int kPieces = KT * DP / 4;                    // of X, and of Y
-  static constexpr int kPer = (kPieces + NT - 1) / NT;
-  static constexpr int kTile = Tl::kBytes + 16 * ((KT / 8 + 15) / 16);   // the tile and its visible rows, a bit each
-  static constexpr int kLds = kTile * (DMA ? 2 : 1);
+  static constexpr int kPer = (kPieces + NT - 1) / NT, NW = NT / 64;
+  static constexpr int kBufs = Tl::kBytes * (DMA ? 2 : 1);
+  static constexpr int kLds = kBufs + 32 + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
   static_assert(!DMA || kPieces % 64 == 0, "whole waves copy");
   static_assert(NT * 4 / DP % 8 == 0 || kPer == 1, "a thread's pieces stand at one place of their rows");
+  static_assert(KT <= 128 && (Tl::kBytes & (Tl::kBytes - 1)) == 0, "room for the visible rows; tiles told apart by one address bit");
 
   char* lds;
-  int tid, wave, cur;       // cur: the buffer that next() returns
+  int tid, wave, cur;       // cur: the buffer that next() left current
   bool bit;
+  unsigned ux, uy, uz;      // fp32: absolute bits of the largest value so far in X, in Y, and of next()'s third value
+  float sx, sy;             // the scales of X and Y in LDS
   Raw8<T> x[DMA ? 1 : kPer], y[DMA ? 1 : kPer];
 
-  __device__ __forceinline__ Feed(char* l, int t) : lds(l), tid(t), wave(__builtin_amdgcn_readfirstlane(t >> 6)), cur(0), bit(false) {}
+  __device__ __forceinline__ Feed(char* l, int t)
+      : lds(l), tid(t), wave(__builtin_amdgcn_readfirstlane(t >> 6)), cur(0), bit(false), ux(0), uy(0), uz(0), sx(1.f), sy(1.f) {}
 
   // piece e of a matrix of the tile -> its row and column piece
   static __device__ __forceinline__ void place(int e, int& row, int& c) {
@@ -215,86 +279,125 @@ struct Feed {
       c = (e % (DP / 4)) ^ (((row & 3) << 1) | ((row >> 2) & 1));
     }
   }
-  static __device__ __forceinline__ void words(char* tile, int tid, bool bit) {
+  __device__ __forceinline__ unsigned* words(int buf) const { return reinterpret_cast<unsigned*>(lds + kBufs) + 4 * buf; }
+  __device__ __forceinline__ void write_words(int buf) {
     if (tid < KT) {
       const unsigned long long w = __ballot(bit);
-      if ((tid & 31) == 0) reinterpret_cast<unsigned*>(tile + Tl::kBytes)[tid >> 5] = (unsigned)(w >> (tid & 32));
+      if ((tid & 31) == 0) words(buf)[tid >> 5] = (unsigned)(w >> (tid & 32));
     }
   }
-  static __device__ __forceinline__ void copy16(const void* g, char* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+  static __device__ __forceinline__ void copy16(const T* g, unsigned off, char* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)g + off),
                                      (__attribute__((address_space(3))) void*)l, 16, 0, 0);
   }
 
   __device__ __forceinline__ void issue(const Rows<T>& R, int row0) {
     bit = tid < KT && row0 + tid < R.n && (!R.mask || R.mask[row0 + tid]);
+    const T* xt = R.x + (long)row0 * R.x_rs;
+    const T* yt = R.y + (long)row0 * R.y_rs;
     if constexpr (DMA) {
-      char* tile = lds + (cur ^ 1) * kTile;
       int row, c;
       place(tid, row, c);
       const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
-      const bool all = R.d == DP && row0 + KT <= R.n && !R.mask;      // uniform
-      const long xo = (long)row * R.x_rs + map * R.x_ms + o, yo = (long)row * R.y_rs + c * 8;
-      const T* xt = R.x + row0 * R.x_rs;
-      const T* yt = R.y + row0 * R.y_rs;
+      // (byte offsets of a tile fit into 32 bits: rows are at most 2^23 elements apart, a map at most 2^28)
+      const unsigned xo = (unsigned)(row * R.x_rs + map * (int)R.x_ms + o) * 2u, yo = (unsigned)(row * R.y_rs + c * 8) * 2u;
       constexpr int kRows = NT * 4 / DP;       // rows between a thread's pieces
+      char* l = lds + (cur ^ 1) * Tl::kBytes + 64 * wave * 16;
+      if (R.d == DP && row0 + KT <= R.n && !R.mask) {      // uniform
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (kPieces % NT && 64 * wave + NT * i >= kPieces) break;
-        char* l = tile + (64 * wave + NT * i) * 16;
-        const T *px = xt + xo + i * kRows * R.x_rs, *py = yt + yo + i * kRows * R.y_rs;
-        if (!all) {
+        for (int i = 0; i < kPer; ++i) {
+          if (kPieces % NT && 64 * wave + NT * i >= kPieces) break;
+          copy16(xt + (long)i * kRows * R.x_rs, xo, l + NT * i * 16);
+          copy16(yt + (long)i * kRows * R.y_rs, yo, l + NT * i * 16 + Tl::kPlane);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kPer; ++i) {
+          if (kPieces % NT && 64 * wave + NT * i >= kPieces) break;
           const int r = row0 + row + i * kRows;
           const bool ok = r < R.n && (!R.mask || R.mask[r]);
-          px = ok && o < R.d ? px : (const T*)da_zero;
-          py = ok && c * 8 < 2 * R.d ? py : (const T*)da_zero;
+          const char *px = (const char*)(xt + (long)i * kRows * R.x_rs) + xo, *py = (const char*)(yt + (long)i * kRows * R.y_rs) + yo;
+          copy16((const T*)(ok && o < R.d ? px : (const char*)da_zero), 0, l + NT * i * 16);
+          copy16((const T*)(ok && c * 8 < 2 * R.d ? py : (const char*)da_zero), 0, l + NT * i * 16 + Tl::kPlane);
         }
-        copy16(px, l);
-        copy16(py, l + Tl::kPlane);
       }
-      words(tile, tid, bit);
+      write_words(cur ^ 1);
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int e = tid + NT * i;
-        if (kPieces % NT && e >= kPieces) break;
+        if (kPieces % NT && e >= kPieces) {
+          x[i].load(nullptr, false);
+          y[i].load(nullptr, false);
+          continue;
+        }
         const int row = e / (DP / 4), c = e % (DP / 4);
         const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
-        const long r = row0 + row;
-        const bool ok = r < R.n && (!R.mask || R.mask[r]);
-        x[i].load(R.x + r * R.x_rs + map * R.x_ms + o, ok && o < R.d);
-        y[i].load(R.y + r * R.y_rs + c * 8, ok && c * 8 < 2 * R.d);
+        const bool ok = row0 + row < R.n && (!R.mask || R.mask[row0 + row]);
+        x[i].load(xt + (unsigned)(row * R.x_rs + map * (int)R.x_ms + o), ok && o < R.d);
+        y[i].load(yt + (unsigned)(row * R.y_rs + c * 8), ok && c * 8 < 2 * R.d);
       }
     }
   }
-  // the tile issued last, in LDS for every wave; every wave is done with the tile before it
-  __device__ __forceinline__ const char* next() {
+  // the tile issued last, in LDS for every wave; every wave is done with the tile before it.  fp32: its scales are sx, sy,
+  // never above those of the tiles before; `third`: a value of each thread whose largest so far joins uz; between(): run by
+  // every thread before the second barrier, with the new scales
+  template <typename F>
+  __device__ __forceinline__ void next(Lane<DP>& L, unsigned third, F between) {
     if constexpr (DMA) {
+      between();
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       cur ^= 1;
-      return lds + cur * kTile;
+      L.flip(Tl::kBytes);
     } else {
+      unsigned mx = 0, my = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        mx = x[i].bits(mx);
+        my = y[i].bits(my);
+      }
+      mx = da_wave_max(mx);
+      my = da_wave_max(my);
+      third = da_wave_max(third);
+      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 32);
+      if ((tid & 63) == 0) {
+        const u32x4 m = {mx, my, third, 0u};
+        red[wave] = m;
+      }
       __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const u32x4 m = red[w];
+        ux = max(ux, m[0]);
+        uy = max(uy, m[1]);
+        uz = max(uz, m[2]);
+      }
+      ux = __builtin_amdgcn_readfirstlane(ux);
+      uy = __builtin_amdgcn_readfirstlane(uy);
+      uz = __builtin_amdgcn_readfirstlane(uz);
+      sx = da_scale(ux);
+      sy = da_scale(uy);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int e = tid + NT * i;
         if (kPieces % NT && e >= kPieces) break;
         const int o = da_off<DP>(e / (DP / 4), e % (DP / 4));
-        const Frag<T> fx = x[i].frag(), fy = y[i].frag();
+        const Frag<T> fx = x[i].frag(sx), fy = y[i].frag(sy);
 #pragma unroll
         for (int p = 0; p < Tl::NP; ++p) {
           *reinterpret_cast<vec8<typename Tl::E>*>(lds + p * Tl::kPlane + o) = fx.p[p];
           *reinterpret_cast<vec8<typename Tl::E>*>(lds + (Tl::NP + p) * Tl::kPlane + o) = fy.p[p];
         }
       }
-      words(lds, tid, bit);
+      write_words(0);
+      between();
       __syncthreads();
-      return lds;
     }
   }
-  static __device__ __forceinline__ unsigned word(const char* tile, int row0) {
-    return reinterpret_cast<const unsigned*>(tile + Tl::kBytes)[row0 >> 5];
+  __device__ __forceinline__ void next(Lane<DP>& L) {
+    next(L, 0u, [] {});
   }
+  __device__ __forceinline__ unsigned word(int row0) const { return words(DMA ? cur : 0)[row0 >> 5]; }
 };
 
 template <typename T>
@@ -307,12 +410,15 @@ __device__ __forceinline__ int da_len(const DaArgs& A, int b) {
   const int n = A.lengths ? A.lengths[b] : A.Nk;
   return n < 0 ? 0 : n > A.Nk ? A.Nk : n;
 }
-__device__ __forceinline__ long da_start(const DaArgs& A, int b) { return A.q_start ? (long)A.q_start[b] : (long)A.Nk - A.Nq; }
+__device__ __forceinline__ int da_start(const DaArgs& A, int b) {      // (sizes end at 2^30: beyond that, all or none)
+  const int s = A.q_start ? A.q_start[b] : A.Nk - A.Nq;
+  return s < -(1 << 30) - 1 ? -(1 << 30) - 1 : s > 1 << 30 ? 1 << 30 : s;
+}
 // keys that query i sees
-__device__ __forceinline__ int da_limit(const DaArgs& A, int len, long start, int i) {
+__device__ __forceinline__ int da_limit(const DaArgs& A, int len, int start, int i) {
   if (!A.causal) return len;
-  const long n = start + i + 1;
-  return n < 0 ? 0 : n > len ? len : (int)n;
+  const int n = start + i + 1;
+  return n < 0 ? 0 : n > len ? len : n;
 }
 
 // workgroups of one (batch item, key head) on one XCD, so that its keys and values are read once into that XCD's L2:

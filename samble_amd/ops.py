@@ -429,14 +429,15 @@ ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # incl
 
 
 def _rows16(t: torch.Tensor):
-    """(t, its strides but the last; 0 for axes of one): every row on 16 bytes and contiguous, a copy where it is not so."""
+    """(t, its strides but the last; 0 for axes of one): every row on 16 bytes and contiguous, rows within 2^23 and maps within
+    2^28 elements of each other, a copy where it is not so."""
     unit = 16 // t.element_size()
     for copy in (False, True):
         if copy:
             t = t.clone(memory_format=torch.contiguous_format)
         st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
         last = st.pop()
-        if copy or (last == 1 and t.data_ptr() % 16 == 0 and not any([s % unit for s in st])):
+        if copy or (last == 1 and t.data_ptr() % 16 == 0 and st[1] <= 1 << 23 and st[-1] <= 1 << 28 and not any([s % unit for s in st])):
             return t, st
 
 

@@ -41,6 +41,8 @@ def _check(q, k, v, lam, g, got, scale, causal, lengths, q_start, key_mask):
     half = torch.finfo(dt).eps / 2
     hp = 0.0 if dt == torch.float32 else half       # P and dS as operands
     sub = 2.0 ** -25 if dt == torch.float16 else 0.0
+    three = dt == torch.float32
+    subp = 2.0 ** -31 if three else sub
     ok_all = _visible(B, Nq, Nk, causal, lengths, q_start, key_mask, q.device)
     lam_err = torch.zeros(H, dtype=torch.float64, device=q.device)
     lam_ref = torch.zeros(H, dtype=torch.float64, device=q.device)
@@ -75,18 +77,20 @@ def _check(q, k, v, lam, g, got, scale, causal, lengths, q_start, key_mask):
                     dP.append(2 * ((d + 32) * U * L + 16 * U) + Nk * U)                # relative error of the map, per row
                 o1, o2 = P[0] @ vv, P[1] @ vv
                 av = vv.abs()
-                e1 = (P[0] * (dP[0] + hp)) @ av + sub * (ok.double() @ av)             # error of o1, o2 before rounding
-                e2 = (P[1] * (dP[1] + hp)) @ av + sub * (ok.double() @ av)
+                e1 = (P[0] * (dP[0] + hp)) @ av + subp * (ok.double() @ av)            # error of o1, o2 before rounding
+                e2 = (P[1] * (dP[1] + hp)) @ av + subp * (ok.double() @ av)
                 ref = o1 - lm * o2
                 held(got[0][b, :, hq], ref, e1 + abs(lm) * e2 + 4 * U * (o1.abs() + abs(lm) * o2.abs()), f"out b{b} h{hq}")
                 if g is None:
                     continue
                 gg = g[b, :, hq].double()
                 A = P[0] - lm * P[1]
-                eA = P[0] * dP[0] + abs(lm) * P[1] * dP[1] + hp * A.abs() + sub * ok
+                eA = P[0] * dP[0] + abs(lm) * P[1] * dP[1] + hp * A.abs() + (2.0 ** -37 * (1 + abs(lm)) if three else sub) * ok
                 dv_ref += A.T @ gg
                 dv_tol += eA.T @ gg.abs() + Nq * G * U * (A.abs().T @ gg.abs())
                 dA = gg @ vv.T
+                subs = (2.0 ** -35 * (1 + lam.double().abs().max()) * g[b].double().norm(dim=-1).max() * vv.norm(dim=-1).max()
+                        if three else sub)
                 edA = (2 * d + 32) * U * (gg.abs() @ av.T)
                 t2 = (P[1] * dA).sum(-1, keepdim=True)
                 t1 = (P[0] * dA).sum(-1, keepdim=True)
@@ -99,7 +103,7 @@ def _check(q, k, v, lam, g, got, scale, causal, lengths, q_start, key_mask):
                 lam_err[hq] += et2.sum() + Nq * B * U * t2.abs().sum()
                 for m, (t, et, sign) in enumerate(((t1, et1, 1.0), (t2, et2, -lm))):
                     dS = sign * P[m] * (dA - t)
-                    edS = abs(sign) * P[m] * (edA + et + (dP[m] + 4 * U) * (dA - t).abs()) + hp * dS.abs() + sub * ok
+                    edS = abs(sign) * P[m] * (edA + et + (dP[m] + 4 * U) * (dA - t).abs()) + hp * dS.abs() + subs * ok
                     dq_ref = scale * dS @ kk[:, m]
                     dq_tol = scale * (edS + Nk * U * dS.abs()) @ kk[:, m].abs()
                     held(got[1][b, :, hq, m], dq_ref, dq_tol, f"dq b{b} h{hq} m{m}")
