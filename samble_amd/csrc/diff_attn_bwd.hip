@@ -32,12 +32,12 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rw = wave % RW, mw = Cfg::MW > 1 ? wave / RW : 0;
+  const int wave = da_uni(tid >> 6), rw = wave % RW, mw = Cfg::MW > 1 ? wave / RW : 0;
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = (long)blocks * A.B * A.Hkv, unit = da_unit(units);
   if (unit >= units) return;
-  const unsigned blk = blocks - 1 - (unsigned)(unit % blocks);
-  const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
+  const unsigned blk = blocks - 1 - (unsigned)da_uni((int)(unit % blocks));
+  const int pair = da_uni((int)(unit / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int len = da_len(A, b);
   const int start = da_start(A, b);
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
@@ -45,8 +45,8 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   const int qi = live ? (int)(r / (unsigned)A.G) : 0, head = hk * A.G + (live ? (int)(r % (unsigned)A.G) : 0);
   const int limit = live ? da_limit(A, len, start, qi) : 0;
   const unsigned last = blk * 32 * RW + 32 * RW - 1;
-  const int kmax = da_limit(A, len, start, (int)((last < rows ? last : rows - 1) / (unsigned)A.G));
-  const int kmin = first + 31 < rows ? da_limit(A, len, start, (int)(first / (unsigned)A.G)) : 0;
+  const int kmax = da_limit(A, len, start, da_uni((last < rows ? last : rows - 1) / (unsigned)A.G));
+  const int kmin = first + 31 < rows ? da_limit(A, len, start, da_uni(first / (unsigned)A.G)) : 0;
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
 
   const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_ms, (int)A.k_rs, (int)A.v_rs,
@@ -133,8 +133,8 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
       const int row0 = 32 * sub, k0 = t * Cfg::KT + row0;
       if (k0 >= kmax) continue;
-      const unsigned word = feed.word(row0);
-      const bool masked = __builtin_amdgcn_readfirstlane(word) != 0xffffffffu || k0 + 32 > kmin;
+      const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;      // (rows end at their limits, at most len)
+      const bool masked = word != 0xffffffffu || k0 + 32 > kmin;
       f32x16 da = zero16();
 #pragma unroll
       for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(L, 1, row0, ks), gf[ks], da);
@@ -163,7 +163,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
       for (int m = 0; m < MPW; ++m) {
         f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, row0, (m + mw) * KS + ks), qf[m][ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::map_rows(L, m, mw, row0, ks), qf[m][ks], s);
         const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cm, -lse[m]));
@@ -193,7 +193,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
           Frag<T> kf;
 #pragma unroll
           for (int m = 0; m < MPW; ++m) {
-            if (DP >= 32 || m == 0) kf = Tl::cols(L, 0, row0, u, DP < 32 ? 0 : (m + mw) * DP + 32 * dt);
+            if (DP >= 32 || m == 0) kf = DP < 32 ? Tl::cols(L, 0, row0, u, 0) : Tl::map_cols(L, m, mw, row0, u, 32 * dt);
             acc[m][dt] = da_mma<T>(kf, ds[m][u], acc[m][dt]);
           }
         }
@@ -270,13 +270,13 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     return;
   }
 
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kb = wave % KBW, rww = RWW > 1 ? wave / KBW : 0;
+  const int wave = da_uni(tid >> 6), kb = wave % KBW, rww = RWW > 1 ? wave / KBW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
   const long units = (long)blocks * A.B * A.Hkv;
   const long unit = (long)(blockIdx.x & 7) * (main_grid / 8) + (blockIdx.x >> 3);
   if (unit >= units) return;
-  const int blk = (int)(unit % blocks);           // (under a causal mask the keys that most rows see first)
-  const int pair = (int)(unit / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
+  const int blk = da_uni((int)(unit % blocks));   // (under a causal mask the keys that most rows see first)
+  const int pair = da_uni((int)(unit / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int len = da_len(A, b);
   const int start = da_start(A, b);
   const int key0 = blk * Cfg::KB, kw0 = key0 + 32 * kb, key = kw0 + (lane & 31);
@@ -431,7 +431,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 #pragma unroll
         for (int ks = 0; ks < 2 * KS; ++ks) {
           if constexpr (Cfg::VL) {
-            const unsigned at = (L.r[ks & 3] & (unsigned)(Tl::kBytes - 1)) + (unsigned)(Cfg::kLds - Cfg::kVal + (32 * kb - 32 * rww) * 4 * DP);
+            const unsigned at = L.r[(ks >> 1) & (Lane<DP>::NR - 1)] + (unsigned)(Cfg::kLds - Cfg::kVal + (32 * kb - 32 * rww) * 4 * DP - (Fd::DMA ? feed.cur * Tl::kBytes : 0));
             da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), Cfg::Vt::rows_at(at, 0, 0, ks), da);
           } else {
             da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), vf[ks], da);

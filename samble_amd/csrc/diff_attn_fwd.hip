@@ -16,7 +16,7 @@ namespace samble {
 template <typename T, int DP, int RW, int KW, int MW>
 struct FwdCfg {
   static constexpr int NW = RW * KW * MW, NT = 64 * NW;
-  static constexpr int SUB = KW > 1 ? 1 : DP <= 64 ? 2 : 1;   // 32-key steps of a wave per tile
+  static constexpr int SUB = KW > 1 ? 1 : 2;                  // 32-key steps of a wave per tile
   static constexpr int KT = 32 * KW * SUB;
   static constexpr int DVT = 2 * DP / 32, MPW = 2 / MW;      // 32-column pieces of an output, maps of a wave
   typedef Feed<T, DP, KT, NT> Fd;
@@ -45,16 +45,16 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = da_uni(tid >> 6);
   const int rw = wave % RW, kw = KW > 1 ? (wave / RW) % KW : 0, mw = MW > 1 ? wave / (RW * KW) : 0;
   const unsigned rows = (unsigned)A.Nq * A.G;
   const unsigned blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = (long)blocks * A.splits * A.B * A.Hkv;
   const long unit = da_unit(units);
   if (unit >= units) return;
-  const unsigned split = (unsigned)(unit % A.splits), rest = (unsigned)(unit / A.splits);
-  const unsigned blk = blocks - 1 - rest % blocks;      // (under a causal mask the long rows first)
-  const int pair = (int)(rest / blocks), b = pair / A.Hkv, hk = pair % A.Hkv;
+  const unsigned rest = da_uni((int)(unit / A.splits)), split = (unsigned)(unit - (long)rest * A.splits);
+  const int pair = da_uni((int)(rest / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
+  const unsigned blk = blocks - 1 - (rest - pair * blocks);      // (under a causal mask the long rows first)
 
   const int len = da_len(A, b);
   const int start = da_start(A, b);
@@ -65,11 +65,11 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   const int limit = live ? da_limit(A, len, start, qi) : 0;
   // keys that the last row of the workgroup sees; fewest keys of this wave's rows
   const unsigned last = blk * 32 * RW + 32 * RW - 1;
-  const int kmax = da_limit(A, len, start, (int)((last < rows ? last : rows - 1) / (unsigned)A.G));
-  const int kmin = first + 31 < rows ? da_limit(A, len, start, (int)(first / (unsigned)A.G)) : 0;
+  const int kmax = da_limit(A, len, start, da_uni((last < rows ? last : rows - 1) / (unsigned)A.G));
+  const int kmin = first + 31 < rows ? da_limit(A, len, start, da_uni(first / (unsigned)A.G)) : 0;
 
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
-  const int t0 = (int)((long)tiles * split / A.splits), t1 = (int)((long)tiles * (split + 1) / A.splits);
+  const int t0 = da_uni((int)((long)tiles * split / A.splits)), t1 = da_uni((int)((long)tiles * (split + 1) / A.splits));
 
   const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_ms, (int)A.k_rs, (int)A.v_rs,
                         len, A.d, A.key_mask ? A.key_mask + b * A.km_bs : nullptr};
@@ -86,15 +86,95 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
   }
 
   f32x16 o[MPW][DVT];
-  float mx[MPW], l[MPW];
+  // reference of the exponentials, maximum from which it moves on (minus infinity: no key seen), sum
+  float ref[MPW], more_at[MPW], l[MPW];
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    mx[m] = kNegInf;
-    l[m] = 0.f;
+    ref[m] = l[m] = 0.f;
+    more_at[m] = kNegInf;
 #pragma unroll
     for (int t = 0; t < DVT; ++t) o[m][t] = zero16();
   }
   float vscale = 1.f;       // scale of the outputs' sums (fp32: the values')
+
+  Frag<T> pf[MPW][2];       // the step's probabilities, operands of the value products
+  // logits of the 32 keys at L + off
+  auto logits = [&](const Lane<DP>& L, int off, f32x16 (&s)[MPW]) {
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) {
+      s[m] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[m] = da_mma<T>(Tl::map_rows(L, m, mw, off, ks), qf[m][ks], s[m]);
+    }
+  };
+  // O += P V of the 32 keys at L + off
+  auto values = [&](const Lane<DP>& L, int off) {
+#pragma unroll
+    for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const Frag<T> vf = Tl::cols(L, 1, off, u, 32 * dt);
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) o[m][dt] = da_mma<T>(vf, pf[m][u], o[m][dt]);
+      }
+  };
+  float cm[MPW];
+  auto hide = [&](f32x16 (&s)[MPW], int k0, unsigned word) {       // what the rows do not see
+    unsigned w = word >> (4 * h);
+    int left = limit - k0 - 4 * h;
+    asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every step, in front of the branch)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int j = crow(e, 0);
+      const bool see = ((w >> j) & 1) && j < left;
+#pragma unroll
+      for (int m = 0; m < MPW; ++m) s[m][e] = see ? s[m][e] : kNegInf;
+    }
+  };
+  // The reference of the exponentials follows the maximum only when that has grown by more than 8 (a factor of 256 in the
+  // sums): any reference gives the same quotients, and the outputs are rescaled in few of the steps.
+  auto refer = [&](const f32x16 (&s)[MPW]) {
+    float top[MPW];
+    bool more = false;
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) {
+      top[m] = s[m][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top[m] = fmaxf(top[m], s[m][e]);      // (of this half of the keys: enough for the question)
+      more = more || top[m] * cm[m] > more_at[m];
+    }
+    if (__any(more)) {
+#pragma unroll
+      for (int m = 0; m < MPW; ++m) {
+        const float mx = fmaxf(more_at[m] == kNegInf ? kNegInf : ref[m], xor32_max(top[m]) * cm[m]);
+        const float now = mx == kNegInf ? 0.f : mx;
+        const float al = more_at[m] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ref[m] - now);      // (first: sums of zero)
+        l[m] *= al;
+#pragma unroll
+        for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[m][dt][e] *= al;
+        ref[m] = now;
+        more_at[m] = mx + 8.f;
+      }
+    }
+  };
+  auto weigh = [&](const f32x16 (&s)[MPW], Frag<T> (&f)[MPW][2]) {
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) {
+      const float sub = ref[m] - (float)DaT<T>::kP;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(s[m][8 * u + e], cm[m], -sub));
+          l[m] += p[e];
+        }
+        f[m][u] = da_pack<T>(p);
+      }
+    }
+  };
 
   for (int t = t0; t < t1; ++t) {
     feed.next(L);
@@ -108,70 +188,28 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[m][dt][e] *= f;
     }
+#pragma unroll
+    for (int m = 0; m < MPW; ++m) cm[m] = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
     if (t + 1 < t1) feed.issue(keys, (t + 1) * Cfg::KT);
+    f32x16 s[2][MPW];
+    logits(L, 0, s[0]);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
       const int row0 = 32 * (kw + sub), k0 = t * Cfg::KT + row0;
-      if (k0 >= kmax) continue;   // (uniform; nothing of it is seen)
-      const unsigned word = feed.word(row0);
-      const bool masked = __builtin_amdgcn_readfirstlane(word) != 0xffffffffu || k0 + 32 > kmin;
-      Frag<T> pf[MPW][2];
-#pragma unroll
-      for (int m = 0; m < MPW; ++m) {
-        f32x16 s = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, 32 * sub, (m + mw) * KS + ks), qf[m][ks], s);
-        if (masked) {
-          unsigned w = word >> (4 * h);
-          int left = limit - k0 - 4 * h;
-          asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every tile, in front of the branch)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = crow(e, 0);
-            s[e] = ((w >> j) & 1) && j < left ? s[e] : kNegInf;
-          }
-        }
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
-        top = xor32_max(top) * cm;
-        // the reference of the exponentials follows the maximum only when that has grown by more than 8 (a factor of 256 in
-        // the sums): any reference gives the same quotients, and the outputs are rescaled in few of the steps
-        if (__any(top > mx[m] + 8.f)) {
-          const float nm = fmaxf(mx[m], top), use = nm == kNegInf ? 0.f : nm;
-          const float al = __builtin_amdgcn_exp2f(mx[m] - use);
-          l[m] *= al;
-#pragma unroll
-          for (int dt = 0; dt < DVT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[m][dt][e] *= al;
-          mx[m] = nm;
-        }
-        const float ref = (mx[m] == kNegInf ? 0.f : mx[m]) - (float)DaT<T>::kP;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(s[8 * u + e], cm, -ref));
-            l[m] += p[e];
-          }
-          pf[m][u] = da_pack<T>(p);
-        }
-      }
-#pragma unroll
-      for (int dt = 0; dt < DVT; ++dt)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const Frag<T> vf = Tl::cols(L, 1, 32 * sub, u, 32 * dt);
-#pragma unroll
-          for (int m = 0; m < MPW; ++m) o[m][dt] = da_mma<T>(vf, pf[m][u], o[m][dt]);
-        }
+      if (sub && k0 >= kmax) break;   // (uniform; nothing of it is seen)
+      const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;
+      if (word != 0xffffffffu || k0 + 32 > kmin) hide(s[sub & 1], k0, word);
+      refer(s[sub & 1]);
+      if (sub + 1 < Cfg::SUB) logits(L, 32 * (sub + 1), s[(sub + 1) & 1]);
+      weigh(s[sub & 1], pf);
+      values(L, 32 * sub);
     }
   }
 #pragma unroll
-  for (int m = 0; m < MPW; ++m) l[m] = da_xor32_sum(l[m]);
+  for (int m = 0; m < MPW; ++m) {
+    l[m] = da_xor32_sum(l[m]);
+    if (more_at[m] == kNegInf) ref[m] = kNegInf;
+  }
 
   if constexpr (KW > 1) {   // the waves along the keys: pairwise, the upper half hands its state to the lower
     float* f = reinterpret_cast<float*>(smem);
@@ -182,7 +220,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
         float* w = f + ((kw - s) * RW * MW + rw * MW + mw) * Cfg::kState + lane;
 #pragma unroll
         for (int m = 0; m < MPW; ++m) {
-          w[(2 * m) * 64] = mx[m];
+          w[(2 * m) * 64] = ref[m];
           w[(2 * m + 1) * 64] = l[m];
 #pragma unroll
           for (int dt = 0; dt < DVT; ++dt)
@@ -196,9 +234,9 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
 #pragma unroll
         for (int m = 0; m < MPW; ++m) {
           const float m2 = w[(2 * m) * 64], l2 = w[(2 * m + 1) * 64];
-          const float nm = fmaxf(mx[m], m2), use = nm == kNegInf ? 0.f : nm;
-          const float a1 = __builtin_amdgcn_exp2f(mx[m] - use), a2 = __builtin_amdgcn_exp2f(m2 - use);
-          mx[m] = nm;
+          const float nm = fmaxf(ref[m], m2), use = nm == kNegInf ? 0.f : nm;
+          const float a1 = __builtin_amdgcn_exp2f(ref[m] - use), a2 = __builtin_amdgcn_exp2f(m2 - use);
+          ref[m] = nm;
           l[m] = l[m] * a1 + l2 * a2;
 #pragma unroll
           for (int dt = 0; dt < DVT; ++dt)
@@ -217,7 +255,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
 #pragma unroll
     for (int m = 0; m < MPW; ++m) {
       if (h == 0) {
-        w[2 * (m + mw)] = mx[m];
+        w[2 * (m + mw)] = ref[m];
         w[2 * (m + mw) + 1] = l[m];
       }
 #pragma unroll
@@ -241,7 +279,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
     for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[m][dt][e] *= inv;
-    if (A.lse && live && kw == 0 && h == 0) A.lse[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = da_lse(mx[m], l[m], DaT<T>::kP);
+    if (A.lse && live && kw == 0 && h == 0) A.lse[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = da_lse(ref[m], l[m], DaT<T>::kP);
   }
   const float* f = reinterpret_cast<const float*>(smem) + rw * DVT * 16 * 64 + lane;   // two waves: the second map's output
   if constexpr (MW > 1) {

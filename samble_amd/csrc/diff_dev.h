@@ -20,9 +20,9 @@
 // never leave registers.
 //
 // Tiles.  A tile is KT rows of two matrices X (two maps of DP elements) and Y (2 DP elements) of 16-bit operands, row-major in
-// LDS, 16-byte pieces; NP planes of each.  Piece c of a row stands at place c ^ f(row): eight rows' pieces of one column (a
-// ds_read_b128 of a wave's quarter) and four rows' pairs of pieces (a transposing read) both fall on eight different places
-// of a 128-byte line.
+// LDS, 16-byte pieces; NP planes of each.  The pieces of a 256-byte line stand at places turned by a function of the
+// line: the four pieces of four rows that half of a transposing read takes fall on sixteen different places, sixteen rows' pieces
+// of one column (a quarter of a wave's ds_read_b128) on eight.
 #pragma once
 #include "diff_args.h"
 #include "samble_dev.h"
@@ -44,6 +44,9 @@ template <typename E> using vec8 = E __attribute__((ext_vector_type(8)));
 template <typename E> using vec4 = E __attribute__((ext_vector_type(4)));
 template <typename E> using vec2 = E __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// a value that is the same in the whole wave, as one the scalar unit holds
+__device__ __forceinline__ int da_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 __device__ __forceinline__ f32x16 da_mfma(vec8<bf16> a, vec8<bf16> b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -158,35 +161,45 @@ __device__ __forceinline__ float da_row(const T* p, int n, bool live, int h, Fra
   return sc;
 }
 
-// byte offset of piece c of a row of 2 DP 16-bit elements
+// byte offset of piece c of a row of 2 DP 16-bit elements, and back from the e-th piece in LDS
+template <int DP>
+__device__ __forceinline__ int da_turn(int line) {     // what the places of a 256-byte line are turned by (bits 0, 2, 3)
+  if constexpr (DP == 16) return line & 1;                                    // four rows a line
+  else if constexpr (DP == 32) return ((line & 1) << 2) | ((line >> 1) & 1);  // two rows
+  else if constexpr (DP == 64) return ((line & 3) << 2) | ((line >> 2) & 1);  // one row
+  else return ((line & 6) << 1) | ((line >> 3) & 1);                          // half a row
+}
 template <int DP>
 __device__ __forceinline__ int da_off(int row, int c) {
-  if constexpr (DP == 16) {   // two rows of four pieces on a 128-byte line
-    const int line = row >> 1;
-    return line * 128 + (((((row & 1) << 2) | c) ^ (((line & 1) << 1) | ((line >> 1) & 1))) << 4);
-  } else {
-    return row * (4 * DP) + ((c ^ (((row & 3) << 1) | ((row >> 2) & 1))) << 4);
-  }
+  const int e = row * (DP / 4) + c, line = e >> 4;
+  return (line << 8) + (((e & 15) ^ da_turn<DP>(line)) << 4);
+}
+template <int DP>
+__device__ __forceinline__ void da_place(int e, int& row, int& c) {
+  const int line = e >> 4, q = line * 16 + ((e & 15) ^ da_turn<DP>(line));
+  row = q / (DP / 4);
+  c = q % (DP / 4);
 }
 
 // The LDS addresses a lane reads a tile's operands at: few registers, everything else is an offset of the instruction.
 template <int DP>
 struct Lane {
-  unsigned r[DP == 16 ? 2 : 4], c[DP == 16 ? 1 : 2];
+  static constexpr int NR = DP >= 64 ? 4 : DP / 16, NC = NR;
+  unsigned r[NR], c[NC];
   // row0: the wave's first row of every tile (a multiple of 32)
   __device__ __forceinline__ Lane(int lane, int row0) {
     const int h = lane >> 5, i = lane & 15;
 #pragma unroll
-    for (int k = 0; k < (DP == 16 ? 2 : 4); ++k) r[k] = da_off<DP>(lane & 31, 2 * k + h) + row0 * (4 * DP);
+    for (int k = 0; k < NR; ++k) r[k] = da_off<DP>(lane & 31, 4 * k + h) + row0 * (4 * DP);
 #pragma unroll
-    for (int v = 0; v < (DP == 16 ? 1 : 2); ++v)
+    for (int v = 0; v < NC; ++v)
       c[v] = da_off<DP>(4 * h + (i >> 2), 4 * v + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) + 8 * (i & 1) + row0 * (4 * DP);
   }
-  __device__ __forceinline__ void flip(unsigned bit) {
+  __device__ __forceinline__ void move(int bytes) {
 #pragma unroll
-    for (int k = 0; k < (DP == 16 ? 2 : 4); ++k) r[k] ^= bit;
+    for (int k = 0; k < NR; ++k) r[k] += bytes;
 #pragma unroll
-    for (int v = 0; v < (DP == 16 ? 1 : 2); ++v) c[v] ^= bit;
+    for (int v = 0; v < NC; ++v) c[v] += bytes;
   }
 };
 
@@ -198,14 +211,19 @@ struct Tile {
   typedef typename DaT<T>::E E;
   typedef __attribute__((address_space(3))) const vec8<E> lds_vec8;
 
-  // A operand, 32 rows row0 .. row0 + 31 of the wave's (a multiple of 32), step ks of the 16-deep steps along the row (X: map m starts at
-  // step m DP / 16)
+  // A operand, 32 rows row0 .. row0 + 31 of the wave's (a multiple of 32), step ks of the 16-deep steps along the row; X: of
+  // map m + (second, the same in the whole wave)
   static __device__ __forceinline__ Frag<T> rows(const Lane<DP>& L, int which, int row0, int ks) {
-    return rows_at(L.r[DP == 16 ? ks : ks & 3], which * NP, row0, ks);
+    return rows_at(L.r[(ks >> 1) & (Lane<DP>::NR - 1)], which * NP, row0, ks);
+  }
+  static __device__ __forceinline__ Frag<T> map_rows(const Lane<DP>& L, int m, int second, int row0, int ks) {
+    constexpr int KS = DP / 16, N = Lane<DP>::NR - 1;
+    const int a = m * KS + ks, b = a + KS;
+    return rows_at(second ? L.r[(b >> 1) & N] : L.r[(a >> 1) & N], 0, row0, second ? b : a);
   }
   static __device__ __forceinline__ Frag<T> rows_at(unsigned at, int plane, int row0, int ks) {
     Frag<T> f;
-    const int o = row0 * (4 * DP) + (DP == 16 ? 0 : (ks >> 2) * 128);
+    const int o = row0 * (4 * DP) + (ks & 1) * 32 + (ks >> 1) / Lane<DP>::NR * 256;
 #pragma unroll
     for (int p = 0; p < NP; ++p) f.p[p] = *(lds_vec8*)(at + (unsigned)((plane + p) * kPlane + o));
     return f;
@@ -213,9 +231,16 @@ struct Tile {
   // A operand of the transposed tile: 32 columns col0 .. (a multiple of 32), reduced rows row0 + 16 t + {4 h + 0..3,
   // 8 + 4 h + 0..3}
   static __device__ __forceinline__ Frag<T> cols(const Lane<DP>& L, int which, int row0, int t, int col0) {
+    return cols_at(L.c[(col0 >> 5) & (Lane<DP>::NC - 1)], which, row0, t, col0);
+  }
+  static __device__ __forceinline__ Frag<T> map_cols(const Lane<DP>& L, int m, int second, int row0, int t, int col0) {
+    constexpr int N = Lane<DP>::NC - 1;
+    const int a = m * DP + col0, b = a + DP;
+    return cols_at(second ? L.c[(b >> 5) & N] : L.c[(a >> 5) & N], 0, row0, t, second ? b : a);
+  }
+  static __device__ __forceinline__ Frag<T> cols_at(unsigned at, int which, int row0, int t, int col0) {
     Frag<T> f;
-    const unsigned at = L.c[DP == 16 ? 0 : (col0 >> 5) & 1];
-    const int o = (row0 + 16 * t) * (4 * DP) + (col0 >> 6) * 128;
+    const int o = (row0 + 16 * t) * (4 * DP) + col0 / 32 / Lane<DP>::NC * 256;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const unsigned b = at + (unsigned)((which * NP + p) * kPlane + o);
@@ -241,22 +266,22 @@ struct Rows {
 };
 
 // Tiles on their way from memory to LDS, NT threads together, at LDS address 0.
-//   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), two tiles: while one is computed on, the next
+//   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), NB tiles: while one is computed on, the next
 //   lands.  The 64 pieces of a wave's copy stand one behind the other in LDS, so the lane picks the piece that belongs there.
 //   fp32: through registers, where the values are scaled and split into planes; one tile.
 // use:  feed.issue(first, row0);  for each tile: { feed.next(L);  [feed.issue(following, row0)];  compute }
 // next() is a barrier of the workgroup.
-template <typename T, int DP, int KT, int NT>
+template <typename T, int DP, int KT, int NT, int NB = 2>
 struct Feed {
   typedef Tile<T, DP, KT> Tl;
   static constexpr bool DMA = Tl::NP == 1;
   static constexpr int kPieces = KT * DP / 4;                    // of X, and of Y
   static constexpr int kPer = (kPieces + NT - 1) / NT, NW = NT / 64;
-  static constexpr int kBufs = Tl::kBytes * (DMA ? 2 : 1);
-  static constexpr int kLds = kBufs + 32 + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
+  static constexpr int kBufs = Tl::kBytes * (DMA ? NB : 1);
+  static constexpr int kLds = kBufs + 16 * NB + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
   static_assert(!DMA || kPieces % 64 == 0, "whole waves copy");
-  static_assert(NT * 4 / DP % 8 == 0 || kPer == 1, "a thread's pieces stand at one place of their rows");
-  static_assert(KT <= 128 && (Tl::kBytes & (Tl::kBytes - 1)) == 0, "room for the visible rows; tiles told apart by one address bit");
+  static_assert(!DMA || NT % 256 == 0, "a thread's pieces stand at one place of their rows");
+  static_assert(KT <= 128, "room for the visible rows");
 
   char* lds;
   int tid, wave, cur;       // cur: the buffer that next() left current
@@ -266,19 +291,9 @@ struct Feed {
   Raw8<T> x[DMA ? 1 : kPer], y[DMA ? 1 : kPer];
 
   __device__ __forceinline__ Feed(char* l, int t)
-      : lds(l), tid(t), wave(__builtin_amdgcn_readfirstlane(t >> 6)), cur(0), bit(false), ux(0), uy(0), uz(0), sx(1.f), sy(1.f) {}
+      : lds(l), tid(t), wave(da_uni(t >> 6)), cur(0), bit(false), ux(0), uy(0), uz(0), sx(1.f), sy(1.f) {}
 
-  // piece e of a matrix of the tile -> its row and column piece
-  static __device__ __forceinline__ void place(int e, int& row, int& c) {
-    if constexpr (DP == 16) {
-      const int line = e >> 3, q = (e & 7) ^ (((line & 1) << 1) | ((line >> 1) & 1));
-      row = line * 2 + (q >> 2);
-      c = q & 3;
-    } else {
-      row = e / (DP / 4);
-      c = (e % (DP / 4)) ^ (((row & 3) << 1) | ((row >> 2) & 1));
-    }
-  }
+  __device__ __forceinline__ int after() const { return cur + 1 == NB ? 0 : cur + 1; }      // the buffer that issue() fills
   __device__ __forceinline__ unsigned* words(int buf) const { return reinterpret_cast<unsigned*>(lds + kBufs) + 4 * buf; }
   __device__ __forceinline__ void write_words(int buf) {
     if (tid < KT) {
@@ -297,12 +312,12 @@ struct Feed {
     const T* yt = R.y + (long)row0 * R.y_rs;
     if constexpr (DMA) {
       int row, c;
-      place(tid, row, c);
+      da_place<DP>(tid, row, c);
       const int map = c / (DP / 8), o = (c % (DP / 8)) * 8;
       // (byte offsets of a tile fit into 32 bits: rows are at most 2^23 elements apart, a map at most 2^28)
       const unsigned xo = (unsigned)(row * R.x_rs + map * (int)R.x_ms + o) * 2u, yo = (unsigned)(row * R.y_rs + c * 8) * 2u;
       constexpr int kRows = NT * 4 / DP;       // rows between a thread's pieces
-      char* l = lds + (cur ^ 1) * Tl::kBytes + 64 * wave * 16;
+      char* l = lds + after() * Tl::kBytes + 64 * wave * 16;
       if (R.d == DP && row0 + KT <= R.n && !R.mask) {      // uniform
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -321,7 +336,7 @@ struct Feed {
           copy16((const T*)(ok && c * 8 < 2 * R.d ? py : (const char*)da_zero), 0, l + NT * i * 16 + Tl::kPlane);
         }
       }
-      write_words(cur ^ 1);
+      write_words(after());
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -347,8 +362,9 @@ struct Feed {
     if constexpr (DMA) {
       between();
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      cur ^= 1;
-      L.flip(Tl::kBytes);
+      const int was = cur;
+      cur = after();
+      L.move((cur - was) * Tl::kBytes);
     } else {
       unsigned mx = 0, my = 0;
 #pragma unroll
@@ -359,7 +375,7 @@ struct Feed {
       mx = da_wave_max(mx);
       my = da_wave_max(my);
       third = da_wave_max(third);
-      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 32);
+      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 16 * NB);
       if ((tid & 63) == 0) {
         const u32x4 m = {mx, my, third, 0u};
         red[wave] = m;
@@ -372,9 +388,9 @@ struct Feed {
         uy = max(uy, m[1]);
         uz = max(uz, m[2]);
       }
-      ux = __builtin_amdgcn_readfirstlane(ux);
-      uy = __builtin_amdgcn_readfirstlane(uy);
-      uz = __builtin_amdgcn_readfirstlane(uz);
+      ux = da_uni(ux);
+      uy = da_uni(uy);
+      uz = da_uni(uz);
       sx = da_scale(ux);
       sy = da_scale(uy);
 #pragma unroll
@@ -397,7 +413,8 @@ struct Feed {
   __device__ __forceinline__ void next(Lane<DP>& L) {
     next(L, 0u, [] {});
   }
-  __device__ __forceinline__ unsigned word(int row0) const { return words(DMA ? cur : 0)[row0 >> 5]; }
+  // visible rows row0 .. row0 + 31 of the current tile, a bit each
+  __device__ __forceinline__ unsigned word(int row0) const { return da_uni(words(DMA ? cur : 0)[row0 >> 5]); }
 };
 
 template <typename T>
@@ -407,11 +424,11 @@ __device__ __forceinline__ float da_lam(const DaArgs& A, int head) {
 // keys of batch item b, and the position of its first query (keys <= position are seen); both are taken into range here, so
 // that no value of theirs reaches behind the tensors
 __device__ __forceinline__ int da_len(const DaArgs& A, int b) {
-  const int n = A.lengths ? A.lengths[b] : A.Nk;
+  const int n = da_uni(A.lengths ? A.lengths[b] : A.Nk);
   return n < 0 ? 0 : n > A.Nk ? A.Nk : n;
 }
 __device__ __forceinline__ int da_start(const DaArgs& A, int b) {      // (sizes end at 2^30: beyond that, all or none)
-  const int s = A.q_start ? A.q_start[b] : A.Nk - A.Nq;
+  const int s = da_uni(A.q_start ? A.q_start[b] : A.Nk - A.Nq);
   return s < -(1 << 30) - 1 ? -(1 << 30) - 1 : s > 1 << 30 ? 1 << 30 : s;
 }
 // keys that query i sees
