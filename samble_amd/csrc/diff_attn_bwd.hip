@@ -219,7 +219,10 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   }
 }
 
-// KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  VL: the values, a stationary operand like
+// KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  With waves along the rows the workgroups
+// are few: half of a workgroup's keys are then taken from the front and half from the back, so that under a causal mask, where
+// the first keys are seen by all rows and the last ones by few, every workgroup has the same work; the four waves of a key
+// block stand on the four SIMDs.  VL: the values, a stationary operand like
 // the keys, stay in LDS instead of registers (64-deep heads: room for a second wave on the SIMD; 128-deep: room at all).
 template <typename T, int DP, int KBW, int RWW>
 struct DkvCfg {
@@ -230,7 +233,7 @@ struct DkvCfg {
   typedef Feed<T, DP, RT, NT> Fd;
   typedef Tile<T, DP, KB> Vt;
   static constexpr int DT = DP < 32 ? 1 : DP / 32, DVT = 2 * DP / 32;
-  static constexpr int kStat = 6 * RT;       // lse_1, lse_2, t_1, t_2, limit (int), spare: floats per tile
+  static constexpr int kStat = 4 * RT;       // lse_1, lse_2, t_1, t_2 of a tile's rows
   static constexpr int kVal = VL ? DaT<T>::NP * Vt::kPlane : 0;
   static constexpr int kState = (2 * DT + DVT) * 16 * 64;
   static constexpr int kMerge = RWW > 1 ? kState * 4 * KBW : 0;      // one wave's sums per key block at a time
@@ -270,7 +273,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     return;
   }
 
-  const int wave = da_uni(tid >> 6), kb = wave % KBW, rww = RWW > 1 ? wave / KBW : 0;
+  const int wave = da_uni(tid >> 6), kb = wave / RWW, rww = RWW > 1 ? wave % RWW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
   const long units = (long)blocks * A.B * A.Hkv;
   const long unit = (long)(blockIdx.x & 7) * (main_grid / 8) + (blockIdx.x >> 3);
@@ -279,10 +282,18 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const int pair = da_uni((int)(unit / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int len = da_len(A, b);
   const int start = da_start(A, b);
-  const int key0 = blk * Cfg::KB, kw0 = key0 + 32 * kb, key = kw0 + (lane & 31);
+  // first key of the workgroup's k-th block of 32 (mirrored ones end where the blocks from the front begin: Nk, no key)
+  auto block_key = [&](int k) {
+    if (RWW == 1) return blk * Cfg::KB + 32 * k;
+    constexpr int HB = KBW / 2;
+    if (k < HB) return 32 * (blk * HB + k);
+    const int back = (A.Nk + 31) / 32 - 1 - (blk * HB + k - HB);
+    return back >= (int)blocks * HB ? 32 * back : A.Nk;
+  };
+  const int key0 = block_key(0), kw0 = block_key(kb), key = kw0 + (lane & 31);
   const unsigned char* km = A.key_mask ? A.key_mask + b * A.km_bs : nullptr;
   const bool valid = key < len && (!km || km[key]);
-  const bool all_valid = __all(valid);
+  const bool all_valid = __all(valid), any_valid = __any(valid);
 
   // rows that see any key of the workgroup: all behind the first such query
   const long i0 = A.causal && key0 > start ? (long)key0 - start : 0;
@@ -293,22 +304,36 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const T* gb = (const T*)A.dout + b * A.g_bs + (long)hk * A.G * A.g_hs;
   Fd feed(smem, tid);
   Lane<DP> L(lane, 32 * rww);
-  float sv[5] = {0.f, 0.f, 0.f, 0.f, 0.f}, gn = 0.f;
+  // the rows' statistics go with their tile: copied like it (fp16 / bf16; rows behind the last: zeros), or through registers,
+  // where they take on the scales (fp32; rows behind the last: P = 0)
+  float sv[4] = {0.f, 0.f, 0.f, 0.f}, gn = 0.f;
+  int buf = 1;               // the statistics that are current; issue() fills the other ones
   auto issue = [&](int g, int t) {
     src.x = qb + g * A.q_hs;
     src.y = gb + g * A.g_hs;
     feed.issue(src, t * RT);
-    if (tid < RT) {
+    const long hd = (long)b * A.H + hk * A.G + g;
+    const float *ls = A.lse + hd * 2 * A.Nq, *tt = A.delta + hd * 2 * A.Nq;
+    if constexpr (Fd::DMA) {
+      float* to = stats + (buf ^ 1) * Cfg::kStat;
+#pragma unroll
+      for (int x = 0; x < 4 * RT / 64; x += Cfg::NW) {
+        if (x + wave >= 4 * RT / 64) break;
+        const int f = (x + wave) * 64 + lane, row = f % RT, i = t * RT + row;
+        const float* from = f < 2 * RT ? ls : tt;
+        if ((f / RT) & 1) from += A.Nq;
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(i < A.Nq ? from + i : reinterpret_cast<const float*>(da_zero)),
+            (__attribute__((address_space(3))) void*)(to + (x + wave) * 64), 4, 0, 0);
+      }
+    } else if (tid < RT) {
       const int i = t * RT + tid;
       const bool ok = i < A.Nq;
-      const long hd = (long)b * A.H + hk * A.G + g;
-      const float *ls = A.lse + hd * 2 * A.Nq, *tt = A.delta + hd * 2 * A.Nq;
-      sv[0] = ok ? ls[i] : __builtin_huge_valf();     // (rows behind the last: P = 0)
+      sv[0] = ok ? ls[i] : __builtin_huge_valf();
       sv[1] = ok ? (ls + A.Nq)[i] : __builtin_huge_valf();
       sv[2] = ok ? tt[i] : 0.f;
       sv[3] = ok ? (tt + A.Nq)[i] : 0.f;
-      sv[4] = __int_as_float(ok ? da_limit(A, len, start, i) : 0);
-      if (DaT<T>::NP == 2) gn = ok ? A.delta[2l * A.B * A.H * A.Nq + hd * A.Nq + i] : 0.f;
+      gn = ok ? A.delta[2l * A.B * A.H * A.Nq + hd * A.Nq + i] : 0.f;
     }
   };
   if (tile0 < per_head) issue(0, tile0);
@@ -356,7 +381,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     }
     if constexpr (Cfg::VL) {
       for (int e = tid; e < Cfg::KB * DP / 4; e += NT) {
-        const int row = e / (DP / 4), pc = e % (DP / 4), kk = key0 + row;
+        const int row = e / (DP / 4), pc = e % (DP / 4), kk = block_key(row >> 5) + (row & 31);
         Raw8<T> raw;
         raw.load(vp + (long)kk * A.v_rs + pc * 8, kk < len && (!km || km[kk]) && pc * 8 < 2 * A.d);
         const Frag<T> f = raw.frag(vscale);
@@ -383,11 +408,11 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   float fscale = 1.f, qscale = 1.f, gscale = 1.f;
   bool fresh = true;
 
-  int buf = 0, g = 0, t = tile0;
+  int g = 0, t = tile0;
   while (t < per_head) {
     const float lam = da_lam<T>(A, hk * A.G + g);
-    float* stat = stats + buf * Cfg::kStat;
     buf ^= 1;
+    float* stat = stats + buf * Cfg::kStat;
     feed.next(L, __float_as_uint(gn), [&] {
       if (DaT<T>::NP == 2) {
         const float f = 0.5f * da_scale(__float_as_uint(__uint_as_float(feed.uz) * vnorm));
@@ -415,11 +440,12 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         sv[2] *= fscale;
         sv[3] *= fscale;
       }
-      if (tid < RT) {
+      if (!Fd::DMA && tid < RT) {
 #pragma unroll
-        for (int e = 0; e < 5; ++e) stat[e * RT + tid] = sv[e];
+        for (int e = 0; e < 4; ++e) stat[e * RT + tid] = sv[e];
       }
     });
+    const int here = t;
     // the tile behind this one
     if (++t == per_head && ++g < A.G) t = tile0;
     if (t < per_head) issue(g, t);
@@ -427,6 +453,9 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
         const int row0 = 32 * (rww + sub);
+        const int i0 = here * RT + row0;
+        // (uniform in the wave; a workgroup of neighbouring keys has hardly such a step)
+        if (RWW > 1 && (!any_valid || i0 >= A.Nq || da_limit(A, len, start, min(i0 + 31, A.Nq - 1)) <= kw0)) continue;
         f32x16 da = zero16();
 #pragma unroll
         for (int ks = 0; ks < 2 * KS; ++ks) {
@@ -437,63 +466,57 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
             da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), vf[ks], da);
           }
         }
-        const int fewest = __builtin_amdgcn_readfirstlane(__float_as_int(stat[4 * RT + row0]));   // (limits rise with the row)
-        const bool masked = !all_valid || kw0 + 32 > fewest;
-        f32x16 p1;
-        Frag<T> f[2][2], af[2];
+        // row i sees the key if i is at least `from`; rows behind the last see nothing
+        const int from = key - start;
+        const bool masked = !all_valid || (A.causal && kw0 + 31 - start > i0) || i0 + 32 > A.Nq;
+        f32x16 s[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          f32x16 s = zero16();
+          s[m] = zero16();
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, 32 * sub, m * KS + ks), kf[m][ks], s);
-          const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
-          if (masked) {       // (what a row does not see: exp2 gives 0)
-            int mine = valid ? key : 0x7fffffff;
-            asm volatile("" : "+v"(mine));
+          for (int ks = 0; ks < KS; ++ks) s[m] = da_mma<T>(Tl::rows(L, 0, 32 * sub, m * KS + ks), kf[m][ks], s[m]);
+        }
+        if (masked) {       // (what a row does not see: exp2 gives 0)
+          int low = !valid ? 32 : A.causal ? from - i0 - 4 * h : -32, end = A.Nq - i0 - 4 * h;
+          asm volatile("" : "+v"(low), "+v"(end));
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              const f32x4 lt = *reinterpret_cast<const f32x4*>(stat + 4 * RT + row0 + 8 * q4 + 4 * h);
+          for (int e = 0; e < 16; ++e) {
+            const bool see = crow(e, 0) >= low && crow(e, 0) < end;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[4 * q4 + e] = mine < __float_as_int(lt[e]) ? s[4 * q4 + e] : kNegInf;
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float d[8], a[8];
-#pragma unroll
-            for (int q4 = 0; q4 < 2; ++q4) {
-              const int at = row0 + 16 * u + 8 * q4 + 4 * h;
-              const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + m * RT + at);
-              const f32x4 tt = *reinterpret_cast<const f32x4*>(stat + (2 + m) * RT + at);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int i = 8 * u + 4 * q4 + e;
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i], cm, -ls[e]));
-                const float dt = DaT<T>::NP == 2 ? fmaf(da[i], a1, -tt[e]) : da[i] - tt[e];
-                if (m == 0) {
-                  p1[i] = p0;
-                  d[4 * q4 + e] = p0 * dt;
-                } else {
-                  const float p = p0 * lam;
-                  a[4 * q4 + e] = p1[i] - p;
-                  d[4 * q4 + e] = -p * dt;
-                }
-              }
-            }
-            f[m][u] = da_pack<T>(d);
-            if (m == 1) af[u] = da_pack<T>(a);
+            for (int m = 0; m < 2; ++m) s[m][e] = see ? s[m][e] : kNegInf;
           }
         }
+        float cm[2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) cm[m] = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
+        // half of the rows at a time: their products run under the other half's exponentials
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+          float a[8], d1[8], d2[8];
 #pragma unroll
-          for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(L, 1, 32 * sub, u, 32 * dt), af[u], dv[dt]);
+          for (int q4 = 0; q4 < 2; ++q4) {
+            const float* at = stat + row0 + 16 * u + 8 * q4 + 4 * h;
+            const f32x4 l1 = *reinterpret_cast<const f32x4*>(at), l2 = *reinterpret_cast<const f32x4*>(at + RT);
+            const f32x4 t1 = *reinterpret_cast<const f32x4*>(at + 2 * RT), t2 = *reinterpret_cast<const f32x4*>(at + 3 * RT);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 8 * u + 4 * q4 + e, j = 4 * q4 + e;
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], cm[0], -l1[e]));
+              const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][i], cm[1], -l2[e]));
+              a[j] = p1 - p2;
+              d1[j] = p1 * (DaT<T>::NP == 2 ? fmaf(da[i], a1, -t1[e]) : da[i] - t1[e]);
+              d2[j] = p2 * (DaT<T>::NP == 2 ? fmaf(da[i], -a1, t2[e]) : t2[e] - da[i]);
+            }
+          }
+          const Frag<T> af = da_pack<T>(a), f1 = da_pack<T>(d1), f2 = da_pack<T>(d2);
+#pragma unroll
+          for (int dt = 0; dt < DVT; ++dt) dv[dt] = da_mma<T>(Tl::cols(L, 1, 32 * sub, u, 32 * dt), af, dv[dt]);
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
             const Frag<T> q1 = Tl::cols(L, 0, 32 * sub, u, 32 * dt);
-            dk[0][dt] = da_mma<T>(q1, f[0][u], dk[0][dt]);
+            dk[0][dt] = da_mma<T>(q1, f1, dk[0][dt]);
             const Frag<T> q2 = DP < 32 ? q1 : Tl::cols(L, 0, 32 * sub, u, DP + 32 * dt);
-            dk[1][dt] = da_mma<T>(q2, f[1][u], dk[1][dt]);
+            dk[1][dt] = da_mma<T>(q2, f2, dk[1][dt]);
           }
         }
     }

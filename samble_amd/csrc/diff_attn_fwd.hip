@@ -16,6 +16,7 @@ namespace samble {
 template <typename T, int DP, int RW, int KW, int MW>
 struct FwdCfg {
   static constexpr int NW = RW * KW * MW, NT = 64 * NW;
+  static constexpr bool AHEAD = MW > 1 || DP < 64;            // the next step's logits before this one's exponentials (registers)
   static constexpr int SUB = KW > 1 ? 1 : 2;                  // 32-key steps of a wave per tile
   static constexpr int KT = 32 * KW * SUB;
   static constexpr int DVT = 2 * DP / 32, MPW = 2 / MW;      // 32-column pieces of an output, maps of a wave
@@ -200,9 +201,10 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
       const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;
       if (word != 0xffffffffu || k0 + 32 > kmin) hide(s[sub & 1], k0, word);
       refer(s[sub & 1]);
-      if (sub + 1 < Cfg::SUB) logits(L, 32 * (sub + 1), s[(sub + 1) & 1]);
+      if (Cfg::AHEAD && sub + 1 < Cfg::SUB) logits(L, 32 * (sub + 1), s[(sub + 1) & 1]);
       weigh(s[sub & 1], pf);
       values(L, 32 * sub);
+      if (!Cfg::AHEAD && sub + 1 < Cfg::SUB) logits(L, 32 * (sub + 1), s[(sub + 1) & 1]);
     }
   }
 #pragma unroll
@@ -340,7 +342,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DaArgs A) {
       if (m[k] == kNegInf) m[k] = 0.f;
     }
     float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, l[2] = {0.f, 0.f};
-    for (int s = wave; s < A.splits; s += 4) {
+#pragma unroll 4
+    for (int s = wave; s < A.splits; s += 4) {      // (four splits' loads in flight)
       const float* p = w + s * step;
       const f32x4 t = *reinterpret_cast<const f32x4*>(p);
       const float a0 = __builtin_amdgcn_exp2f(t[0] - m[0]), a1 = __builtin_amdgcn_exp2f(t[2] - m[1]);
