@@ -26,10 +26,6 @@ struct FwdCfg {
   static constexpr int kLds = Fd::kLds > kMergeBytes ? Fd::kLds : kMergeBytes;
 };
 
-// waves per SIMD that the registers are held to: two, so that one wave's matrix instructions run under the other's
-// exponentials (and the whole file of 512 would put every accumulator into the half that the vector unit cannot read)
-template <typename T, int DP> struct FwdWaves { static constexpr int value = 2; };
-
 // partial results of a split: per row (row order of the pair) m_1, l_1, m_2, l_2, then O_1, O_2 (2 d each)
 __device__ __forceinline__ long da_part_floats(int d) { return 4 + 4l * d; }
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }   // (0 for a row without keys, NaN stays)
@@ -37,8 +33,10 @@ __device__ __forceinline__ float da_lse(float m, float l, int shift) {      // l
   return l == 0.f ? __builtin_huge_valf() : m - (float)shift + __builtin_amdgcn_logf(l);
 }
 
+// (Registers are held to two waves per SIMD, so that one wave's matrix instructions run under the other's exponentials; the
+// whole file of 512 would put every accumulator into the half that the vector unit cannot read.)
 template <typename T, int DP, int RW, int KW, int MW>
-__global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void diff_fwd_kernel(DaArgs A) {
+__global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A) {
   typedef FwdCfg<T, DP, RW, KW, MW> Cfg;
   typedef typename Cfg::Fd Fd;
   typedef typename Fd::Tl Tl;
@@ -318,15 +316,17 @@ __global__ __launch_bounds__(64 * RW * KW * MW, (FwdWaves<T, DP>::value)) void d
     }
 }
 
-// adds the splits of a row: a workgroup per row, its waves take every fourth split, a lane every 64th column
-template <typename T>
-__global__ __launch_bounds__(256) void diff_join_kernel(DaArgs A) {
-  __shared__ float red[4][2][256 + 1];
+// adds the splits of a row.  NW = 16: a workgroup per row, a wave takes every sixteenth split (many splits, few rows); NW = 1:
+// a wave per row.  A lane takes four columns.
+template <typename T, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaArgs A) {
+  __shared__ float red[NW == 1 ? 1 : NW][2][NW == 1 ? 4 : 256 + 4];
   const unsigned rows = (unsigned)A.Nq * A.G;
   const long all = (long)rows * A.B * A.Hkv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cols = 2 * A.d;
+  const int lane = threadIdx.x & 63, wave = da_uni(threadIdx.x >> 6), cols = 2 * A.d;
   const long pf = da_part_floats(A.d), step = all * pf;
-  for (long u = blockIdx.x; u < all; u += gridDim.x) {
+  constexpr int RPB = NW == 1 ? 4 : 1;
+  for (long u = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); u < all; u += (long)gridDim.x * RPB) {
     const unsigned pair = (unsigned)(u / rows), r = (unsigned)(u % rows);
     const int b = pair / A.Hkv, hk = pair % A.Hkv, qi = (int)(r / (unsigned)A.G), head = hk * A.G + (int)(r % (unsigned)A.G);
     const float* w = A.part + u * pf;
@@ -341,68 +341,84 @@ __global__ __launch_bounds__(256) void diff_join_kernel(DaArgs A) {
       m[k] = wave_max64(m[k]);
       if (m[k] == kNegInf) m[k] = 0.f;
     }
-    float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, l[2] = {0.f, 0.f};
-#pragma unroll 4
-    for (int s = wave; s < A.splits; s += 4) {      // (four splits' loads in flight)
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[2] = {none, none};
+    float l[2] = {0.f, 0.f};
+    const int c4 = 4 * lane < cols ? 4 * lane : 0;      // (lanes behind the last column: the first ones again, not used)
+#pragma unroll(NW == 1 ? 4 : 2)
+    for (int s = NW == 1 ? 0 : wave; s < A.splits; s += NW) {
       const float* p = w + s * step;
-      const f32x4 t = *reinterpret_cast<const f32x4*>(p);
+      const f32x4 t = *reinterpret_cast<const f32x4*>(p), x = *reinterpret_cast<const f32x4*>(p + 4 + c4);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(p + 4 + cols + c4);
       const float a0 = __builtin_amdgcn_exp2f(t[0] - m[0]), a1 = __builtin_amdgcn_exp2f(t[2] - m[1]);
       l[0] = fmaf(t[1], a0, l[0]);
       l[1] = fmaf(t[3], a1, l[1]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = lane + 64 * k;
-        if (c < cols) {
-          acc[0][k] = fmaf(p[4 + c], a0, acc[0][k]);
-          acc[1][k] = fmaf(p[4 + cols + c], a1, acc[1][k]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        acc[0][e] = fmaf(x[e], a0, acc[0][e]);
+        acc[1][e] = fmaf(y[e], a1, acc[1][e]);
       }
     }
+    if constexpr (NW > 1) {      // onto the first wave, in order
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < 2; ++k) {
+        *reinterpret_cast<f32x4*>(&red[wave][k][4 * lane]) = acc[k];
+        if (lane == 0) red[wave][k][256] = l[k];
+      }
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll 1
+        for (int i = 1; i < NW; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) red[wave][k][lane + 64 * j] = acc[k][j];
-      if (lane == 0) red[wave][k][256] = l[k];
+          for (int k = 0; k < 2; ++k) {
+            l[k] += red[i][k][256];
+            acc[k] += *reinterpret_cast<const f32x4*>(&red[i][k][4 * lane]);
+          }
+      }
     }
-    __syncthreads();
-    const int c = threadIdx.x;
-    float v[2];
+    if (NW == 1 || wave == 0) {
+      if (4 * lane < cols) {
+        const float i1 = da_inv(l[0]), i2 = da_inv(l[1]), lam = da_lam<T>(A, head);
+        const long o = (((long)b * A.Nq + qi) * A.H + head) * cols + 4 * lane;
+        typedef T vec __attribute__((ext_vector_type(4)));
+        vec a, z;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      l[k] = (red[0][k][256] + red[1][k][256]) + (red[2][k][256] + red[3][k][256]);
-      v[k] = ((red[0][k][c] + red[1][k][c]) + (red[2][k][c] + red[3][k][c])) * da_inv(l[k]);
-      if (A.lse && c == 0) A.lse[(((long)b * A.H + head) * 2 + k) * A.Nq + qi] = da_lse(m[k], l[k], DaT<T>::kP);
+        for (int e = 0; e < 4; ++e) {
+          const float v2 = acc[1][e] * i2;
+          a[e] = (T)fmaf(-lam, v2, acc[0][e] * i1);
+          z[e] = (T)v2;
+        }
+        *reinterpret_cast<vec*>((T*)A.out + o) = a;
+        if (A.out2) *reinterpret_cast<vec*>((T*)A.out2 + o) = z;
+      }
+      if (A.lse && lane == 0) {
+        float* ls = A.lse + ((long)b * A.H + head) * 2 * A.Nq + qi;
+        ls[0] = da_lse(m[0], l[0], DaT<T>::kP);
+        ls[A.Nq] = da_lse(m[1], l[1], DaT<T>::kP);
+      }
     }
-    if (c < cols) {
-      const long o = (((long)b * A.Nq + qi) * A.H + head) * cols + c;
-      ((T*)A.out)[o] = (T)fmaf(-da_lam<T>(A, head), v[1], v[0]);
-      if (A.out2) ((T*)A.out2)[o] = (T)v[1];
-    }
-    __syncthreads();
+    if (NW > 1) __syncthreads();
   }
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
 struct FwdPlan { bool few; long blocks; int splits; };
 
-// Few rows (at most 32 of a key head) take the kernels whose waves stand along the keys.  Splits: workgroups for two rounds of
-// the 256 CUs when rows and heads alone give fewer, each split with at least four tiles of 128 keys (a split costs its
-// partial results' way through memory), at most 128.
-static FwdPlan fwd_plan(int B, int Nq, int Nk, int H, int Hkv) {
+// Few rows (at most 32 of a key head) take the kernels whose waves stand along the keys.  Splits: as many as fill the waves that
+// the card holds at once (two workgroups of four waves to a CU, one of eight) and no more, since a part of a second round costs
+// a whole one (8 clouds of 1999 points, one head, fp32, d 64: 2 splits 113 us, 3 splits 138 us); each split has
+// at least four tiles of 128 keys (a split costs its partial results' way through memory), at most 128.
+static FwdPlan fwd_plan(bool wide, int B, int Nq, int Nk, int H, int Hkv, int d) {
   const long rows = (long)Nq * (H / Hkv), pairs = (long)B * Hkv;
   FwdPlan p;
   p.few = rows <= 32;
   p.blocks = p.few ? 1 : (rows + 127) / 128;
-  const long have = p.blocks * pairs;
-  long s = 1;
-  if (have < 256) {
-    s = (512 + have - 1) / have;
-    const long most = Nk / 512;
-    if (s > most) s = most;
-    if (s > 128) s = 128;
-    if (s < 1) s = 1;
-  }
-  p.splits = (int)s;
+  const long have = p.blocks * pairs, room = !p.few && d > (wide ? 32 : 64) ? 256 : 512;
+  long s = room / have;
+  const long most = Nk / 512;
+  if (s > most) s = most;
+  if (s > 128) s = 128;
+  p.splits = s < 1 ? 1 : (int)s;
   return p;
 }
 
@@ -423,21 +439,25 @@ static int fwd_go(const DaArgs& A, hipStream_t s) {
 
 template <typename T>
 static int fwd_type(DaArgs& A, hipStream_t s) {
-  const FwdPlan p = fwd_plan(A.B, A.Nq, A.Nk, A.H, A.Hkv);
+  const FwdPlan p = fwd_plan(DaT<T>::NP == 2, A.B, A.Nq, A.Nk, A.H, A.Hkv, A.d);
   A.splits = p.splits;
   constexpr bool F = DaT<T>::NP == 2;
   int rc = -22;
   if (A.d <= 16) rc = p.few ? fwd_go<T, 16, 1, 4, 1>(A, s) : fwd_go<T, 16, 4, 1, 1>(A, s);
-  else if (A.d <= 32) rc = p.few ? fwd_go<T, 32, 1, 4, 1>(A, s) : fwd_go<T, 32, 4, 1, 1>(A, s);
+  else if (A.d <= 32) rc = p.few ? fwd_go<T, 32, 1, 2, 2>(A, s) : fwd_go<T, 32, 4, 1, 1>(A, s);
   else if (A.d <= 64) {
     if constexpr (F) rc = p.few ? fwd_go<T, 64, 1, 2, 2>(A, s) : fwd_go<T, 64, 4, 1, 2>(A, s);
-    else rc = p.few ? fwd_go<T, 64, 1, 4, 1>(A, s) : fwd_go<T, 64, 4, 1, 1>(A, s);
+    else rc = p.few ? fwd_go<T, 64, 1, 2, 2>(A, s) : fwd_go<T, 64, 4, 1, 1>(A, s);
   } else if constexpr (!F) {
     if (A.d <= 128) rc = p.few ? fwd_go<T, 128, 1, 2, 2>(A, s) : fwd_go<T, 128, 4, 1, 2>(A, s);
   }
   if (rc || A.splits == 1) return rc;
   const long all = (long)A.Nq * A.H * A.B;
-  hipLaunchKernelGGL((diff_join_kernel<T>), dim3((unsigned)(all < (1 << 20) ? all : (1 << 20))), dim3(256), 0, s, A);
+  const long most = 1 << 20;      // workgroups of a launch: the kernel walks on
+  if (A.splits >= 16)
+    hipLaunchKernelGGL((diff_join_kernel<T, 16>), dim3((unsigned)(all < most ? all : most)), dim3(1024), 0, s, A);
+  else
+    hipLaunchKernelGGL((diff_join_kernel<T, 1>), dim3((unsigned)((all + 3) / 4 < most ? (all + 3) / 4 : most)), dim3(256), 0, s, A);
   return (int)hipGetLastError();
 }
 
@@ -446,8 +466,7 @@ static int fwd_type(DaArgs& A, hipStream_t s) {
 using namespace samble;
 
 extern "C" size_t samble_diff_fwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d) {
-  (void)type;
-  const FwdPlan p = fwd_plan(B, Nq, Nk, H, Hkv);
+  const FwdPlan p = fwd_plan(type == 0, B, Nq, Nk, H, Hkv, d);
   return p.splits == 1 ? 0 : (size_t)p.splits * B * H * Nq * (4 + 4l * d) * sizeof(float);
 }
 

@@ -82,7 +82,15 @@ __device__ __forceinline__ Frag<T> da_pack(const float (&v)[8]) {
     f.p[0][e] = h[0];
     f.p[0][e + 1] = h[1];
     if constexpr (DaT<T>::NP == 2) {
-      const f32x2 r = {fmaf((float)h[0], -1.f, v[e]), fmaf((float)h[1], -1.f, v[e + 1])};
+      // what the first plane leaves, exactly; v_fma_mix widens the fp16 factor itself (the compiler takes two instructions).
+      // The asm reads vector results only, and v[] not before the conversion above did.
+      f32x2 r;
+      float r0, r1;
+      const unsigned hh = __builtin_bit_cast(unsigned, h);
+      asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hh), "v"(v[e]));
+      asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hh), "v"(v[e + 1]));
+      r[0] = r0;
+      r[1] = r1;
       const vec2<E> l = __builtin_convertvector(r, vec2<E>);
       f.p[1][e] = l[0];
       f.p[1][e + 1] = l[1];
