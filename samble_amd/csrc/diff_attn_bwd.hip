@@ -3,7 +3,10 @@
 //     dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P_1 - lam P_2)^T g,  dlam = - sum_i t_2
 // The logits are formed again from q and k; P = exp2(logit - lse) with the forward's row statistics.  Two launches, no atomics:
 //   diff_dq_kernel   a wave owns 32 rows (layout of the forward): first t_1 = g . out + lam t_2 and t_2 = g . out2 from the
-//                    saved outputs, kept for the second launch, then one sweep over the keys
+//                    saved outputs, then one sweep over the keys.  16-bit outputs are rounded, and so is a t of them; since
+//                    sum_j P = 1, sum_j P (dA - t) is what it lacks, and t plus that sum is kept for the second launch
+//                    (dlam adds t over all rows: there the roundings of 2^-9 or 2^-12 would not be small beside a sum of
+//                    both signs)
 //   diff_dkv_kernel  a wave owns 32 keys and sweeps over the rows of all query heads that share the key head; workgroups
 //                    behind the last one sum dlam
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
@@ -92,13 +95,13 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
     dot[0] = fmaf(lam, dot[1], dot[0]);
     if (DaT<T>::NP == 2) norm = da_xor32_sum(norm);
   }
-  float lse[MPW], tm[MPW];
+  float lse[MPW], tm[MPW], lack[MPW];
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
     const long at = (((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi;
     lse[m] = live ? A.lse[at] : __builtin_huge_valf();
     tm[m] = MPW == 2 ? dot[m] : mw ? dot[1] : dot[0];
-    if (live && h == 0) A.delta[at] = tm[m];
+    lack[m] = 0.f;
   }
   if (DaT<T>::NP == 2 && live && h == 0 && mw == 0)
     A.delta[2l * A.B * A.H * A.Nq + ((long)b * A.H + head) * A.Nq + qi] = sqrtf(norm);
@@ -183,6 +186,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             p[e] = s[8 * u + e] * (DaT<T>::NP == 2 ? fmaf(da[8 * u + e], a1, -tm[m] * fscale) : da[8 * u + e] - tm[m]);
+          if (DaT<T>::NP == 1) lack[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           ds[m][u] = da_pack<T>(p);
         }
       }
@@ -198,6 +202,11 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
           }
         }
     }
+  }
+#pragma unroll
+  for (int m = 0; m < MPW; ++m) {
+    if (DaT<T>::NP == 1) tm[m] += da_xor32_sum(lack[m]);
+    if (live && h == 0) A.delta[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = tm[m];
   }
   if (!live) return;
   T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d + mw * A.d;

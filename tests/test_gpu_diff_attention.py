@@ -2,7 +2,7 @@
 
 Tolerances are sums of the roundings that the kernels are allowed, per element:
   * U = 2^-24 arithmetic.  A dot product of n terms in fp32 is off by at most (n + 32) U times the sum of magnitudes (fp32
-    tensors: the three bf16 planes and six products lose a few U of the same sum, inside the 32).  With L the largest such sum
+    tensors: the two fp16 planes and three products lose a few U of the same sum, inside the 32).  With L the largest such sum
     over a row's logits, a probability is off by the factor 2 * ((d + 32) U L + 16 U); sums over n keys or rows by n U.
   * h = eps / 2 of the tensors' type: P, P_1 - lam P_2 and dS enter the second products rounded once (fp16 / bf16 only; fp32
     enters whole), saved outputs and results are rounded once.  fp16 adds half a subnormal step, 2^-25, where values are small.
@@ -240,6 +240,29 @@ def test_nothing_of_missing_keys_is_used(dtype):
     out, dq, dk, dv, _ = res[0]
     assert not out[1].any() and not dq[1].any()
     assert not dk[gone].any() and not dv[gone].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_dlam_is_not_that_of_rounded_outputs(dtype, d):
+    """Values 1 and 1 + eps, two in five of them the larger: every output of the second map is 1 + 0.4 eps, which the tensors'
+    type rounds to 1 in all rows and columns.  With q = 0 the maps are uniform, and dlam = - Nq 2 d (1 + 0.4 eps) but for fp32
+    sums over 2 d columns, Nk keys and Nq rows and a few steps each for the map, its normaliser and t."""
+    from samble_amd.attention import differential_attention
+
+    dt = TYPES[dtype]
+    Nq, Nk = 40, 320
+    eps = torch.finfo(dt).eps
+    larger = torch.tensor([0.0, 0.0, 1.0, 0.0, 1.0], device=DEV).repeat(Nk // 5)
+    q = torch.zeros(1, Nq, 1, 2, d, dtype=dt, device=DEV)
+    k = torch.ones(1, Nk, 1, 2, d, dtype=dt, device=DEV)
+    v = (1 + eps * larger).to(dt)[None, :, None, None].expand(1, Nk, 1, 2 * d).contiguous()
+    lam = torch.full((1,), 0.5, device=DEV, requires_grad=True)
+    out = differential_attention(q, k, v, lam)
+    (dlam,) = torch.autograd.grad(out, lam, torch.ones_like(out))
+    ref = -Nq * 2 * d * (1 + 0.4 * eps)
+    assert abs(dlam.item() - ref) <= (2 * d + Nk + Nq + 96) * U * abs(ref)
 
 
 @pytest.mark.gpu
