@@ -58,6 +58,25 @@ __device__ __forceinline__ void ln_store(T* p, long n, const float (&v)[LnT<T>::
       if (e < n) p[e] = (T)v[e];
   }
 }
+// a piece as it stands in memory, and its values: for what is read ahead (4 registers a piece whatever the type)
+template <typename T>
+__device__ __forceinline__ u32x4 ln_piece(const T* p, long n) {
+  constexpr int V = LnT<T>::V;
+  typedef T vec __attribute__((ext_vector_type(V)));
+  if (n >= V) return *reinterpret_cast<const typename LnT<T>::piece*>(p);
+  vec t;
+#pragma unroll
+  for (int e = 0; e < V; ++e) t[e] = e < n ? p[e] : (T)0.f;
+  return __builtin_bit_cast(u32x4, t);
+}
+template <typename T>
+__device__ __forceinline__ void ln_widen(const u32x4& raw, float (&v)[LnT<T>::V]) {
+  constexpr int V = LnT<T>::V;
+  typedef T vec __attribute__((ext_vector_type(V)));
+  const vec t = __builtin_bit_cast(vec, raw);
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = (float)t[e];
+}
 // weight / bias: fp32 or the tensors' type (one uniform branch); null: `none`
 template <typename T>
 __device__ __forceinline__ void ln_load_w(const void* w, int w_f32, long c, long n, float none, float (&v)[LnT<T>::V]) {
@@ -94,7 +113,7 @@ __device__ __forceinline__ void ln_sum2(float& a, float& b, float* red) {
   }
   if constexpr (TPR > 64) {
     constexpr int NW = TPR / 64;
-    const int w = threadIdx.x >> 6;
+    const int w = (threadIdx.x % TPR) >> 6;
     if ((threadIdx.x & 63) == 0) {
       red[w] = a;
       red[NW + w] = b;
@@ -122,81 +141,117 @@ struct LnArgs {
 };
 
 // ---- rows (inner == 1) ---------------------------------------------------------------------------------------------------
+// A workgroup walks the rows blockIdx.x * RPB + slot, + gridDim.x * RPB, ...  The columns of a thread stay the same, so that
+// weight and bias stay in its registers, and the next row is read while the sums of this one are formed.
 template <typename T, int TPR, int P>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_fwd_kernel(LnArgs A) {
   constexpr int V = LnT<T>::V, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
   __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
   const int t = threadIdx.x % TPR;
-  for (long r0 = (long)blockIdx.x * RPB; r0 < A.outer; r0 += (long)gridDim.x * RPB) {
-  const long row = r0 + threadIdx.x / TPR;
-  const bool live = row < A.outer;      // (uniform over the threads of a row; a workgroup per row has no dead rows)
-  const T* x = (const T*)A.x + (live ? row : 0) * A.x_os;
-  float v[P][V];
-  float sum = 0.f, sq = 0.f;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const long c = (long)(p * TPR + t) * V, n = live ? A.C - c : 0;
-    ln_load<T>(x + c, n, v[p]);
-  }
-  if (A.res) {
-    const T* r = (const T*)A.res + (live ? row : 0) * A.res_os;
-    T* s = (T*)A.s + (live ? row : 0) * A.C;
+  const long step = (long)gridDim.x * RPB;
+  long row = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  u32x4 xr[P], rr[P];
+  auto fetch = [&](long row) {
+    const long at = row < A.outer ? row : 0;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const long c = (long)(p * TPR + t) * V, n = live ? A.C - c : 0;
-      float q[V];
-      ln_load<T>(r + c, n, q);
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[p][e] = (float)(T)(v[p][e] + q[e]);
-      ln_store<T>(s + c, n, v[p]);
+      const long c = (long)(p * TPR + t) * V, n = row < A.outer ? A.C - c : 0;
+      xr[p] = ln_piece<T>((const T*)A.x + at * A.x_os + c, n);
+      if (A.res) rr[p] = ln_piece<T>((const T*)A.res + at * A.res_os + c, n);
     }
-  }
-#pragma unroll
-  for (int p = 0; p < P; ++p)
-#pragma unroll
-    for (int e = 0; e < V; ++e) sum += v[p][e];
-  ln_sum2<TPR>(sum, sq, red);
-  const float cc = (float)A.C, mean = sum / cc;   // (a quotient: a constant row has its own value as mean)
-  sq = 0.f;
+  };
+  fetch(row);
+  float w[P][V], b[P][V];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const long c = (long)(p * TPR + t) * V;
+    ln_load_w<T>(A.w, A.w_f32, c, A.C - c, 1.f, w[p]);
+    ln_load_w<T>(A.b, A.w_f32, c, A.C - c, 0.f, b[p]);
+  }
+  const float cc = (float)A.C;
+  for (long r0 = (long)blockIdx.x * RPB; r0 < A.outer; r0 += step, row += step) {
+    const bool live = row < A.outer;      // (uniform over the threads of a row; a workgroup per row has no dead rows)
+    float v[P][V];
+    float sum = 0.f, sq = 0.f;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[p][e] -= mean;
-      if (c + e < A.C) sq = fmaf(v[p][e], v[p][e], sq);
+    for (int p = 0; p < P; ++p) ln_widen<T>(xr[p], v[p]);
+    if (A.res) {
+      T* s = (T*)A.s + (live ? row : 0) * A.C;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const long c = (long)(p * TPR + t) * V;
+        float q[V];
+        ln_widen<T>(rr[p], q);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[p][e] = (float)(T)(v[p][e] + q[e]);
+        ln_store<T>(s + c, live ? A.C - c : 0, v[p]);
+      }
     }
-  }
-  sum = 0.f;
-  ln_sum2<TPR>(sq, sum, red);
-  const float rstd = 1.f / sqrtf(sq / cc + A.eps);
-  if (!live) continue;
-  if (t == 0 && A.mean) {
-    A.mean[row] = mean;
-    A.rstd[row] = rstd;
-  }
-  T* y = (T*)A.y + row * A.C;
+    if (r0 + step < A.outer) fetch(row + step);
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const long c = (long)(p * TPR + t) * V, n = A.C - c;
-    if (n <= 0) break;
-    float w[V], b[V], o[V];
-    ln_load_w<T>(A.w, A.w_f32, c, n, 1.f, w);
-    ln_load_w<T>(A.b, A.w_f32, c, n, 0.f, b);
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = fmaf(v[p][e] * rstd, w[e], b[e]);
-    ln_store<T>(y + c, n, o);
-  }
+      for (int e = 0; e < V; ++e) sum += v[p][e];
+    ln_sum2<TPR>(sum, sq, red);
+    const float mean = sum / cc;   // (a quotient: a constant row has its own value as mean)
+    sq = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const long c = (long)(p * TPR + t) * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[p][e] -= mean;
+        if (c + e < A.C) sq = fmaf(v[p][e], v[p][e], sq);
+      }
+    }
+    sum = 0.f;
+    ln_sum2<TPR>(sq, sum, red);
+    const float rstd = 1.f / sqrtf(sq / cc + A.eps);
+    if (!live) continue;
+    if (t == 0 && A.mean) {
+      A.mean[row] = mean;
+      A.rstd[row] = rstd;
+    }
+    T* y = (T*)A.y + row * A.C;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const long c = (long)(p * TPR + t) * V;
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = fmaf(v[p][e] * rstd, w[p][e], b[p][e]);
+      ln_store<T>(y + c, A.C - c, o);
+    }
   }
 }
 
-// a workgroup walks the rows blockIdx.x * RPB + slot, + gridDim.x * RPB, ...; the columns of a thread stay the same, so that
-// the weight gradients add up in its registers
+// The same walk; the weight gradients add up in a thread's registers, then over the workgroup's rows in LDS, and leave one
+// line of partial sums.
+constexpr int ln_bwd_threads(int tpr) { return tpr > 512 ? tpr : 512; }
+
 template <typename T, int TPR, int P, bool WG>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_bwd_kernel(LnArgs A) {
-  constexpr int V = LnT<T>::V, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
-  __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
+__global__ __launch_bounds__(ln_bwd_threads(TPR)) void ln_rows_bwd_kernel(LnArgs A) {
+  constexpr int V = LnT<T>::V, NT = ln_bwd_threads(TPR), RPB = NT / TPR;
+  constexpr int U = TPR >= 64 ? RPB : NT / 64, W = TPR * P * V;      // sums of the workgroup in LDS: units, columns
+  __shared__ float red[RPB][2 * (TPR > 64 ? TPR / 64 : 1)];
+  __shared__ float join[WG && U > 1 ? (U - 1) * W : 1];
+  constexpr bool kAhead = P * V <= 24;      // (with four 16-bit pieces there are no registers for the next row's)
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const long step = (long)gridDim.x * RPB;
+  long row = (long)blockIdx.x * RPB + slot;
+  u32x4 xr[P], gr[P];
+  float mean, rstd;
+  auto fetch = [&](long row) {
+    const long at = row < A.outer ? row : 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const long c = (long)(p * TPR + t) * V, n = row < A.outer ? A.C - c : 0;
+      xr[p] = ln_piece<T>((const T*)A.x + at * A.x_os + c, n);
+      gr[p] = ln_piece<T>((const T*)A.dy + at * A.dy_os + c, n);
+    }
+    mean = A.mean[at];
+    rstd = A.rstd[at];
+  };
+  if (kAhead) fetch(row);
   float w[P][V], dw[P][V], db[P][V];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -206,26 +261,18 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_bwd_kernel(LnAr
     for (int e = 0; e < V; ++e) dw[p][e] = db[p][e] = 0.f;
   }
   const float inv = 1.f / (float)A.C;
-  for (long r0 = (long)blockIdx.x * RPB; r0 < A.outer; r0 += (long)gridDim.x * RPB) {
-    const long row = r0 + slot;
-    const bool live = row < A.outer;
-    const long rr = live ? row : 0;
-    const T* x = (const T*)A.x + rr * A.x_os;
-    const T* dy = (const T*)A.dy + rr * A.dy_os;
-    const float mean = A.mean[rr], rstd = A.rstd[rr];
+  for (long r0 = (long)blockIdx.x * RPB; r0 < A.outer; r0 += step, row += step) {
+    if (!kAhead) fetch(row);
     float v[P][V], g[P][V];
     float s1 = 0.f, s2 = 0.f;
+    const float rs = rstd;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const long c = (long)(p * TPR + t) * V, n = live ? A.C - c : 0;
-      ln_load<T>(x + c, n, v[p]);
-      ln_load<T>(dy + c, n, g[p]);
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
+      ln_widen<T>(xr[p], v[p]);
+      ln_widen<T>(gr[p], g[p]);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float xh = (v[p][e] - mean) * rstd;   // (behind the row's end g = 0: no sum sees it)
+        const float xh = (v[p][e] - mean) * rs;   // (behind the row's end and in missing rows g = 0: no sum sees it)
         v[p][e] = xh;
         if (WG) {
           dw[p][e] = fmaf(g[p][e], xh, dw[p][e]);
@@ -236,10 +283,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_bwd_kernel(LnAr
         s2 = fmaf(g[p][e], xh, s2);
       }
     }
-    ln_sum2<TPR>(s1, s2, red);
+    if (kAhead && r0 + step < A.outer) fetch(row + step);
+    ln_sum2<TPR>(s1, s2, red[slot]);
     s1 *= inv;
     s2 *= inv;
-    if (!live) continue;   // (a row's threads are dead together; with a workgroup per row none is)
+    if (row >= A.outer) continue;   // (the barriers of the sums are passed by all threads of the workgroup)
     T* dx = (T*)A.y + row * A.C;
     const T* ex = A.extra ? (const T*)A.extra + row * A.ex_os : nullptr;
 #pragma unroll
@@ -248,7 +296,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_bwd_kernel(LnAr
       if (n <= 0) break;
       float o[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) o[e] = rstd * (g[p][e] - s1 - v[p][e] * s2);
+      for (int e = 0; e < V; ++e) o[e] = rs * (g[p][e] - s1 - v[p][e] * s2);
       if (ex) {
         float q[V];
         ln_load<T>(ex + c, n, q);
@@ -258,17 +306,42 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void ln_rows_bwd_kernel(LnAr
       ln_store<T>(dx + c, n, o);
     }
   }
-  if (WG) {
-    float* line = A.part + ((long)blockIdx.x * RPB + slot) * 2 * A.C;
+  if constexpr (WG) {
+    const int unit = TPR >= 64 ? slot : threadIdx.x >> 6;
+    const bool lead = TPR >= 64 || (threadIdx.x & 63) < TPR;
+    float* line = A.part + (long)blockIdx.x * 2 * A.C;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const long c = (long)(p * TPR + t) * V;
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c + e < A.C) {
-          line[c + e] = dw[p][e];
-          line[A.C + c + e] = db[p][e];
+      for (int p = 0; p < P; ++p) {
+        float a[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          a[e] = k ? db[p][e] : dw[p][e];
+#pragma unroll
+          for (int o = TPR; o < 64; o <<= 1) a[e] += __shfl_xor(a[e], o, 64);
+          if (k) db[p][e] = a[e];
+          else dw[p][e] = a[e];
         }
+        if (U > 1 && unit && lead) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) join[(unit - 1) * W + (p * V + e) * TPR + t] = a[e];
+        }
+      }
+      if (U > 1) __syncthreads();
+      if (unit == 0 && lead) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const long c = (long)(p * TPR + t) * V;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            float a = k ? db[p][e] : dw[p][e];
+            for (int u = 1; u < U; ++u) a += join[(u - 1) * W + (p * V + e) * TPR + t];
+            if (c + e < A.C) line[k * A.C + c + e] = a;
+          }
+        }
+      }
+      if (U > 1) __syncthreads();
     }
   }
 }
@@ -360,25 +433,6 @@ __global__ __launch_bounds__(256) void ln_rows_wgrad_loop_kernel(LnArgs A) {
 // ---- channel-major (inner > 1) -------------------------------------------------------------------------------------------
 // A workgroup: TN lanes along N (V values each), TC threads along C with channels tc, tc + TC, ...  The pieces stay in
 // registers as they were read (4 registers a piece whatever the type); they are widened where they are used.
-template <typename T>
-__device__ __forceinline__ u32x4 ln_piece(const T* p, long n) {
-  constexpr int V = LnT<T>::V;
-  typedef T vec __attribute__((ext_vector_type(V)));
-  if (n >= V) return *reinterpret_cast<const typename LnT<T>::piece*>(p);
-  vec t;
-#pragma unroll
-  for (int e = 0; e < V; ++e) t[e] = e < n ? p[e] : (T)0.f;
-  return __builtin_bit_cast(u32x4, t);
-}
-template <typename T>
-__device__ __forceinline__ void ln_widen(const u32x4& raw, float (&v)[LnT<T>::V]) {
-  constexpr int V = LnT<T>::V;
-  typedef T vec __attribute__((ext_vector_type(V)));
-  const vec t = __builtin_bit_cast(vec, raw);
-#pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = (float)t[e];
-}
-
 // sums over the TC threads of every column (K sums of V columns per thread), the same value in every thread
 template <int TN, int TC, int KV>
 __device__ __forceinline__ void ln_colsum(float (&a)[KV], float* red) {
@@ -695,9 +749,10 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
 }
 
 // ---- launches -------------------------------------------------------------------------------------------------------------
-// Threads per row and pieces per thread of a width: up to 64 pieces (2 KB rows of 16-bit values, 1 KB of fp32) stay inside a
-// wave, which needs no barrier; wider rows take a workgroup of 256, then 512 threads (the backward's registers: three fp32
-// arrays beside the two tensors' rows end at four pieces).
+// Threads per row and pieces per thread of a width: up to 128 pieces (2 KB rows) stay inside a wave, which needs no barrier;
+// wider rows take 256, then 512 threads (the backward's registers: three fp32 arrays beside the two tensors' rows and the next
+// ones' end at three pieces of 16-bit values; the widest rows are not read ahead.  4096 x 8192 bf16, backward: 512 threads of
+// two pieces 53 us, 256 of four 77 us).
 struct LnPlan { int tpr, p; };
 static LnPlan ln_plan(int C, int V) {
   const long pieces = ((long)C + V - 1) / V;
@@ -709,7 +764,7 @@ static LnPlan ln_plan(int C, int V) {
   if (pieces <= 256) return {256, 1};
   if (pieces <= 512) return {256, 2};
   if (pieces <= 768) return {256, 3};
-  if (pieces <= 1024) return {256, 4};
+  if (pieces <= 1024) return {512, 2};
   if (pieces <= 2048) return {512, 4};
   return {0, 0};
 }
@@ -726,15 +781,22 @@ static LnPlan ln_chan_plan(int C) {   // threads along C, pieces per thread
 constexpr long kLnGrid = 1 << 20;   // workgroups of a launch at most (a launch holds fewer than 2^32 threads): the kernels walk on
 static unsigned ln_grid(long n) { return (unsigned)(n < kLnGrid ? n : kLnGrid); }
 constexpr int kLnLoopLines = 128;
-constexpr int kLnLines = 512;    // workgroups of a backward launch: two per CU
+// Workgroups of a backward launch at most, each with a line of partial sums: two per CU, and one (of eight waves) for rows of
+// two pieces a thread and more, whose next row in flight keeps memory busy and whose lines cost (8192 x 4096 bf16: 256 lines
+// 38 + 4 us, 512 lines 45 + 4 us; one piece, 65 536 x 512 bf16: 40 us, 33 us).
+constexpr int kLnLines = 512;
+// workgroups for n units of work that walk on: at most `most`, each the same number of units
+static long ln_even(long n, long most) {
+  const long rounds = (n + most - 1) / most;
+  return rounds ? (n + rounds - 1) / rounds : 0;
+}
 
 template <typename T> static long ln_lines(int C, long outer, long inner) {
   if (inner == 1) {
     const LnPlan pl = ln_plan(C, LnT<T>::V);
     if (!pl.tpr) return outer < kLnLoopLines ? outer : kLnLoopLines;
-    const int rpb = pl.tpr >= 256 ? 1 : 256 / pl.tpr;
-    const long groups = (outer + rpb - 1) / rpb;
-    return (groups < kLnLines ? groups : kLnLines) * rpb;
+    const int rpb = ln_bwd_threads(pl.tpr) / pl.tpr;
+    return ln_even((outer + rpb - 1) / rpb, pl.p > 1 ? kLnLines / 2 : kLnLines);
   }
   const LnPlan pl = ln_chan_plan(C);
   if (!pl.tpr) {
@@ -742,18 +804,19 @@ template <typename T> static long ln_lines(int C, long outer, long inner) {
     return need < kLnLoopLines ? need : kLnLoopLines;
   }
   const int tn = pl.tpr == 128 ? 8 : 16;
-  const long tiles = outer * ((inner + tn * LnT<T>::V - 1) / (tn * LnT<T>::V));
-  return tiles < kLnLines ? tiles : kLnLines;
+  return ln_even(outer * ((inner + tn * LnT<T>::V - 1) / (tn * LnT<T>::V)), kLnLines);
 }
 
 template <typename T, int TPR, int P>
 static int ln_rows(const LnArgs& A, bool bwd, hipStream_t s) {
-  constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
-  const long groups = (A.outer + RPB - 1) / RPB;
   if (!bwd) {
-    hipLaunchKernelGGL((ln_rows_fwd_kernel<T, TPR, P>), dim3(ln_grid(groups)), dim3(NT), 0, s, A);
+    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+    // (as many as stand on the card at once: the registers of four pieces halve that)
+    const unsigned grid = (unsigned)ln_even((A.outer + RPB - 1) / RPB, 256 * (P < 4 ? 2048 : 1024) / NT);
+    hipLaunchKernelGGL((ln_rows_fwd_kernel<T, TPR, P>), dim3(grid), dim3(NT), 0, s, A);
   } else {
-    const unsigned grid = (unsigned)(groups < kLnLines ? groups : kLnLines);
+    constexpr int NT = ln_bwd_threads(TPR);
+    const unsigned grid = (unsigned)ln_lines<T>(A.C, A.outer, 1);
     if (A.part) hipLaunchKernelGGL((ln_rows_bwd_kernel<T, TPR, P, true>), dim3(grid), dim3(NT), 0, s, A);
     else hipLaunchKernelGGL((ln_rows_bwd_kernel<T, TPR, P, false>), dim3(grid), dim3(NT), 0, s, A);
   }
@@ -765,8 +828,8 @@ static int ln_chan(const LnArgs& A, bool bwd, hipStream_t s) {
   const long tiles = A.outer * ((A.inner + TN * V - 1) / (TN * V));
   if (!bwd) hipLaunchKernelGGL((ln_chan_fwd_kernel<T, TN, TC, P>), dim3(ln_grid(tiles)), dim3(TN * TC), 0, s, A);
   else
-    hipLaunchKernelGGL((ln_chan_bwd_kernel<T, TN, TC, P>), dim3((unsigned)(tiles < kLnLines ? tiles : kLnLines)), dim3(TN * TC),
-                       0, s, A);
+    hipLaunchKernelGGL((ln_chan_bwd_kernel<T, TN, TC, P>), dim3((unsigned)ln_lines<T>(A.C, A.outer, A.inner)), dim3(TN * TC), 0,
+                       s, A);
   return (int)hipGetLastError();
 }
 
@@ -783,7 +846,7 @@ static int ln_launch(const LnArgs& A, bool bwd, hipStream_t s) {
       case 256 * 8 + 1: return ln_rows<T, 256, 1>(A, bwd, s);
       case 256 * 8 + 2: return ln_rows<T, 256, 2>(A, bwd, s);
       case 256 * 8 + 3: return ln_rows<T, 256, 3>(A, bwd, s);
-      case 256 * 8 + 4: return ln_rows<T, 256, 4>(A, bwd, s);
+      case 512 * 8 + 2: return ln_rows<T, 512, 2>(A, bwd, s);
       case 512 * 8 + 4: return ln_rows<T, 512, 4>(A, bwd, s);
     }
     if (!bwd) {
