@@ -37,10 +37,10 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int wave = da_uni(tid >> 6), rw = wave % RW, mw = Cfg::MW > 1 ? wave / RW : 0;
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
-  const long units = (long)blocks * A.B * A.Hkv, unit = da_unit(units);
-  if (unit >= units) return;
-  const unsigned blk = blocks - 1 - (unsigned)da_uni((int)(unit % blocks));
-  const int pair = da_uni((int)(unit / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
+  unsigned blk, pr;
+  if (!da_unit(gridDim.x, blocks, A.B * A.Hkv, A.causal, blk, pr)) return;
+  blk = blocks - 1 - blk;      // (under a causal mask the long rows first)
+  const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int len = da_len(A, b);
   const int start = da_start(A, b);
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
@@ -252,7 +252,8 @@ struct DkvCfg {
 
 template <typename T, int DP, int KBW, int RWW>
 __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, RWW>::WPS)) void diff_dkv_kernel(DaArgs A,
-                                                                                                               unsigned main_grid) {
+                                                                                                               unsigned main_grid,
+                                                                                                               bool mirror) {
   typedef DkvCfg<T, DP, KBW, RWW> Cfg;
   typedef typename Cfg::Fd Fd;
   typedef typename Fd::Tl Tl;
@@ -284,16 +285,14 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 
   const int wave = da_uni(tid >> 6), kb = wave / RWW, rww = RWW > 1 ? wave % RWW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
-  const long units = (long)blocks * A.B * A.Hkv;
-  const long unit = (long)(blockIdx.x & 7) * (main_grid / 8) + (blockIdx.x >> 3);
-  if (unit >= units) return;
-  const int blk = da_uni((int)(unit % blocks));   // (under a causal mask the keys that most rows see first)
-  const int pair = da_uni((int)(unit / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
+  unsigned bl, pr;
+  if (!da_unit(main_grid, blocks, A.B * A.Hkv, A.causal, bl, pr)) return;
+  const int blk = bl, pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;   // (causal: the keys that most rows see first)
   const int len = da_len(A, b);
   const int start = da_start(A, b);
   // first key of the workgroup's k-th block of 32 (mirrored ones end where the blocks from the front begin: Nk, no key)
   auto block_key = [&](int k) {
-    if (RWW == 1) return blk * Cfg::KB + 32 * k;
+    if (!mirror) return blk * Cfg::KB + 32 * k;
     constexpr int HB = KBW / 2;
     if (k < HB) return 32 * (blk * HB + k);
     const int back = (A.Nk + 31) / 32 - 1 - (blk * HB + k - HB);
@@ -603,12 +602,12 @@ static int big_lds(K kernel, int bytes) {
 }
 
 template <typename T, int DP, int KBW, int RWW>
-static int dkv_go(const DaArgs& A, hipStream_t s) {
+static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
   typedef DkvCfg<T, DP, KBW, RWW> K;
   const long grid = (((long)A.Nk + K::KB - 1) / K::KB * A.B * A.Hkv + 7) / 8 * 8;
   if ((grid + A.H) * K::NT >= (1ll << 32)) return -22;
   if (const int rc = big_lds(diff_dkv_kernel<T, DP, KBW, RWW>, K::kLds)) return rc;
-  hipLaunchKernelGGL((diff_dkv_kernel<T, DP, KBW, RWW>), dim3((unsigned)(grid + A.H)), dim3(K::NT), K::kLds, s, A, (unsigned)grid);
+  hipLaunchKernelGGL((diff_dkv_kernel<T, DP, KBW, RWW>), dim3((unsigned)(grid + A.H)), dim3(K::NT), K::kLds, s, A, (unsigned)grid, mirror);
   return (int)hipGetLastError();
 }
 
@@ -624,10 +623,10 @@ static int bwd_go(const DaArgs& A, hipStream_t s) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
   if constexpr (DP == 128 || (DaT<T>::NP == 2 && DP == 64)) {
-    return dkv_go<T, DP, 4, 1>(A, s);
+    return dkv_go<T, DP, 4, 1>(A, false, s);
   } else {
     const long blocks = ((long)A.Nk + 127) / 128 * pairs;
-    return blocks < 512 ? dkv_go<T, DP, 2, 4>(A, s) : dkv_go<T, DP, 4, 1>(A, s);
+    return blocks < (A.causal ? 1024 : 512) ? dkv_go<T, DP, 2, 4>(A, A.causal && blocks < 256, s) : dkv_go<T, DP, 4, 1>(A, false, s);
   }
 }
 

@@ -17,7 +17,7 @@ template <typename T, int DP, int RW, int KW, int MW>
 struct FwdCfg {
   static constexpr int NW = RW * KW * MW, NT = 64 * NW;
   static constexpr bool AHEAD = MW > 1 || DP < 64;            // the next step's logits before this one's exponentials (registers)
-  static constexpr int SUB = KW > 1 ? 1 : 2;                  // 32-key steps of a wave per tile
+  static constexpr int SUB = KW > 1 && RW == 1 ? 1 : 2;                  // 32-key steps of a wave per tile
   static constexpr int KT = 32 * KW * SUB;
   static constexpr int DVT = 2 * DP / 32, MPW = 2 / MW;      // 32-column pieces of an output, maps of a wave
   typedef Feed<T, DP, KT, NT> Fd;
@@ -48,12 +48,11 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   const int rw = wave % RW, kw = KW > 1 ? (wave / RW) % KW : 0, mw = MW > 1 ? wave / (RW * KW) : 0;
   const unsigned rows = (unsigned)A.Nq * A.G;
   const unsigned blocks = (rows + 32 * RW - 1) / (32 * RW);
-  const long units = (long)blocks * A.splits * A.B * A.Hkv;
-  const long unit = da_unit(units);
-  if (unit >= units) return;
-  const unsigned rest = da_uni((int)(unit / A.splits)), split = (unsigned)(unit - (long)rest * A.splits);
-  const int pair = da_uni((int)(rest / blocks)), b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
-  const unsigned blk = blocks - 1 - (rest - pair * blocks);      // (under a causal mask the long rows first)
+  unsigned part, pr;
+  if (!da_unit(gridDim.x, blocks * A.splits, A.B * A.Hkv, A.causal, part, pr)) return;
+  const unsigned split = A.splits > 1 ? part % A.splits : 0;
+  const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
+  const unsigned blk = blocks - 1 - (A.splits > 1 ? part / A.splits : part);      // (under a causal mask the long rows first)
 
   const int len = da_len(A, b);
   const int start = da_start(A, b);
@@ -68,14 +67,19 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   const int kmin = first + 31 < rows ? da_limit(A, len, start, da_uni(first / (unsigned)A.G)) : 0;
 
   const int tiles = (kmax + Cfg::KT - 1) / Cfg::KT;
-  const int t0 = da_uni((int)((long)tiles * split / A.splits)), t1 = da_uni((int)((long)tiles * (split + 1) / A.splits));
+  int t0 = 0, t1 = tiles;
+  if (A.splits > 1) {
+    const int each = da_uni(tiles / A.splits), more = tiles - each * A.splits;
+    t0 = split * each + ((int)split < more ? split : more);
+    t1 = t0 + each + ((int)split < more);
+  }
 
   const Rows<T> keys = {(const T*)A.k + b * A.k_bs + hk * A.k_hs, (const T*)A.v + b * A.v_bs + hk * A.v_hs, A.k_ms, (int)A.k_rs, (int)A.v_rs,
                         len, A.d, A.key_mask ? A.key_mask + b * A.km_bs : nullptr};
   Fd feed(smem, tid);
   if (t0 < t1) feed.issue(keys, t0 * Cfg::KT);
 
-  Lane<DP> L(lane, 32 * kw);
+  Lane<DP> L(lane, 32 * kw * Cfg::SUB);
   Frag<T> qf[MPW][KS];
   float c[MPW];             // logits' base-2 exponents per unit of the products
   {
@@ -194,7 +198,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
     logits(L, 0, s[0]);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
-      const int row0 = 32 * (kw + sub), k0 = t * Cfg::KT + row0;
+      const int row0 = 32 * (kw * Cfg::SUB + sub), k0 = t * Cfg::KT + row0;
       if (sub && k0 >= kmax) break;   // (uniform; nothing of it is seen)
       const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;
       if (word != 0xffffffffu || k0 + 32 > kmin) hide(s[sub & 1], k0, word);

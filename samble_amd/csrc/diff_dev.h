@@ -446,11 +446,20 @@ __device__ __forceinline__ int da_limit(const DaArgs& A, int len, int start, int
   return n < 0 ? 0 : n > len ? len : n;
 }
 
-// workgroups of one (batch item, key head) on one XCD, so that its keys and values are read once into that XCD's L2:
-// workgroups are dealt to the XCDs in turn.  Any bijection is correct.
-__device__ __forceinline__ long da_unit(long n) {
-  const long per = (n + 7) / 8;
-  return (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+// This workgroup's block and (batch item, key head) pair, of `pairs` x `blocks` (fewer than 2^32); false: none.  Workgroups are
+// dealt to the XCDs in turn, and the blocks of a pair stand on one XCD, so that its tiles are read once into that XCD's L2.
+// Under a causal mask (`order`) blocks come longest first, over all the XCD's pairs where these are few.
+__device__ __forceinline__ bool da_unit(unsigned grid, unsigned blocks, unsigned pairs, bool order, unsigned& blk, unsigned& pair) {
+  const unsigned x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  if (order && pairs % 8 == 0 && pairs <= 64) {
+    blk = da_uni(j / (pairs / 8));
+    pair = x * (pairs / 8) + da_uni(j % (pairs / 8));
+    return blk < blocks;
+  }
+  const unsigned unit = x * (grid / 8) + j;
+  pair = da_uni(unit / blocks);
+  blk = unit - pair * blocks;
+  return pair < pairs;
 }
 
 __device__ __forceinline__ float da_xor32_sum(float x) {
