@@ -15,27 +15,27 @@
 
 namespace samble {
 
-// MW waves along the maps (each forms dA for itself): where both maps' operands and gradients would leave no registers for a
-// second wave on the SIMD
+// WPS: waves per SIMD.  Two, but where both maps' operands and gradients need more than 256 registers (8 x 2048 x 8 heads of
+// 128, bf16: one wave with 512 registers 604 us, a wave for each map, both forming dA, 1194 us).
 template <typename T, int DP>
 struct DqCfg {
-  static constexpr int MW = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 2 : 1, MPW = 2 / MW, RW = 4, NW = RW * MW, NT = 64 * NW;
-  static constexpr int SUB = DP <= 64 ? 2 : 1, KT = 32 * SUB;
+  static constexpr int RW = 4, NT = 64 * RW, WPS = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 1 : 2;
+  static constexpr int SUB = 2, KT = 32 * SUB;
   typedef Feed<T, DP, KT, NT> Fd;
   static constexpr int DT = DP < 32 ? 1 : DP / 32;     // 32-column pieces of a map's gradient (16 columns: both maps on one)
   static constexpr int kLds = Fd::kLds;
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A) {
+__global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_dq_kernel(DaArgs A) {
   typedef DqCfg<T, DP> Cfg;
   typedef typename Cfg::Fd Fd;
   typedef typename Fd::Tl Tl;
-  constexpr int KS = DP / 16, DT = Cfg::DT, RW = Cfg::RW, MPW = Cfg::MPW;
+  constexpr int KS = DP / 16, DT = Cfg::DT, RW = Cfg::RW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
-  const int wave = da_uni(tid >> 6), rw = wave % RW, mw = Cfg::MW > 1 ? wave / RW : 0;
+  const int rw = da_uni(tid >> 6);
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   unsigned blk, pr;
   if (!da_unit(gridDim.x, blocks, A.B * A.Hkv, A.causal, blk, pr)) return;
@@ -58,12 +58,12 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
   if (tiles) feed.issue(keys, 0);
 
   Lane<DP> L(lane, 0);
-  Frag<T> qf[MPW][KS], gf[2 * KS];
-  float c[MPW], gscale;
+  Frag<T> qf[2][KS], gf[2 * KS];
+  float c[2], gscale;
   {
-    const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs + mw * A.q_ms;
+    const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs;
 #pragma unroll
-    for (int m = 0; m < MPW; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
+    for (int m = 0; m < 2; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
   }
   const float lam = da_lam<T>(A, head);
   float dot[2] = {0.f, 0.f}, norm = 0.f;      // t_1, t_2, |g|^2
@@ -95,27 +95,27 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
     dot[0] = fmaf(lam, dot[1], dot[0]);
     if (DaT<T>::NP == 2) norm = da_xor32_sum(norm);
   }
-  float lse[MPW], tm[MPW], lack[MPW];
+  float lse[2], tm[2], lack[2];
 #pragma unroll
-  for (int m = 0; m < MPW; ++m) {
-    const long at = (((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi;
+  for (int m = 0; m < 2; ++m) {
+    const long at = (((long)b * A.H + head) * 2 + m) * A.Nq + qi;
     lse[m] = live ? A.lse[at] : __builtin_huge_valf();
-    tm[m] = MPW == 2 ? dot[m] : mw ? dot[1] : dot[0];
+    tm[m] = dot[m];
     lack[m] = 0.f;
   }
-  if (DaT<T>::NP == 2 && live && h == 0 && mw == 0)
+  if (DaT<T>::NP == 2 && live && h == 0)
     A.delta[2l * A.B * A.H * A.Nq + ((long)b * A.H + head) * A.Nq + qi] = sqrtf(norm);
 
-  f32x16 acc[MPW][DT];
+  f32x16 acc[2][DT];
 #pragma unroll
-  for (int m = 0; m < MPW; ++m)
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[m][t] = zero16();
   // fp32: the scale of dS (this lane's row: from the largest dA - t so far) and of the keys in the sums
   float fscale = 1.f, kscale = 1.f;
   unsigned fbits = 0;
   if (DaT<T>::NP == 2) {
-    for (int m = 0; m < MPW; ++m) fbits = da_max_bits(fbits, tm[m]);
+    for (int m = 0; m < 2; ++m) fbits = da_max_bits(fbits, tm[m]);
     fscale = 0.5f * da_scale(fbits);
   }
 
@@ -125,7 +125,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
       const float f = t == 0 ? 1.f : feed.sx / kscale;
       kscale = feed.sx;
 #pragma unroll
-      for (int m = 0; m < MPW; ++m)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -153,7 +153,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
           const float n = 0.5f * da_scale(fbits), f = n / fscale;
           fscale = n;
 #pragma unroll
-          for (int m = 0; m < MPW; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -161,12 +161,12 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
         }
         a1 *= fscale;
       }
-      Frag<T> ds[MPW][2];
+      Frag<T> ds[2][2];
 #pragma unroll
-      for (int m = 0; m < MPW; ++m) {
+      for (int m = 0; m < 2; ++m) {
         f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::map_rows(L, m, mw, row0, ks), qf[m][ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::map_rows(L, m, 0, row0, ks), qf[m][ks], s);
         const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cm, -lse[m]));
@@ -196,23 +196,23 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), 2) void diff_dq_kernel(DaArgs A
         for (int dt = 0; dt < DT; ++dt) {
           Frag<T> kf;
 #pragma unroll
-          for (int m = 0; m < MPW; ++m) {
-            if (DP >= 32 || m == 0) kf = DP < 32 ? Tl::cols(L, 0, row0, u, 0) : Tl::map_cols(L, m, mw, row0, u, 32 * dt);
+          for (int m = 0; m < 2; ++m) {
+            if (DP >= 32 || m == 0) kf = DP < 32 ? Tl::cols(L, 0, row0, u, 0) : Tl::map_cols(L, m, 0, row0, u, 32 * dt);
             acc[m][dt] = da_mma<T>(kf, ds[m][u], acc[m][dt]);
           }
         }
     }
   }
 #pragma unroll
-  for (int m = 0; m < MPW; ++m) {
+  for (int m = 0; m < 2; ++m) {
     if (DaT<T>::NP == 1) tm[m] += da_xor32_sum(lack[m]);
-    if (live && h == 0) A.delta[(((long)b * A.H + head) * 2 + m + mw) * A.Nq + qi] = tm[m];
+    if (live && h == 0) A.delta[(((long)b * A.H + head) * 2 + m) * A.Nq + qi] = tm[m];
   }
   if (!live) return;
-  T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d + mw * A.d;
+  T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
 #pragma unroll
-  for (int m = 0; m < MPW; ++m) {
-    const float f = A.scale * (m + mw ? -lam : 1.f) / fscale / kscale;      // dS_2 = -lam P_2 (dA - t_2)
+  for (int m = 0; m < 2; ++m) {
+    const float f = A.scale * (m ? -lam : 1.f) / fscale / kscale;      // dS_2 = -lam P_2 (dA - t_2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
