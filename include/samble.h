@@ -14,7 +14,8 @@
  *     failure on the calling thread is available from samble_last_error();
  *   - re-entrant and thread-safe; the current HIP device is the caller's business;
  *   - strides are in ELEMENTS; "bs" = batch stride, "rs" = row stride;
- *   - fp32 everywhere, indices int32 (neighbour lists) or int64 (sampled indices, as the
+ *   - fp32 everywhere (layer normalisation and differential attention, which name their type, also fp16 and
+ *     bf16), indices int32 (neighbour lists) or int64 (sampled indices, as the
  *     reference's (B,1,M) int64 tensor).  Attention kernels require D == 128 in this round.
  */
 #ifndef SAMBLE_H
@@ -730,7 +731,8 @@ int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const
                     backward dout: batch, row, head.  The last axes are contiguous; every row starts on 16 bytes; rows at
                     most 2^23, maps at most 2^28 elements apart
      lengths (B) or null: item b has that many keys (taken into 0 .. Nk); key_mask (B, Nk) or null: 0 = the key does not exist
-     causal          query i sees the keys up to position q_start[b] + i; q_start null: Nk - Nq
+     causal          query i sees the keys up to position q_start[b] + i (q_start null: Nk - Nq); keys behind the last
+                     query's position do not exist
    A row that sees no key gives zeros and takes no part in the gradients.  Values of keys that do not exist are never used.
      samble_diff_attn_fwd   out (B, Nq, H, 2 d) contiguous; out2 (sum_j P_1 v, same shape) and lse (B, H, 2, Nq) for the
                             backward, both or neither null; workspace: samble_diff_attn_fwd_workspace_bytes (may be 0)

@@ -572,7 +572,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     lengths (B,): item b has that many keys (out of 0 .. Nk: the nearest); key_mask (B, Nk) bool: False = the key does not
     exist.  Whatever stands at keys that do not exist, NaN included, is not used and gets gradient 0.
     causal: query i sees the keys up to position q_start[b] + i; q_start (B,) is Nk - Nq unless given (the queries are the
-    last ones).  Keys that only the causal order hides must be finite.
+    last ones).  Keys behind the last query's position do not exist either (the unwritten end of a cache); those that some
+    queries see and the causal order hides from others must be finite.
     A row that sees no key gives zeros and gets no gradient.  The calls Nq = 1 over a long cache split the keys over the GPU."""
     for name, t, n in (("q", q, 5), ("k", k, 5), ("v", v, 4)):
         if not isinstance(t, torch.Tensor) or t.dim() != n:

@@ -41,8 +41,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   if (!da_unit(gridDim.x, blocks, A.B * A.Hkv, A.causal, blk, pr)) return;
   blk = blocks - 1 - blk;      // (under a causal mask the long rows first)
   const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
-  const int len = da_len(A, b);
-  const int start = da_start(A, b);
+  const int start = da_start(A, b), len = da_len(A, b, start);
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
   const bool live = r < rows;
   const int qi = live ? (int)(r / (unsigned)A.G) : 0, head = hk * A.G + (live ? (int)(r % (unsigned)A.G) : 0);
@@ -288,8 +287,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   unsigned bl, pr;
   if (!da_unit(main_grid, blocks, A.B * A.Hkv, A.causal, bl, pr)) return;
   const int blk = bl, pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;   // (causal: the keys that most rows see first)
-  const int len = da_len(A, b);
-  const int start = da_start(A, b);
+  const int start = da_start(A, b), len = da_len(A, b, start);
   // first key of the workgroup's k-th block of 32 (mirrored ones end where the blocks from the front begin: Nk, no key)
   auto block_key = [&](int k) {
     if (!mirror) return blk * Cfg::KB + 32 * k;

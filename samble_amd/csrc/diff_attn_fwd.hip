@@ -54,8 +54,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const unsigned blk = blocks - 1 - (A.splits > 1 ? part / A.splits : part);      // (under a causal mask the long rows first)
 
-  const int len = da_len(A, b);
-  const int start = da_start(A, b);
+  const int start = da_start(A, b), len = da_len(A, b, start);
   // this lane's row
   const unsigned first = blk * 32 * RW + 32 * rw, r = first + (lane & 31);
   const bool live = r < rows;

@@ -429,15 +429,16 @@ template <typename T>
 __device__ __forceinline__ float da_lam(const DaArgs& A, int head) {
   return A.lam_f32 ? ((const float*)A.lam)[head] : (float)((const T*)A.lam)[head];
 }
-// keys of batch item b, and the position of its first query (keys <= position are seen); both are taken into range here, so
-// that no value of theirs reaches behind the tensors
-__device__ __forceinline__ int da_len(const DaArgs& A, int b) {
-  const int n = da_uni(A.lengths ? A.lengths[b] : A.Nk);
-  return n < 0 ? 0 : n > A.Nk ? A.Nk : n;
+// the position of batch item b's first query (keys <= position are seen), and its keys: under a causal mask those behind the
+// last query's position do not exist either.  Both are taken into range here, so that no value of theirs reaches behind the
+// tensors (sizes end at 2^30: beyond that, all or none)
+__device__ __forceinline__ int da_start(const DaArgs& A, int b) {
+  const int s = da_uni(A.q_start ? A.q_start[b] : A.Nk - A.Nq), far = (1 << 30) - 1;
+  return s < -far - 2 ? -far - 2 : s > far ? far : s;
 }
-__device__ __forceinline__ int da_start(const DaArgs& A, int b) {      // (sizes end at 2^30: beyond that, all or none)
-  const int s = da_uni(A.q_start ? A.q_start[b] : A.Nk - A.Nq);
-  return s < -(1 << 30) - 1 ? -(1 << 30) - 1 : s > 1 << 30 ? 1 << 30 : s;
+__device__ __forceinline__ int da_len(const DaArgs& A, int b, int start) {
+  const int n = da_uni(A.lengths ? A.lengths[b] : A.Nk), end = A.causal && start + A.Nq < A.Nk ? start + A.Nq : A.Nk;
+  return n < 0 || end < 0 ? 0 : n > end ? end : n;
 }
 // keys that query i sees
 __device__ __forceinline__ int da_limit(const DaArgs& A, int len, int start, int i) {

@@ -243,6 +243,30 @@ def test_nothing_of_missing_keys_is_used(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Nq,starts", [(1, [40, 5, -3]), (33, [0, 57, -40]), (200, [10, -150, 60])])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_keys_behind_the_last_query_are_not_used(dtype, Nq, starts):
+    """A cache with room to grow: what stands behind the positions of the queries has not been written yet."""
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, gen = _inputs(3, Nq, 300, 4, 2, 32, TYPES[dtype], 33)
+    start = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    gone = torch.arange(300, device=DEV) >= (start + Nq)[:, None]
+    res = []
+    for filler in (0.0, float("nan"), float("inf")):
+        kk, vv = k.clone(), v.clone()
+        kk[gone], vv[gone] = filler, filler
+        leaves = [t.detach().requires_grad_(True) for t in (q, kk, vv, lam)]
+        out = differential_attention(*leaves, causal=True, q_start=start)
+        assert torch.equal(differential_attention(q, kk, vv, lam, causal=True, q_start=start), out)
+        res.append((out.detach(),) + torch.autograd.grad(out, leaves, g))
+    for other in res[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(res[0], other))
+    assert not res[0][2][gone].any() and not res[0][3][gone].any()
+    kk, vv = torch.where(gone[:, :, None, None, None], 0, k), torch.where(gone[:, :, None, None], 0, v)
+    _check(q, kk, vv, lam, g, res[0], 32 ** -0.5, True, None, start, None)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [16, 64, 128])
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_dlam_is_not_that_of_rounded_outputs(dtype, d):
