@@ -241,11 +241,6 @@ struct Tile {
   static __device__ __forceinline__ Frag<T> cols(const Lane<DP>& L, int which, int row0, int t, int col0) {
     return cols_at(L.c[(col0 >> 5) & (Lane<DP>::NC - 1)], which, row0, t, col0);
   }
-  static __device__ __forceinline__ Frag<T> map_cols(const Lane<DP>& L, int m, int second, int row0, int t, int col0) {
-    constexpr int N = Lane<DP>::NC - 1;
-    const int a = m * DP + col0, b = a + DP;
-    return cols_at(second ? L.c[(b >> 5) & N] : L.c[(a >> 5) & N], 0, row0, t, second ? b : a);
-  }
   static __device__ __forceinline__ Frag<T> cols_at(unsigned at, int which, int row0, int t, int col0) {
     Frag<T> f;
     const int o = (row0 + 16 * t) * (4 * DP) + col0 / 32 / Lane<DP>::NC * 256;
@@ -274,19 +269,19 @@ struct Rows {
 };
 
 // Tiles on their way from memory to LDS, NT threads together, at LDS address 0.
-//   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), NB tiles: while one is computed on, the next
+//   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), two tiles: while one is computed on, the next
 //   lands.  The 64 pieces of a wave's copy stand one behind the other in LDS, so the lane picks the piece that belongs there.
 //   fp32: through registers, where the values are scaled and split into planes; one tile.
 // use:  feed.issue(first, row0);  for each tile: { feed.next(L);  [feed.issue(following, row0)];  compute }
 // next() is a barrier of the workgroup.
-template <typename T, int DP, int KT, int NT, int NB = 2>
+template <typename T, int DP, int KT, int NT>
 struct Feed {
   typedef Tile<T, DP, KT> Tl;
   static constexpr bool DMA = Tl::NP == 1;
   static constexpr int kPieces = KT * DP / 4;                    // of X, and of Y
   static constexpr int kPer = (kPieces + NT - 1) / NT, NW = NT / 64;
-  static constexpr int kBufs = Tl::kBytes * (DMA ? NB : 1);
-  static constexpr int kLds = kBufs + 16 * NB + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
+  static constexpr int kBufs = Tl::kBytes * (DMA ? 2 : 1);
+  static constexpr int kLds = kBufs + 32 + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
   static_assert(!DMA || kPieces % 64 == 0, "whole waves copy");
   static_assert(!DMA || NT % 256 == 0, "a thread's pieces stand at one place of their rows");
   static_assert(KT <= 128, "room for the visible rows");
@@ -301,7 +296,7 @@ struct Feed {
   __device__ __forceinline__ Feed(char* l, int t)
       : lds(l), tid(t), wave(da_uni(t >> 6)), cur(0), bit(false), ux(0), uy(0), uz(0), sx(1.f), sy(1.f) {}
 
-  __device__ __forceinline__ int after() const { return cur + 1 == NB ? 0 : cur + 1; }      // the buffer that issue() fills
+  __device__ __forceinline__ int after() const { return cur ^ 1; }      // the buffer that issue() fills
   __device__ __forceinline__ unsigned* words(int buf) const { return reinterpret_cast<unsigned*>(lds + kBufs) + 4 * buf; }
   __device__ __forceinline__ void write_words(int buf) {
     if (tid < KT) {
@@ -383,7 +378,7 @@ struct Feed {
       mx = da_wave_max(mx);
       my = da_wave_max(my);
       third = da_wave_max(third);
-      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 16 * NB);
+      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 32);
       if ((tid & 63) == 0) {
         const u32x4 m = {mx, my, third, 0u};
         red[wave] = m;

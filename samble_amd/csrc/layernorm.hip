@@ -8,13 +8,15 @@
 //
 // Every byte is touched once (forward: x [residual] in, y [s] out; backward: s, dy in, ds out): the kernels are bound by HBM.
 //   inner == 1  rows of C contiguous values.  TPR threads own a row and keep it in registers, in P pieces of 16 bytes each:
-//               TPR = 8 .. 64 inside a wave for narrow rows, a workgroup above.
+//               TPR = 8 .. 64 inside a wave for narrow rows, 256 and 512 above.  Workgroups walk the rows and read the next
+//               one ahead.  8192 x 4096 bf16: forward 24 us (5.6 TB/s, part of it from the caches), backward 38 + 4 us.
 //   inner > 1   channel-major (B, C, N) tensors: 16 lanes stand along N (16 bytes each), the other threads along C.
-// Pieces are loaded at the alignment of one element: a row of an odd width costs the same loads as an even one, with one
-// short piece at its end.  Rows beyond what registers hold (16 384 16-bit or 8 192 fp32 values) take the *_loop kernels that
-// read them again from the caches.
-// Weight gradients: each workgroup adds its rows in registers and leaves one line of partial sums; ln_reduce_kernel adds the
-// lines in a fixed order (no atomics: run to run identical).
+//               32 x 128 x 2048 fp32 with residual: forward 27 us (5.0 TB/s), backward 24.5 + 4 us (4.1 TB/s).
+// Pieces are loaded at the alignment of one element, with one short piece at the end of an odd row (4099 x 5001 fp16 with
+// residual: forward 36 us, 4.6 TB/s, backward 39 + 5 us; rows of 5000 take 3 % less).  Rows beyond what registers hold (16 384
+// 16-bit or 8 192 fp32 values) take the *_loop kernels that read them again from the caches.
+// Weight gradients: each workgroup adds its rows in registers and LDS and leaves one line of partial sums; ln_reduce_kernel
+// adds the lines in a fixed order (no atomics: run to run identical).
 #include "samble_dev.h"
 
 namespace samble {

@@ -6,6 +6,9 @@ Tolerances are sums of the roundings that the kernels are allowed, per element:
     over a row's logits, a probability is off by the factor 2 * ((d + 32) U L + 16 U); sums over n keys or rows by n U.
   * h = eps / 2 of the tensors' type: P, P_1 - lam P_2 and dS enter the second products rounded once (fp16 / bf16 only; fp32
     enters whole), saved outputs and results are rounded once.  fp16 adds half a subnormal step, 2^-25, where values are small.
+  * fp32 operands are two fp16 planes of scaled values, whose smallest step leaves 2^-25 of the scaled value.  Forward: P
+    (sum at least 1) is held times 2^6, 2^-31 of 1.  dv: the maps times 2^12, 2^-37 of 1 and of lam.  dS: times 2^12 and a
+    factor that takes |g| |v| to at least 2^-2: 2^-35 |g| |v|.
 """
 import math
 
