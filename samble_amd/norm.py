@@ -64,10 +64,10 @@ def stage_layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, dim: int, re
     _need_gpu(x, weight, bias, residual)
     outer, C, inner = _extent(x, dim)
     with _on(x.device) as stream:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         s = torch.empty_like(y) if residual is not None else x
         n = outer * inner
-        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device) if stats else (None, None)
+        mean, rstd = torch.empty((2, n), dtype=torch.float32, device=x.device).unbind(0) if stats else (None, None)
         if n:
             xv, x_os, x_cs = _slices(x, dim)
             rv, r_os, r_cs = _slices(residual, dim) if residual is not None else (None, 0, 0)
@@ -84,11 +84,11 @@ def stage_layer_norm_bwd(s: torch.Tensor, dy: torch.Tensor, weight, mean: torch.
     outer, C, inner = _extent(s, dim)
     w_dtype = weight.dtype if weight is not None else (w_dtype or s.dtype)
     with _on(s.device) as stream:
-        ds = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+        ds = torch.empty_like(s, memory_format=torch.contiguous_format)
         if outer * inner == 0:
             zero = lambda: torch.zeros(C, dtype=w_dtype, device=s.device) if want_weight_grads else None  # noqa: E731
             return ds, zero(), zero()
-        dw, db = torch.empty((2, C), dtype=w_dtype, device=s.device) if want_weight_grads else (None, None)
+        dw, db = torch.empty((2, C), dtype=w_dtype, device=s.device).unbind(0) if want_weight_grads else (None, None)
         sv, s_os, s_cs = _slices(s, dim)
         gv, g_os, g_cs = _slices(dy, dim)
         ev, e_os, e_cs = _slices(extra, dim) if extra is not None else (None, 0, 0)
