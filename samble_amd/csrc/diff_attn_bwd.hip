@@ -44,7 +44,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   const int rw = da_uni(tid >> 6);
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   unsigned blk, pr;
-  if (!da_unit(gridDim.x, blocks, A.B * A.Hkv, A.causal, blk, pr)) return;
+  if (!da_unit(A, gridDim.x, blocks, A.lengths != nullptr, blk, pr)) return;
   blk = blocks - 1 - blk;      // (under a causal mask the long rows first)
   const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int start = da_start(A, b), len = da_len(A, b, start);
@@ -291,7 +291,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const int wave = da_uni(tid >> 6), kb = wave / RWW, rww = RWW > 1 ? wave % RWW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
   unsigned bl, pr;
-  if (!da_unit(main_grid, blocks, A.B * A.Hkv, A.causal, bl, pr)) return;
+  if (!da_unit(A, main_grid, blocks, false, bl, pr)) return;
   const int blk = bl, pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;   // (causal: the keys that most rows see first)
   const int start = da_start(A, b), len = da_len(A, b, start);
   // first key of the workgroup's k-th block of 32 (mirrored ones end where the blocks from the front begin: Nk, no key)

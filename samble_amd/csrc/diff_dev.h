@@ -442,17 +442,21 @@ __device__ __forceinline__ int da_limit(const DaArgs& A, int len, int start, int
   return n < 0 ? 0 : n > len ? len : n;
 }
 
-// This workgroup's block and (batch item, key head) pair, of `pairs` x `blocks` (fewer than 2^32); false: none.  Workgroups are
-// dealt to the XCDs in turn, and the blocks of a pair stand on one XCD, so that its tiles are read once into that XCD's L2.
-// Under a causal mask (`order`) blocks come longest first, over all the XCD's pairs where these are few.
-__device__ __forceinline__ bool da_unit(unsigned grid, unsigned blocks, unsigned pairs, bool order, unsigned& blk, unsigned& pair) {
+// This workgroup's block and (batch item, key head) pair, of B Hkv x `blocks` (fewer than 2^32); false: none.  Workgroups are
+// dealt to the XCDs in turn.
+//   spread     (the sweep over the keys is as long as the item) the blocks of a pair go to all XCDs, so that none is left with
+//              the short items alone: 32 items of 256 .. 2048 keys, 8 heads of 64, bf16, forward 808 -> 692 us
+//   otherwise  the blocks of a pair stand on one XCD, so that its tiles are read once into that XCD's L2
+// Under a causal mask blocks come longest first, over all the XCD's pairs where these are few.
+__device__ __forceinline__ bool da_unit(const DaArgs& A, unsigned grid, unsigned blocks, bool spread, unsigned& blk, unsigned& pair) {
+  const unsigned pairs = A.B * A.Hkv;
   const unsigned x = blockIdx.x & 7, j = blockIdx.x >> 3;
-  if (order && pairs % 8 == 0 && pairs <= 64) {
+  if (A.causal && pairs % 8 == 0 && pairs <= 64) {
     blk = da_uni(j / (pairs / 8));
     pair = x * (pairs / 8) + da_uni(j % (pairs / 8));
     return blk < blocks;
   }
-  const unsigned unit = x * (grid / 8) + j;
+  const unsigned unit = spread ? blockIdx.x : x * (grid / 8) + j;
   pair = da_uni(unit / blocks);
   blk = unit - pair * blocks;
   return pair < pairs;
