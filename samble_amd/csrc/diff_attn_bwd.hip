@@ -268,12 +268,19 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   float* stats = reinterpret_cast<float*>(smem + Fd::kLds);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
 
-  if (blockIdx.x >= main_grid) {      // dlam of one head: - sum of t_2 over batch and queries
+  if (blockIdx.x >= main_grid) {      // dlam of one head: - sum of t_2 over batch and queries (fewer than 2^31), eight loads in flight
     const int head = blockIdx.x - main_grid;
+    const unsigned nq = A.Nq, all = (unsigned)A.B * nq;
     float sum = 0.f;
-    for (int bb = 0; bb < A.B; ++bb) {
-      const float* t2 = A.delta + (((long)bb * A.H + head) * 2 + 1) * A.Nq;
-      for (int i = tid; i < A.Nq; i += NT) sum += t2[i];
+    for (unsigned first = tid; first < all; first += 8 * NT) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const unsigned e = first + k * NT, bb = e / nq;
+        v[k] = e < all ? A.delta[(((long)bb * A.H + head) * 2 + 1) * nq + (e - bb * nq)] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += v[k];
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
