@@ -44,7 +44,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   const int rw = da_uni(tid >> 6);
   const unsigned rows = (unsigned)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   unsigned blk, pr;
-  if (!da_unit(A, gridDim.x, blocks, A.lengths != nullptr, blk, pr)) return;
+  if (!da_unit(A, gridDim.x, blocks, A.lengths && !A.causal && A.Hkv % 8, blk, pr)) return;
   blk = blocks - 1 - blk;      // (under a causal mask the long rows first)
   const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const int start = da_start(A, b), len = da_len(A, b, start);

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   const unsigned rows = (unsigned)A.Nq * A.G;
   const unsigned blocks = (rows + 32 * RW - 1) / (32 * RW);
   unsigned part, pr;
-  if (!da_unit(A, gridDim.x, blocks * A.splits, A.lengths != nullptr, part, pr)) return;
+  if (!da_unit(A, gridDim.x, blocks * A.splits, A.lengths && !A.causal && A.Hkv % 8, part, pr)) return;
   const unsigned split = A.splits > 1 ? part % A.splits : 0;
   const int pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;
   const unsigned blk = blocks - 1 - (A.splits > 1 ? part / A.splits : part);      // (under a causal mask the long rows first)

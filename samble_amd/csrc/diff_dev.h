@@ -443,18 +443,20 @@ __device__ __forceinline__ int da_limit(const DaArgs& A, int len, int start, int
 }
 
 // This workgroup's block and (batch item, key head) pair, of B Hkv x `blocks` (fewer than 2^32); false: none.  Workgroups are
-// dealt to the XCDs in turn.
-//   spread     (the sweep over the keys is as long as the item) the blocks of a pair go to all XCDs, so that none is left with
-//              the short items alone: 32 items of 256 .. 2048 keys, 8 heads of 64, bf16, forward 808 -> 692 us
-//   otherwise  the blocks of a pair stand on one XCD, so that its tiles are read once into that XCD's L2
-// Under a causal mask blocks come longest first, over all the XCD's pairs where these are few.
+// dealt to the XCDs in turn; the blocks of a pair stand on one XCD, so that its tiles are read once into that XCD's L2.
+//   pairs a multiple of 8   every eighth pair on an XCD: items of different lengths are dealt out evenly (32 items of 256 .. 2048
+//                           keys, 8 heads of 64, bf16: dk and dv 1100 us, with neighbouring pairs on an XCD 1390 us); under a
+//                           causal mask the longest blocks first, over all the XCD's pairs where these are few
+//   spread                  the blocks of a pair on all XCDs: where the sweep is as long as the item and an XCD would have
+//                           few items (8 items of one head, fp32: 93 us, 99 us)
 __device__ __forceinline__ bool da_unit(const DaArgs& A, unsigned grid, unsigned blocks, bool spread, unsigned& blk, unsigned& pair) {
-  const unsigned pairs = A.B * A.Hkv;
-  const unsigned x = blockIdx.x & 7, j = blockIdx.x >> 3;
-  if (A.causal && pairs % 8 == 0 && pairs <= 64) {
-    blk = da_uni(j / (pairs / 8));
-    pair = x * (pairs / 8) + da_uni(j % (pairs / 8));
-    return blk < blocks;
+  const unsigned pairs = A.B * A.Hkv, x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  if (pairs % 8 == 0 && !spread) {
+    const bool order = A.causal && pairs <= 64;
+    const unsigned n = order ? pairs / 8 : blocks, q = da_uni(j / n), r = j - q * n;
+    blk = order ? q : r;
+    pair = 8 * (order ? r : q) + x;
+    return blk < blocks && pair < pairs;
   }
   const unsigned unit = spread ? blockIdx.x : x * (grid / 8) + j;
   pair = da_uni(unit / blocks);
