@@ -11,8 +11,9 @@
 //                    behind the last one sum dlam
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
 // are operands of the sums over rows as they stand.
-// P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, as operands of the second products: dq and dk
-// carry that rounding beside their own (relative to float64 2.4e-3 in bf16, where their own alone is 1.7e-3); sums are fp32.
+// P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, the type of the matrix instructions' operands (two
+// planes would double their number): against float64 dq is off by 2.8e-3 and dk by 2.4e-3 of its norm in bf16, where rounding
+// the results alone is 1.7e-3; sums are fp32.
 //
 // Bound: as the forward's, matrix instructions (24 and 32 to a 32 x 32 block of d = 64) and vector ones of a wave in turn.
 // 8 x 2048 x 16 heads of 64, bf16, no mask: dq 510 us (810 TFLOP/s), dk and dv 660 us (835); causal on 4 key heads 281 and
