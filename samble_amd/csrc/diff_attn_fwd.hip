@@ -336,7 +336,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
   const long all = (long)rows * A.B * A.Hkv;
   const int lane = threadIdx.x & 63, wave = da_uni(threadIdx.x >> 6), cols = 2 * A.d;
   const long pf = da_part_floats(A.d), step = all * pf;
-  constexpr int RPB = NW == 1 ? 4 : 1;
+  constexpr int RPB = NW == 1 ? 4 : 1, kAtOnce = NW == 1 ? 4 : 2;
   for (long u = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); u < all; u += (long)gridDim.x * RPB) {
     const unsigned pair = (unsigned)(u / rows), r = (unsigned)(u % rows);
     const int b = pair / A.Hkv, hk = pair % A.Hkv, qi = (int)(r / (unsigned)A.G), head = hk * A.G + (int)(r % (unsigned)A.G);
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
     f32x4 acc[2] = {none, none};
     float l[2] = {0.f, 0.f};
     const int c4 = 4 * lane < cols ? 4 * lane : 0;      // (lanes behind the last column: the first ones again, not used)
-#pragma unroll(NW == 1 ? 4 : 2)
+#pragma unroll kAtOnce
     for (int s = NW == 1 ? 0 : wave; s < A.splits; s += NW) {
       const float* p = w + s * step;
       const f32x4 t = *reinterpret_cast<const f32x4*>(p), x = *reinterpret_cast<const f32x4*>(p + 4 + c4);

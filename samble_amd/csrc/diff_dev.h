@@ -233,7 +233,7 @@ struct Tile {
     Frag<T> f;
     const int o = row0 * (4 * DP) + (ks & 1) * 32 + (ks >> 1) / Lane<DP>::NR * 256;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) f.p[p] = *(lds_vec8*)(at + (unsigned)((plane + p) * kPlane + o));
+    for (int p = 0; p < NP; ++p) f.p[p] = *(lds_vec8*)(unsigned long)(at + (unsigned)((plane + p) * kPlane + o));
     return f;
   }
   // A operand of the transposed tile: 32 columns col0 .. (a multiple of 32), reduced rows row0 + 16 t + {4 h + 0..3,
@@ -247,8 +247,8 @@ struct Tile {
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const unsigned b = at + (unsigned)((which * NP + p) * kPlane + o);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)b);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(b + 8 * 4 * DP));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(unsigned long)b);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(unsigned long)(b + 8 * 4 * DP));
       const vec4<E> x = __builtin_bit_cast(vec4<E>, lo), z = __builtin_bit_cast(vec4<E>, hi);
       f.p[p] = __builtin_shufflevector(x, z, 0, 1, 2, 3, 4, 5, 6, 7);
     }
