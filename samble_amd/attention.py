@@ -604,7 +604,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
         raise ValueError("differential_attention: q_start goes with causal=True")
     q_start = _per_item("q_start", q_start, B, q.device)
     if key_mask is not None:
-        if key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool or key_mask.device != q.device:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.shape != (B, Nk) or key_mask.dtype != torch.bool or key_mask.device != q.device:
             raise ValueError(f"differential_attention: key_mask must be a ({B}, {Nk}) bool tensor on {q.device}")
         if Nk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()

@@ -86,6 +86,34 @@ def test_rows_forward_and_backward(shape, dtype):
     assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db))), "not the same run to run"
 
 
+LONG = [(70001, 24), (40003, 100), (9001, 300), (5003, 1500), (4099, 5001), (2501, 7777), (2101, 16000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: f"{s[0]}x{s[1]}")
+def test_more_rows_than_the_workgroups_of_a_launch(shape, dtype):
+    """Every workgroup walks several rows, the last ones not all of them; residual, and gradients that reach the sum too."""
+    from samble_amd.norm import layer_norm
+    R, C = shape
+    gen = torch.Generator(device=DEV).manual_seed(R + C)
+    rnd = lambda *s: torch.randn(s, generator=gen, device=DEV)  # noqa: E731
+    x, res = (rnd(R, C) + 0.4).to(dtype).requires_grad_(True), rnd(R, C).to(dtype).requires_grad_(True)
+    w, b = (1 + 0.3 * rnd(C)).requires_grad_(True), (0.3 * rnd(C)).requires_grad_(True)
+    dy, ds = rnd(R, C).to(dtype), rnd(R, C).to(dtype)
+    y, s = layer_norm(x, w, b, residual=res)
+    assert torch.equal(s, (x.detach().float() + res.detach().float()).to(dtype))
+    dx, dres, dw, db = torch.autograd.grad((y, s), (x, res, w, b), (dy, ds))
+    ry, my, rdx, mdx, rdw, mdw, rdb, mdb = _ref(s.detach(), w.detach(), b.detach(), 1e-5, 1, dy, ds)
+    n = _n_add(C, True)
+    _close(y.detach(), ry, my, n, "y")
+    _close(dx, rdx, mdx, 2 * n, "dx")
+    assert torch.equal(dx, dres)
+    lines = n + R // 128 + 32 + 32
+    _close(dw, rdw, mdw, lines, "dweight")
+    _close(db, rdb, mdb, lines, "dbias")
+
+
 CHANNELS = [(1, 1, 2), (2, 8, 5), (3, 16, 64), (2, 17, 65), (2, 33, 127), (3, 64, 200), (2, 128, 2048), (2, 129, 130), (1, 256, 63),
             (2, 257, 66), (2, 512, 40), (1, 513, 33), (2, 1000, 31), (1, 1024, 129), (1, 1025, 50), (700, 20, 3), (3, 128, 1001)]
 
