@@ -184,6 +184,20 @@ def test_forward_and_gradients(case, dtype):
     assert all(torch.equal(a, b) for a, b in zip(again, grads)), "not the same run to run"
 
 
+# many pairs of an item and a key head, in the orders that workgroups take them: longest blocks first, keys from both ends, pairs
+# dealt to the XCDs one by one or (pairs no multiple of eight; lengths) block by block
+MANY = [(32, 130, 520, 8, 8, 16, "causal lengths"), (8, 520, 520, 4, 4, 32, "causal"), (16, 300, 1030, 8, 4, 16, "causal lengths keys"),
+        (16, 200, 600, 6, 3, 24, "lengths"), (5, 200, 600, 3, 3, 64, "lengths"), (7, 150, 400, 1, 1, 40, "causal lengths"),
+        (8, 1, 700, 8, 1, 64, "lengths"), (4, 3, 2600, 4, 2, 32, "causal lengths")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(str(x).replace(" ", "+") or "full" for x in c))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_many_pairs(case, dtype):
+    test_forward_and_gradients(case, dtype)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_long_cache_single_token(dtype):
