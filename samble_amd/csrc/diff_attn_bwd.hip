@@ -143,7 +143,6 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
       const int row0 = 32 * sub, k0 = t * Cfg::KT + row0;
       if (k0 >= kmax) continue;
       const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;      // (rows end at their limits, at most len)
-      const bool masked = word != 0xffffffffu || k0 + 32 > kmin;
       f32x16 da = zero16();
 #pragma unroll
       for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(L, 1, row0, ks), gf[ks], da);
@@ -176,15 +175,15 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
         const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cm, -lse[m]));
-        if (masked) {
-          unsigned w = word >> (4 * h);
-          int left = limit - k0 - 4 * h;
-          asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every tile, in front of the branch)
+        if (word != 0xffffffffu) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = crow(e, 0);
-            s[e] = ((w >> j) & 1) && j < left ? s[e] : 0.f;
-          }
+          for (int e = 0; e < 16; ++e) s[e] = da_bit(word, crow(e, 0)) ? s[e] : 0.f;
+        }
+        if (k0 + 32 > kmin) {
+          int left = limit - k0 - 4 * h;
+          asm volatile("" : "+v"(left));   // (else the comparisons are made for every tile, in front of the branch)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[e] = crow(e, 0) < left ? s[e] : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -313,7 +312,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const int key0 = block_key(0), kw0 = block_key(kb), key = kw0 + (lane & 31);
   const unsigned char* km = A.key_mask ? A.key_mask + b * A.km_bs : nullptr;
   const bool valid = key < len && (!km || km[key]);
-  const bool all_valid = __all(valid), any_valid = __any(valid);
+  const bool any_valid = __any(valid);
 
   // rows that see any key of the workgroup: all behind the first such query
   const long i0 = A.causal && key0 > start ? (long)key0 - start : 0;
@@ -486,9 +485,10 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
             da = da_mma<T>(Tl::rows(L, 1, 32 * sub, ks), vf[ks], da);
           }
         }
-        // row i sees the key if i is at least `from`; rows behind the last see nothing
+        // row i sees the key if i is at least `from`; rows behind the last see nothing.  (A key that does not exist is a column
+        // of its own: zeros were read for it, and zeros are written, whatever its sums hold.)
         const int from = key - start;
-        const bool masked = !all_valid || (A.causal && kw0 + 31 - start > i0) || i0 + 32 > A.Nq;
+        const bool masked = (A.causal && kw0 + 31 - start > i0) || i0 + 32 > A.Nq;
         f32x16 s[2];
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -497,7 +497,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
           for (int ks = 0; ks < KS; ++ks) s[m] = da_mma<T>(Tl::rows(L, 0, 32 * sub, m * KS + ks), kf[m][ks], s[m]);
         }
         if (masked) {       // (what a row does not see: exp2 gives 0)
-          int low = !valid ? 32 : A.causal ? from - i0 - 4 * h : -32, end = A.Nq - i0 - 4 * h;
+          int low = A.causal ? from - i0 - 4 * h : -32, end = A.Nq - i0 - 4 * h;
           asm volatile("" : "+v"(low), "+v"(end));
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -591,7 +591,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         if (col >= A.d) continue;
         vec v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(kback * dk[m][dt][reg + e]);
+        for (int e = 0; e < 4; ++e) v[e] = (T)(valid ? kback * dk[m][dt][reg + e] : 0.f);
         *reinterpret_cast<vec*>(dkp + m * A.d + col) = v;
       }
 #pragma unroll
@@ -602,7 +602,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       if (col >= 2 * A.d) continue;
       vec v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(vback * dv[dt][4 * q4 + e]);
+      for (int e = 0; e < 4; ++e) v[e] = (T)(valid ? vback * dv[dt][4 * q4 + e] : 0.f);
       *reinterpret_cast<vec*>(dvp + col) = v;
     }
 }

@@ -130,15 +130,23 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   };
   float cm[MPW];
   auto hide = [&](f32x16 (&s)[MPW], int k0, unsigned word) {       // what the rows do not see
-    unsigned w = word >> (4 * h);
-    int left = limit - k0 - 4 * h;
-    asm volatile("" : "+v"(w), "+v"(left));   // (else the comparisons are made for every step, in front of the branch)
+    if (word != 0xffffffffu) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int j = crow(e, 0);
-      const bool see = ((w >> j) & 1) && j < left;
+      for (int e = 0; e < 16; ++e) {
+        const bool see = da_bit(word, crow(e, 0));
 #pragma unroll
-      for (int m = 0; m < MPW; ++m) s[m][e] = see ? s[m][e] : kNegInf;
+        for (int m = 0; m < MPW; ++m) s[m][e] = see ? s[m][e] : kNegInf;
+      }
+    }
+    if (k0 + 32 > kmin) {
+      int left = limit - k0 - 4 * h;
+      asm volatile("" : "+v"(left));   // (else the comparisons are made for every step, in front of the branch)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool see = crow(e, 0) < left;
+#pragma unroll
+        for (int m = 0; m < MPW; ++m) s[m][e] = see ? s[m][e] : kNegInf;
+      }
     }
   };
   // The reference of the exponentials follows the maximum only when that has grown by more than 8 (a factor of 256 in the
@@ -208,7 +216,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
       const int row0 = 32 * (kw * Cfg::SUB + sub), k0 = t * Cfg::KT + row0;
       if (sub && k0 >= kmax) break;   // (uniform; nothing of it is seen)
       const unsigned word = keys.mask ? feed.word(row0) : 0xffffffffu;
-      if (word != 0xffffffffu || k0 + 32 > kmin) hide(s[sub & 1], k0, word);
+      hide(s[sub & 1], k0, word);
       refer(s[sub & 1]);
       if (Cfg::AHEAD && sub + 1 < Cfg::SUB) logits(L, 32 * (sub + 1), s[(sub + 1) & 1]);
       weigh(s[sub & 1], pf);

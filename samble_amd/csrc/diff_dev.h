@@ -420,6 +420,12 @@ struct Feed {
   __device__ __forceinline__ unsigned word(int row0) const { return da_uni(words(DMA ? cur : 0)[row0 >> 5]); }
 };
 
+// whether row j + 4 h of a tile's 32 is visible, h the lane's half: the comparison's result made on the scalar unit
+__device__ __forceinline__ bool da_bit(unsigned word, int j) {
+  const unsigned lo = (unsigned)((int)(word << (31 - j)) >> 31), hi = (unsigned)((int)(word << (27 - j)) >> 31);
+  return __builtin_amdgcn_inverse_ballot_w64(((unsigned long long)hi << 32) | lo);
+}
+
 template <typename T>
 __device__ __forceinline__ float da_lam(const DaArgs& A, int head) {
   return A.lam_f32 ? ((const float*)A.lam)[head] : (float)((const T*)A.lam)[head];
