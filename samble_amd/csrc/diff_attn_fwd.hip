@@ -336,28 +336,28 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 }
 
 // adds the splits of a row.  NW = 16: a workgroup per row, a wave takes every sixteenth split (many splits, few rows); NW = 1:
-// a wave per row.  A lane takes four columns.
-template <typename T, int NW>
+// LPR lanes per row.  A lane takes four columns.
+template <typename T, int NW, int LPR>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaArgs A) {
   __shared__ float red[NW == 1 ? 1 : NW][2][NW == 1 ? 4 : 256 + 4];
   const unsigned rows = (unsigned)A.Nq * A.G;
   const long all = (long)rows * A.B * A.Hkv;
-  const int lane = threadIdx.x & 63, wave = da_uni(threadIdx.x >> 6), cols = 2 * A.d;
+  const int lane = threadIdx.x % LPR, wave = NW == 1 ? 0 : da_uni(threadIdx.x >> 6), cols = 2 * A.d;
   const long pf = da_part_floats(A.d), step = all * pf;
-  constexpr int RPB = NW == 1 ? 4 : 1, kAtOnce = NW == 1 ? 4 : 2;
-  for (long u = (long)blockIdx.x * RPB + (NW == 1 ? wave : 0); u < all; u += (long)gridDim.x * RPB) {
+  constexpr int RPB = NW == 1 ? 256 / LPR : 1, kAtOnce = NW == 1 ? 4 : 2;
+  for (long u = (long)blockIdx.x * RPB + (NW == 1 ? threadIdx.x / LPR : 0); u < all; u += (long)gridDim.x * RPB) {
     const unsigned pair = (unsigned)(u / rows), r = (unsigned)(u % rows);
     const int b = pair / A.Hkv, hk = pair % A.Hkv, qi = (int)(r / (unsigned)A.G), head = hk * A.G + (int)(r % (unsigned)A.G);
     const float* w = A.part + u * pf;
     float m[2] = {kNegInf, kNegInf};
-    for (int s = lane; s < A.splits; s += 64) {
+    for (int s = NW == 1 ? 0 : lane; s < A.splits; s += NW == 1 ? 1 : 64) {
       const f32x4 t = *reinterpret_cast<const f32x4*>(w + s * step);
       m[0] = fmaxf(m[0], t[0]);
       m[1] = fmaxf(m[1], t[2]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      m[k] = wave_max64(m[k]);
+      if (NW > 1) m[k] = wave_max64(m[k]);
       if (m[k] == kNegInf) m[k] = 0.f;
     }
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
@@ -423,16 +423,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
 // ---- launches -------------------------------------------------------------------------------------------------------------
 struct FwdPlan { bool few; long blocks; int splits; };
 
-// Few rows (at most 32 of a key head) take the kernels whose waves stand along the keys.  Splits: as many as fill the waves that
-// the card holds at once (two workgroups of four waves to a CU, one of eight) and no more, since a part of a second round costs
-// a whole one (8 clouds of 1999 points, one head, fp32, d 64: 2 splits 113 us, 3 splits 138 us); each split has
-// at least four tiles of 128 keys (a split costs its partial results' way through memory), at most 128.
+// Few rows (at most 32 of a key head) take the kernels whose waves stand along the keys.  Splits: as many as fill the CUs and no
+// more, since a part of a second round costs a whole one (8 clouds of 1999 points, one head, fp32, d 64: 2 splits 113 us, 3
+// splits 138 us); each split has at least four tiles of 128 keys, since its partial results go through memory, at most 128.
+// Where two workgroups of four waves fit on a CU: as many as fill both places for few rows, and for keys so long that the parts
+// are small beside them (4 x 1024 rows, 8 heads of 64, bf16: 2048 keys 85 us, in 2 splits 74 + 18; 4096 keys 163 us, 131 + 18).
 static FwdPlan fwd_plan(bool wide, int B, int Nq, int Nk, int H, int Hkv, int d) {
   const long rows = (long)Nq * (H / Hkv), pairs = (long)B * Hkv;
   FwdPlan p;
   p.few = rows <= 32;
   p.blocks = p.few ? 1 : (rows + 127) / 128;
-  const long have = p.blocks * pairs, room = !p.few && d > (wide ? 32 : 64) ? 256 : 512;
+  const long have = p.blocks * pairs, room = p.few || (d <= (wide ? 32 : 64) && Nk >= 4096) ? 512 : 256;
   long s = room / have;
   const long most = Nk / 512;
   if (s > most) s = most;
@@ -473,10 +474,14 @@ static int fwd_type(DaArgs& A, hipStream_t s) {
   if (rc || A.splits == 1) return rc;
   const long all = (long)A.Nq * A.H * A.B;
   const long most = 1 << 20;      // workgroups of a launch: the kernel walks on
-  if (A.splits >= 16)
-    hipLaunchKernelGGL((diff_join_kernel<T, 16>), dim3((unsigned)(all < most ? all : most)), dim3(1024), 0, s, A);
-  else
-    hipLaunchKernelGGL((diff_join_kernel<T, 1>), dim3((unsigned)((all + 3) / 4 < most ? (all + 3) / 4 : most)), dim3(256), 0, s, A);
+  const int lpr = A.splits >= 16 ? 256 : A.d <= 16 ? 8 : A.d <= 32 ? 16 : A.d <= 64 ? 32 : 64;
+  const long need = (all * lpr + 255) / 256;
+  const dim3 grid((unsigned)(need < most ? need : most));
+  if (lpr == 256) hipLaunchKernelGGL((diff_join_kernel<T, 16, 64>), grid, dim3(1024), 0, s, A);
+  else if (lpr == 8) hipLaunchKernelGGL((diff_join_kernel<T, 1, 8>), grid, dim3(256), 0, s, A);
+  else if (lpr == 16) hipLaunchKernelGGL((diff_join_kernel<T, 1, 16>), grid, dim3(256), 0, s, A);
+  else if (lpr == 32) hipLaunchKernelGGL((diff_join_kernel<T, 1, 32>), grid, dim3(256), 0, s, A);
+  else if constexpr (!F) hipLaunchKernelGGL((diff_join_kernel<T, 1, 64>), grid, dim3(256), 0, s, A);
   return (int)hipGetLastError();
 }
 
