@@ -575,11 +575,12 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     last ones).  Keys behind the last query's position do not exist either (the unwritten end of a cache); those that some
     queries see and the causal order hides from others must be finite.
     A row that sees no key gives zeros and gets no gradient.  The calls Nq = 1 over a long cache split the keys over the GPU."""
-    for name, t, n in (("q", q, 5), ("k", k, 5), ("v", v, 4)):
-        if not isinstance(t, torch.Tensor) or t.dim() != n:
-            raise ValueError(f"differential_attention: {name} must be a tensor with {n} axes")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("differential_attention: q, k and v must share one type and device")
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and q.dim() == 5
+            and k.dim() == 5 and v.dim() == 4 and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        for name, t, n in (("q", q, 5), ("k", k, 5), ("v", v, 4)):
+            if not isinstance(t, torch.Tensor) or t.dim() != n:
+                raise ValueError(f"differential_attention: {name} must be a tensor with {n} axes")
+        raise ValueError("differential_attention: q, k and v must share one type and device")
     if q.dtype not in ops.ELEMENT_TYPES:
         raise ValueError(f"differential_attention: float32, float16 or bfloat16, got {q.dtype}")
     B, Nq, H, two, d = q.shape
@@ -614,7 +615,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
         return torch.zeros((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device) + torch.nan_to_num(tie)
     if lam.shape != (H,) or lam.stride(0) != 1:
         lam = lam.expand(H).contiguous()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad):
         return _DiffAttn.apply(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)
     return ops.stage_diff_attn_fwd(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)[0]
 

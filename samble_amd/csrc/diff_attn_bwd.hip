@@ -624,9 +624,10 @@ static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
 }
 
 // Few key blocks of 128: workgroups of eight waves, half the keys, four waves along the rows (64 pairs of 500 rows and 777 keys,
-// fp16, d 32: 448 blocks 34 us, in eight waves 56 us; 200 blocks and fewer: equal or slower).  Under a causal mask
-// more of them, so that the longest blocks, taken first, are not the last to end (32 pairs of 8192 rows and 2048 keys: 512
-// blocks 581 us, in eight waves 438 us); where one round holds them all, keys from both ends (8 pairs: 220 us, mirrored 160 us).
+// fp16, d 32: 448 blocks 34 us, in eight waves 56 us; of 2000 rows and 350 keys, d 64: 192 blocks 114 us, in eight waves 106 us).
+// Under a causal mask more of them, so that the longest blocks, taken first, are not the last to end (32 pairs of 8192 rows and
+// 2048 keys: 512 blocks 581 us, in eight waves 438 us); where one round holds them all, keys from both ends (8 pairs: 220 us,
+// mirrored 160 us).
 template <typename T, int DP>
 static int bwd_go(const DaArgs& A, hipStream_t s) {
   typedef DqCfg<T, DP> Q;
@@ -641,7 +642,7 @@ static int bwd_go(const DaArgs& A, hipStream_t s) {
     return dkv_go<T, DP, 4, 1>(A, false, s);
   } else {
     const long blocks = ((long)A.Nk + 127) / 128 * pairs;
-    return blocks < (A.causal ? 1024 : 192) ? dkv_go<T, DP, 2, 4>(A, A.causal && blocks < 256, s) : dkv_go<T, DP, 4, 1>(A, false, s);
+    return blocks < (A.causal ? 1024 : 200) ? dkv_go<T, DP, 2, 4>(A, A.causal && blocks < 256, s) : dkv_go<T, DP, 4, 1>(A, false, s);
   }
 }
 

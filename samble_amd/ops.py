@@ -431,6 +431,13 @@ ELEMENT_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # incl
 def _rows16(t: torch.Tensor):
     """(t, its strides but the last; 0 for axes of one): every row on 16 bytes and contiguous, rows within 2^23 and maps within
     2^28 elements of each other, a copy where it is not so."""
+    *st, _ = t.stride()
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and st[1] <= 1 << 23:
+        low = 0
+        for s in st:
+            low |= s
+        if not low & 7:      # (an axis of one may have any stride)
+            return t, st
     unit = 16 // t.element_size()
     for copy in (False, True):
         if copy:
@@ -472,7 +479,7 @@ def stage_diff_attn_bwd(q, k, v, lam, scale: float, causal: bool, lengths, q_sta
     """-> (dq, dk, dv, dlam), contiguous, in the shapes and types of q, k, v, lam: csrc/diff_attn_bwd.hip."""
     _need_gpu(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, g)
     with _on(q.device) as stream:
-        dq, dk, dv, dlam = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, lam)]
+        dq, dk, dv, dlam = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam)]
         keep, head, shape, strides, masks = _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask)
         g, gs = _rows16(g)
         nbytes = _lib.query("samble_diff_attn_bwd_workspace_bytes", head[0], shape)

@@ -239,6 +239,20 @@ def test_strided_operands_scale_and_one_lam(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_axes_of_one_with_any_stride(dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, _ = _inputs(1, 1, 40, 1, 1, 16, TYPES[dtype], 8)
+    odd = lambda t: t.as_strided(t.shape, [s if n > 1 else 2 ** 40 + 3 for s, n in zip(t.stride(), t.shape)])  # noqa: E731
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    plain = differential_attention(*leaves)
+    other = differential_attention(odd(q), odd(k), odd(v), lam)
+    assert torch.equal(plain, other)
+    for a, b in zip(torch.autograd.grad(plain, leaves, g), torch.autograd.grad(other, leaves, odd(g))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_nothing_of_missing_keys_is_used(dtype):
     from samble_amd.attention import differential_attention
     q, k, v, lam, g, gen = _inputs(3, 40, 90, 2, 2, 32, TYPES[dtype], 21)
