@@ -321,6 +321,24 @@ def test_dlam_is_not_that_of_rounded_outputs(dtype, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["keys", "causal lengths keys"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_missing_keys_beside_logits_far_below_zero(dtype, kind):
+    """Visible logits around -140: a missing key's column, read as zeros, would get probabilities beyond fp32."""
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, g, gen = _inputs(3, 200, 260, 2, 2, 32, TYPES[dtype], 61, spread=0.3)
+    q, k = q + 5, k - 5
+    causal, lengths, q_start, key_mask = _masks(kind, 3, 200, 260, gen)
+    kw = dict(causal=causal, lengths=lengths, q_start=q_start, key_mask=key_mask)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, **kw)
+    grads = torch.autograd.grad(out, leaves, g)
+    gone = ~_visible(3, 200, 260, causal, lengths, q_start, key_mask, DEV).any(1)
+    assert gone.any() and not grads[1][gone].any() and not grads[2][gone].any()
+    _check(*[t.detach() for t in leaves], g, (out.detach(), *grads), 32 ** -0.5, causal, lengths, q_start, key_mask)
+
+
+@pytest.mark.gpu
 def test_lengths_and_starts_out_of_range_are_taken_to_the_nearest():
     from samble_amd.attention import differential_attention
     q, k, v, lam, _, _ = _inputs(4, 6, 20, 2, 2, 16, torch.float32, 3)
