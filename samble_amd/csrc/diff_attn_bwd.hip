@@ -617,7 +617,6 @@ template <typename T, int DP, int KBW, int RWW>
 static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
   typedef DkvCfg<T, DP, KBW, RWW> K;
   const long grid = (((long)A.Nk + K::KB - 1) / K::KB * A.B * A.Hkv + 7) / 8 * 8;
-  if ((grid + A.H) * K::NT >= (1ll << 32)) return -22;
   if (const int rc = big_lds(diff_dkv_kernel<T, DP, KBW, RWW>, K::kLds)) return rc;
   hipLaunchKernelGGL((diff_dkv_kernel<T, DP, KBW, RWW>), dim3((unsigned)(grid + A.H)), dim3(K::NT), K::kLds, s, A, (unsigned)grid, mirror);
   return (int)hipGetLastError();
@@ -632,8 +631,8 @@ template <typename T, int DP>
 static int bwd_go(const DaArgs& A, hipStream_t s) {
   typedef DqCfg<T, DP> Q;
   const long rows = (long)A.Nq * A.G, pairs = (long)A.B * A.Hkv;
-  const long grid = ((rows + 127) / 128 * pairs + 7) / 8 * 8;
-  if (grid * Q::NT >= (1ll << 32)) return -22;
+  const long grid = ((rows + 127) / 128 * pairs + 7) / 8 * 8, blocks = ((long)A.Nk + 127) / 128 * pairs;
+  if (grid * Q::NT >= (1ll << 32) || (blocks + 8 + A.H) * 256 >= (1ll << 32)) return -22;      // (both launches, before the first)
   if (const int rc = big_lds(diff_dq_kernel<T, DP>, Q::kLds)) return rc;
   hipLaunchKernelGGL((diff_dq_kernel<T, DP>), dim3((unsigned)grid), dim3(Q::NT), Q::kLds, s, A);
   const hipError_t e = hipGetLastError();
@@ -641,7 +640,6 @@ static int bwd_go(const DaArgs& A, hipStream_t s) {
   if constexpr (DP == 128 || (DaT<T>::NP == 2 && DP == 64)) {
     return dkv_go<T, DP, 4, 1>(A, false, s);
   } else {
-    const long blocks = ((long)A.Nk + 127) / 128 * pairs;
     return blocks < (A.causal ? 1024 : 200) ? dkv_go<T, DP, 2, 4>(A, A.causal && blocks < 256, s) : dkv_go<T, DP, 4, 1>(A, false, s);
   }
 }

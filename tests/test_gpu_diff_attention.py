@@ -585,6 +585,12 @@ def test_c_entries_refuse_bad_arguments():
         for name, tail in (("samble_diff_attn_fwd", fwd_tail), ("samble_diff_attn_bwd", bwd_tail)):
             with pytest.raises(_lib.SambleError, match=name):
                 call(name, tail, **change)
+    # more workgroups than a launch holds: refused before anything is launched
+    with pytest.raises(_lib.SambleError, match="more rows and heads"):
+        call("samble_diff_attn_fwd", fwd_tail, shape=(1 << 24, 1, 1, 4, 4, 16))
+    for shape in ((1 << 24, 1, 1, 4, 4, 16), (2, 1, 1 << 30, 1, 1, 8)):
+        with pytest.raises(_lib.SambleError, match="more rows and heads"):
+            call("samble_diff_attn_bwd", bwd_tail[:-2] + (1 << 40, None), shape=shape)
     with pytest.raises(_lib.SambleError, match="out2 with lse"):
         call("samble_diff_attn_fwd", (256, 256, None, None, 0, None))
     with pytest.raises(_lib.SambleError, match="workspace"):
