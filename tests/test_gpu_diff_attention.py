@@ -453,6 +453,44 @@ def test_other_stream_and_graph_replay():
 
 
 @pytest.mark.gpu
+def test_two_threads_on_their_own_streams():
+    """Calls of different shapes at the same time, forward and backward, with the layer norm behind them."""
+    import threading
+
+    from samble_amd.attention import differential_attention
+    from samble_amd.norm import layer_norm
+
+    def work(seed, dims, dtype):
+        q, k, v, lam, g, _ = _inputs(*dims, dtype, seed)
+        leaves = [t.requires_grad_(True) for t in (q, k, v, lam)]
+        y = layer_norm(differential_attention(*leaves, causal=True))
+        return (y.detach(), *torch.autograd.grad(y, leaves, g))
+
+    jobs = [(2, (2, 300, 700, 4, 2, 64), torch.bfloat16), (5, (3, 200, 200, 2, 2, 32), torch.float32),
+            (8, (1, 2, 9000, 8, 2, 128), torch.float16)]
+    alone = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    errors = []
+
+    def run(job, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()) as _:
+                for _ in range(10):
+                    got = work(*job)
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(j, w)) for j, w in zip(jobs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """a cache whose last item starts behind 2^31 elements"""
     from samble_amd.attention import differential_attention
