@@ -1444,6 +1444,7 @@ SAMBLE_API int samble_layer_norm_bwd(int type, int w_type, const void* x, int64_
 #include "diff_args.h"
 extern "C" {
 size_t samble_diff_fwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d);
+size_t samble_diff_bwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d);
 int samble_launch_diff_fwd(int, const samble::DaArgs*, hipStream_t);
 int samble_launch_diff_bwd(int, const samble::DaArgs*, hipStream_t);
 }
@@ -1511,7 +1512,7 @@ SAMBLE_API int samble_diff_attn_fwd(int type, int lam_type, const void* q, const
 }
 
 SAMBLE_API size_t samble_diff_attn_bwd_workspace_bytes(int type, const int64_t* n) {
-  return diff_shape_ok(type, n) ? (size_t)n[0] * n[3] * 3 * n[1] * sizeof(float) : 0;
+  return diff_shape_ok(type, n) ? samble_diff_bwd_ws_bytes(type, (int)n[0], (int)n[1], (int)n[2], (int)n[3], (int)n[4], (int)n[5]) : 0;
 }
 
 SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
@@ -1528,7 +1529,7 @@ SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const
       !rows16(type, dq, &none, 1) || !rows16(type, dk, &none, 1) || !rows16(type, dv, &none, 1) || !lse || !dlam ||
       !aligned_for(lam_type, dlam))
     return fail(SAMBLE_E_INVALID, "samble_diff_attn_bwd: out, out2, lse, dout, dq, dk, dv, dlam are needed, rows on 16 bytes");
-  if (!ws || ws_bytes < samble_diff_attn_bwd_workspace_bytes(type, shape))
+  if (!ws || ws_bytes < samble_diff_attn_bwd_workspace_bytes(type, shape) || (reinterpret_cast<uintptr_t>(ws) & 15))
     return fail(SAMBLE_E_WORKSPACE, "samble_diff_attn_bwd: workspace too small (samble_diff_attn_bwd_workspace_bytes)");
   A.out = const_cast<void*>(out); A.out2 = const_cast<void*>(out2); A.lse = const_cast<float*>(lse); A.dout = dout;
   A.g_bs = strides[12]; A.g_rs = strides[13]; A.g_hs = strides[14];

@@ -1,14 +1,14 @@
 // Differential attention, backward.  With g = d loss / d out and dA = g v^T:
 //     t_m[i] = sum_j P_m dA = g . (P_m v)_i,   dS_1 = P_1 (dA - t_1),   dS_2 = -lam P_2 (dA - t_2)
 //     dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P_1 - lam P_2)^T g,  dlam = - sum_i t_2
-// The logits are formed again from q and k; P = exp2(logit - lse) with the forward's row statistics.  Two launches, no atomics:
+// The logits are formed again from q and k; P = exp2(logit - lse) with the forward's row statistics.  No atomics:
 //   diff_dq_kernel   a wave owns 32 rows (layout of the forward): first t_1 = g . out + lam t_2 and t_2 = g . out2 from the
 //                    saved outputs, then one sweep over the keys.  16-bit outputs are rounded, and so is a t of them; since
 //                    sum_j P = 1, sum_j P (dA - t) is what it lacks, and t plus that sum is kept for the second launch
 //                    (dlam adds t over all rows: there the roundings of 2^-9 or 2^-12 would not be small beside a sum of
 //                    both signs)
-//   diff_dkv_kernel  a wave owns 32 keys and sweeps over the rows of all query heads that share the key head; workgroups
-//                    behind the last one sum dlam
+//   diff_dkv_kernel  a wave owns 32 keys and sweeps over the rows of all query heads that share the key head, or over a part
+//                    of them (`splits`, added by diff_dkv_join_kernel); workgroups behind the last one sum dlam
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
 // are operands of the sums over rows as they stand.
 // P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, the type of the matrix instructions' operands (two
@@ -17,7 +17,7 @@
 //
 // Bound: as the forward's, matrix instructions (24 and 32 to a 32 x 32 block of d = 64) and vector ones of a wave in turn.
 // 8 x 2048 x 16 heads of 64, bf16, no mask: dq 510 us (810 TFLOP/s), dk and dv 660 us (835); causal on 4 key heads 281 and
-// 438 us; fp32, 32 x 1024 x 4 heads of 16: 170 and 196 us (the vector unit: two planes of P and dS).
+// 430 us; fp32, 32 x 1024 x 4 heads of 16: 166 and 190 us (the vector unit: two planes of P and dS).
 #include "diff_dev.h"
 
 namespace samble {
@@ -233,11 +233,11 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   }
 }
 
-// KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  With waves along the rows the workgroups
-// are few: half of a workgroup's keys are then taken from the front and half from the back, so that under a causal mask, where
-// the first keys are seen by all rows and the last ones by few, every workgroup has the same work; the four waves of a key
-// block stand on the four SIMDs.  VL: the values, a stationary operand like
-// the keys, stay in LDS instead of registers (64-deep heads: room for a second wave on the SIMD; 128-deep: room at all).
+// KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  `mirror`: half of a workgroup's keys are
+// taken from the front and half from the back, so that under a causal mask, where the first keys are seen by all rows and the
+// last ones by few, every workgroup has the same work; the four waves of a key block stand on the four SIMDs.  VL: the values, a
+// stationary operand like the keys, stay in LDS instead of registers (64-deep heads: room for a second wave on the SIMD;
+// 128-deep: room at all).
 template <typename T, int DP, int KBW, int RWW>
 struct DkvCfg {
   static constexpr int NW = KBW * RWW, NT = 64 * NW, KB = 32 * KBW;
@@ -298,8 +298,8 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const int wave = da_uni(tid >> 6), kb = wave / RWW, rww = RWW > 1 ? wave % RWW : 0;
   const unsigned blocks = ((unsigned)A.Nk + Cfg::KB - 1) / Cfg::KB;
   unsigned bl, pr;
-  if (!da_unit(A, main_grid, blocks, false, bl, pr)) return;
-  const int blk = bl, pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;   // (causal: the keys that most rows see first)
+  if (!da_unit(A, main_grid, blocks * A.splits, false, bl, pr)) return;
+  const int split = A.splits > 1 ? bl % A.splits : 0, blk = A.splits > 1 ? bl / A.splits : bl, pair = pr, b = da_uni(pair / A.Hkv), hk = pair - b * A.Hkv;   // (causal: the keys that most rows see first)
   const int start = da_start(A, b), len = da_len(A, b, start);
   // first key of the workgroup's k-th block of 32 (mirrored ones end where the blocks from the front begin: Nk, no key)
   auto block_key = [&](int k) {
@@ -318,6 +318,15 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const long i0 = A.causal && key0 > start ? (long)key0 - start : 0;
   const int per_head = (A.Nq + RT - 1) / RT;                            // tiles of a head
   const int tile0 = key0 >= len || i0 >= A.Nq ? per_head : (int)(i0 / RT);
+  int g = 0, t = tile0, left = (per_head - tile0) * A.G;      // the tile that comes, tiles to go
+  if (A.splits > 1) {      // (sizes end at 2^30 rows: the products fit)
+    const int each = left / A.splits, more = left - each * A.splits, first = split * each + (split < more ? split : more);
+    left = each + (split < more);
+    if (left) {
+      g = first / (per_head - tile0);
+      t += first - g * (per_head - tile0);
+    }
+  }
   Rows<T> src = {nullptr, nullptr, A.q_ms, (int)A.q_rs, (int)A.g_rs, A.Nq, A.d, nullptr};
   const T* qb = (const T*)A.q + b * A.q_bs + (long)hk * A.G * A.q_hs;
   const T* gb = (const T*)A.dout + b * A.g_bs + (long)hk * A.G * A.g_hs;
@@ -355,7 +364,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       gn = ok ? A.delta[2l * A.B * A.H * A.Nq + hd * A.Nq + i] : 0.f;
     }
   };
-  if (tile0 < per_head) issue(0, tile0);
+  if (left) issue(g, t);
 
   Frag<T> kf[2][KS], vf[Cfg::VL ? 1 : 2 * KS];
   float c[2], vscale = 1.f;     // logits' base-2 exponents per unit of the products; scale of this lane's values
@@ -427,8 +436,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   float fscale = 1.f, qscale = 1.f, gscale = 1.f;
   bool fresh = true;
 
-  int g = 0, t = tile0;
-  while (t < per_head) {
+  while (left) {
     const float lam = da_lam<T>(A, hk * A.G + g);
     buf ^= 1;
     float* stat = stats + buf * Cfg::kStat;
@@ -466,8 +474,11 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     });
     const int here = t;
     // the tile behind this one
-    if (++t == per_head && ++g < A.G) t = tile0;
-    if (t < per_head) issue(g, t);
+    if (++t == per_head) {
+      t = tile0;
+      ++g;
+    }
+    if (--left) issue(g, t);
     const float a1 = DaT<T>::NP == 2 ? fscale / vscale / feed.sy : 1.f;
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
@@ -578,6 +589,8 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     if (rww) return;
   }
   if (key >= A.Nk) return;
+  const bool part = A.splits > 1;
+  float* pp = part ? A.part + ((((long)split * A.B + b) * A.Nk + key) * A.Hkv + hk) * 4 * A.d : nullptr;      // dk, dv of one split
   typedef T vec __attribute__((ext_vector_type(4)));
   T* dkp = (T*)A.dk + (((long)b * A.Nk + key) * A.Hkv + hk) * 2 * A.d;
   T* dvp = (T*)A.dv + (((long)b * A.Nk + key) * A.Hkv + hk) * 2 * A.d;
@@ -589,10 +602,15 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       for (int q4 = 0; q4 < (DP < 32 ? 2 : 4); ++q4) {
         const int col = 32 * dt + 8 * q4 + 4 * h, reg = 4 * (q4 + (DP < 32 ? 2 * m : 0));
         if (col >= A.d) continue;
+        f32x4 x;
         vec v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(valid ? kback * dk[m][dt][reg + e] : 0.f);
-        *reinterpret_cast<vec*>(dkp + m * A.d + col) = v;
+        for (int e = 0; e < 4; ++e) {
+          x[e] = valid ? kback * dk[m][dt][reg + e] : 0.f;
+          v[e] = (T)x[e];
+        }
+        if (part) *reinterpret_cast<f32x4*>(pp + m * A.d + col) = x;
+        else *reinterpret_cast<vec*>(dkp + m * A.d + col) = v;
       }
 #pragma unroll
   for (int dt = 0; dt < DVT; ++dt)
@@ -600,11 +618,35 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
     for (int q4 = 0; q4 < 4; ++q4) {
       const int col = 32 * dt + 8 * q4 + 4 * h;
       if (col >= 2 * A.d) continue;
+      f32x4 x;
       vec v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(valid ? vback * dv[dt][4 * q4 + e] : 0.f);
-      *reinterpret_cast<vec*>(dvp + col) = v;
+      for (int e = 0; e < 4; ++e) {
+        x[e] = valid ? vback * dv[dt][4 * q4 + e] : 0.f;
+        v[e] = (T)x[e];
+      }
+      if (part) *reinterpret_cast<f32x4*>(pp + 2 * A.d + col) = x;
+      else *reinterpret_cast<vec*>(dvp + col) = v;
     }
+}
+
+// dk, dv = sums of the splits, in order (a split call has few keys: 32-bit indices)
+template <typename T>
+__global__ __launch_bounds__(256) void diff_dkv_join_kernel(DaArgs A) {
+  const unsigned d = A.d, all = (unsigned)A.B * A.Nk * A.Hkv * d;      // in fours
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
+    const float* p = A.part + 4ul * i;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
+    for (int s = 1; s < A.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p + 4ul * all * s);
+    typedef T vec __attribute__((ext_vector_type(4)));
+    vec v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (T)sum[e];
+    const unsigned row = i / d, c = 4 * (i - row * d);
+    T* to = c < 2 * d ? (T*)A.dk + (unsigned long)row * 2 * d + c : (T*)A.dv + (unsigned long)row * 2 * d + c - 2 * d;
+    *reinterpret_cast<vec*>(to) = v;
+  }
 }
 
 template <typename K>
@@ -613,23 +655,50 @@ static int big_lds(K kernel, int bytes) {
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+// How dk and dv are divided.
+//   half     workgroups of eight waves, 64 keys, four waves along the rows, where blocks of 128 keys are few (64 pairs of 500 rows
+//            and 777 keys, fp16, d 32: 448 blocks 34 us, in eight waves 56 us; of 2000 rows and 350 keys, d 64: 192 blocks 114
+//            us, in eight waves 106 us).  Under a causal mask more of them, so that the longest blocks, taken first, are not the
+//            last to end (32 pairs of 8192 rows and 2048 keys: 512 blocks 581 us, in eight waves 438 us).  Wide heads have one form.
+//   splits   of the rows, where even those are fewer than the CUs, under a causal mask fewer than two for each; at least eight
+//            tiles of 128 rows to a split (8 pairs of 8192 rows and 2048 keys, causal, bf16, d 64: 157 us, in 2 splits 127 + 8;
+//            2 pairs of 32 768 rows and 4096 keys, d 128: 1383 us, in 8 splits 371 + 24)
+//   mirror   causal, few and short: keys from both ends in a workgroup
+struct DkvPlan { bool half, mirror; int splits; };
+static DkvPlan dkv_plan(bool wide, int B, int Nq, int Nk, int H, int Hkv, bool causal) {
+  const long rows = (long)Nq * (H / Hkv), blocks = ((long)Nk + 127) / 128 * B * Hkv;
+  DkvPlan p;
+  p.half = !wide && blocks < (causal ? 1024 : 200);
+  const long have = p.half ? 2 * blocks : blocks;
+  long s = (causal ? 512 : 256) / have;
+  if (s > rows / 1024) s = rows / 1024;
+  p.splits = s < 1 ? 1 : s > 16 ? 16 : (int)s;
+  p.mirror = p.half && causal && blocks < 256 && p.splits == 1;
+  return p;
+}
+static size_t dkv_part_floats(bool wide, int B, int Nq, int Nk, int H, int Hkv, int d) {      // (causal: at least as many splits)
+  const int s = dkv_plan(wide, B, Nq, Nk, H, Hkv, true).splits, t = dkv_plan(wide, B, Nq, Nk, H, Hkv, false).splits;
+  return s > 1 || t > 1 ? (size_t)(s > t ? s : t) * B * Nk * Hkv * 4 * d : 0;
+}
+static size_t bwd_row_floats(int B, int Nq, int H) { return ((size_t)B * H * 3 * Nq + 3) / 4 * 4; }      // t_1, t_2, |dout|
+
 template <typename T, int DP, int KBW, int RWW>
 static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
   typedef DkvCfg<T, DP, KBW, RWW> K;
-  const long grid = (((long)A.Nk + K::KB - 1) / K::KB * A.B * A.Hkv + 7) / 8 * 8;
+  const long grid = (((long)A.Nk + K::KB - 1) / K::KB * A.splits * A.B * A.Hkv + 7) / 8 * 8;
   if (const int rc = big_lds(diff_dkv_kernel<T, DP, KBW, RWW>, K::kLds)) return rc;
   hipLaunchKernelGGL((diff_dkv_kernel<T, DP, KBW, RWW>), dim3((unsigned)(grid + A.H)), dim3(K::NT), K::kLds, s, A, (unsigned)grid, mirror);
+  if (A.splits > 1) {
+    const unsigned need = ((unsigned)A.B * A.Nk * A.Hkv * A.d + 255) / 256;
+    hipLaunchKernelGGL((diff_dkv_join_kernel<T>), dim3(need < 2048 ? need : 2048), dim3(256), 0, s, A);
+  }
   return (int)hipGetLastError();
 }
 
-// Few key blocks of 128: workgroups of eight waves, half the keys, four waves along the rows (64 pairs of 500 rows and 777 keys,
-// fp16, d 32: 448 blocks 34 us, in eight waves 56 us; of 2000 rows and 350 keys, d 64: 192 blocks 114 us, in eight waves 106 us).
-// Under a causal mask more of them, so that the longest blocks, taken first, are not the last to end (32 pairs of 8192 rows and
-// 2048 keys: 512 blocks 581 us, in eight waves 438 us); where one round holds them all, keys from both ends (8 pairs: 220 us,
-// mirrored 160 us).
 template <typename T, int DP>
-static int bwd_go(const DaArgs& A, hipStream_t s) {
+static int bwd_go(DaArgs& A, hipStream_t s) {
   typedef DqCfg<T, DP> Q;
+  constexpr bool kWide = DP == 128 || (DaT<T>::NP == 2 && DP == 64);
   const long rows = (long)A.Nq * A.G, pairs = (long)A.B * A.Hkv;
   const long grid = ((rows + 127) / 128 * pairs + 7) / 8 * 8, blocks = ((long)A.Nk + 127) / 128 * pairs;
   if (grid * Q::NT >= (1ll << 32) || (blocks + 8 + A.H) * 256 >= (1ll << 32)) return -22;      // (both launches, before the first)
@@ -637,15 +706,17 @@ static int bwd_go(const DaArgs& A, hipStream_t s) {
   hipLaunchKernelGGL((diff_dq_kernel<T, DP>), dim3((unsigned)grid), dim3(Q::NT), Q::kLds, s, A);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  if constexpr (DP == 128 || (DaT<T>::NP == 2 && DP == 64)) {
-    return dkv_go<T, DP, 4, 1>(A, false, s);
-  } else {
-    return blocks < (A.causal ? 1024 : 200) ? dkv_go<T, DP, 2, 4>(A, A.causal && blocks < 256, s) : dkv_go<T, DP, 4, 1>(A, false, s);
+  const DkvPlan p = dkv_plan(kWide, A.B, A.Nq, A.Nk, A.H, A.Hkv, A.causal);
+  A.splits = p.splits;
+  A.part = A.delta + bwd_row_floats(A.B, A.Nq, A.H);
+  if constexpr (!kWide) {
+    if (p.half) return dkv_go<T, DP, 2, 4>(A, p.mirror, s);
   }
+  return dkv_go<T, DP, 4, 1>(A, false, s);
 }
 
 template <typename T>
-static int bwd_type(const DaArgs& A, hipStream_t s) {
+static int bwd_type(DaArgs& A, hipStream_t s) {
   if (A.d <= 16) return bwd_go<T, 16>(A, s);
   if (A.d <= 32) return bwd_go<T, 32>(A, s);
   if (A.d <= 64) return bwd_go<T, 64>(A, s);
@@ -659,7 +730,12 @@ static int bwd_type(const DaArgs& A, hipStream_t s) {
 
 using namespace samble;
 
+extern "C" size_t samble_diff_bwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d) {
+  return (bwd_row_floats(B, Nq, H) + dkv_part_floats(d > (type == 0 ? 32 : 64), B, Nq, Nk, H, Hkv, d)) * sizeof(float);
+}
+
 extern "C" int samble_launch_diff_bwd(int type, const DaArgs* args, hipStream_t s) {
+  DaArgs A = *args;
   Timed timed(kT_diff_bwd, s);
-  return type == 0 ? bwd_type<float>(*args, s) : type == 1 ? bwd_type<f16>(*args, s) : bwd_type<bf16>(*args, s);
+  return type == 0 ? bwd_type<float>(A, s) : type == 1 ? bwd_type<f16>(A, s) : bwd_type<bf16>(A, s);
 }

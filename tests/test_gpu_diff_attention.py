@@ -198,6 +198,19 @@ def test_many_pairs(case, dtype):
     test_forward_and_gradients(case, dtype)
 
 
+# few keys under many rows: dk and dv as sums of parts of the rows
+ROWS = [(1, 2100, 130, 2, 1, 64, ""), (2, 1100, 300, 8, 2, 16, "causal lengths keys"), (1, 3000, 3000, 1, 1, 32, "causal"),
+        (1, 1500, 77, 4, 2, 128, "lengths"), (1, 5000, 40, 4, 4, 24, "keys"), (1, 2500, 200, 2, 2, 40, "causal"),
+        (1, 1025, 1, 2, 1, 8, "")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ROWS, ids=lambda c: "-".join(str(x).replace(" ", "+") or "full" for x in c))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_few_keys_under_many_rows(case, dtype):
+    test_forward_and_gradients(case, dtype)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_long_cache_single_token(dtype):
