@@ -29,13 +29,13 @@ struct FwdCfg {
   static constexpr int KT = 32 * KW * SUB;
   static constexpr int DVT = 2 * DP / 32, MPW = 2 / MW;      // 32-column pieces of an output, maps of a wave
   typedef Feed<T, DP, KT, NT> Fd;
-  static constexpr int kState = (DVT * 16 + 2) * MPW * 64;   // floats of a wave's state
+  static constexpr int kState = (DVT * 16 + 3) * MPW * 64;   // floats of a wave's state
   static constexpr int kMergeBytes = KW > 1 ? kState * 4 * (KW / 2) * RW * MW : MW > 1 ? DVT * 16 * 64 * 4 * RW : 0;
   static constexpr int kLds = Fd::kLds > kMergeBytes ? Fd::kLds : kMergeBytes;
 };
 
-// partial results of a split: per row (row order of the pair) m_1, l_1, m_2, l_2, then O_1, O_2 (2 d each)
-__device__ __forceinline__ long da_part_floats(int d) { return 4 + 4l * d; }
+// partial results of a split: per row (row order of the pair) reference, n, l of each map, two unused, then O_1, O_2 (2 d each)
+__host__ __device__ __forceinline__ long da_part_floats(int d) { return 8 + 4l * d; }
 __device__ __forceinline__ float da_inv(float l) { return l > 0.f ? 1.f / l : l; }   // (0 for a row without keys, NaN stays)
 __device__ __forceinline__ float da_lse(float m, float l, int shift) {      // log2 of the row's sum
   return l == 0.f ? __builtin_huge_valf() : m - (float)shift + __builtin_amdgcn_logf(l);
@@ -43,7 +43,8 @@ __device__ __forceinline__ float da_lse(float m, float l, int shift) {      // l
 
 // (Registers are held to two waves per SIMD, so that one wave's matrix instructions run under the other's exponentials; the
 // whole file of 512 would put every accumulator into the half that the vector unit cannot read.)
-template <typename T, int DP, int RW, int KW, int MW>
+// (BOTH: the backward comes.)
+template <typename T, int DP, int RW, int KW, int MW, bool BOTH>
 __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A) {
   typedef FwdCfg<T, DP, RW, KW, MW> Cfg;
   typedef typename Cfg::Fd Fd;
@@ -96,11 +97,15 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   }
 
   f32x16 o[MPW][DVT];
-  // reference of the exponentials, maximum from which it moves on (minus infinity: no key seen), sum
-  float ref[MPW], more_at[MPW], l[MPW];
+  // Reference of the exponentials, maximum from which it moves on (minus infinity: no key seen), sums.  The outputs are divided
+  // by the sum of the rounded operands (n): a row that sees one key almost alone gives that key's value, whatever its
+  // probability was rounded to (100 keys, d 16, bf16: outputs off by 2.1e-3 instead of 2.6e-3 of their norm, their own rounding
+  // alone 1.7e-3).  The backward makes its probabilities from the sum before rounding (l, only where it comes; fp32: the same).
+  constexpr bool kRounded = DaT<T>::NP == 1;
+  float ref[MPW], more_at[MPW], l[MPW], n[MPW];
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    ref[m] = l[m] = 0.f;
+    ref[m] = l[m] = n[m] = 0.f;
     more_at[m] = kNegInf;
 #pragma unroll
     for (int t = 0; t < DVT; ++t) o[m][t] = zero16();
@@ -168,6 +173,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         const float now = mx == kNegInf ? 0.f : mx;
         const float al = more_at[m] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ref[m] - now);      // (first: sums of zero)
         l[m] *= al;
+        n[m] *= al;
 #pragma unroll
         for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
@@ -187,9 +193,10 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           p[e] = __builtin_amdgcn_exp2f(fmaf(s[m][8 * u + e], cm[m], -sub));
-          l[m] += p[e];
+          if (BOTH) l[m] += p[e];
         }
         f[m][u] = da_pack<T>(p);
+        if constexpr (kRounded) n[m] = da_sum8(f[m][u].p[0], n[m]);
       }
     }
   };
@@ -227,6 +234,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
     l[m] = da_xor32_sum(l[m]);
+    n[m] = kRounded ? da_xor32_sum(n[m]) : l[m];
     if (more_at[m] == kNegInf) ref[m] = kNegInf;
   }
 
@@ -239,12 +247,13 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         float* w = f + ((kw - s) * RW * MW + rw * MW + mw) * Cfg::kState + lane;
 #pragma unroll
         for (int m = 0; m < MPW; ++m) {
-          w[(2 * m) * 64] = ref[m];
-          w[(2 * m + 1) * 64] = l[m];
+          w[(3 * m) * 64] = ref[m];
+          w[(3 * m + 1) * 64] = n[m];
+          w[(3 * m + 2) * 64] = l[m];
 #pragma unroll
           for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) w[(2 * MPW + (m * DVT + dt) * 16 + e) * 64] = o[m][dt][e];
+            for (int e = 0; e < 16; ++e) w[(3 * MPW + (m * DVT + dt) * 16 + e) * 64] = o[m][dt][e];
         }
       }
       __syncthreads();
@@ -252,16 +261,17 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         const float* w = f + (kw * RW * MW + rw * MW + mw) * Cfg::kState + lane;
 #pragma unroll
         for (int m = 0; m < MPW; ++m) {
-          const float m2 = w[(2 * m) * 64], l2 = w[(2 * m + 1) * 64];
+          const float m2 = w[(3 * m) * 64], n2 = w[(3 * m + 1) * 64], l2 = w[(3 * m + 2) * 64];
           const float nm = fmaxf(ref[m], m2), use = nm == kNegInf ? 0.f : nm;
           const float a1 = __builtin_amdgcn_exp2f(ref[m] - use), a2 = __builtin_amdgcn_exp2f(m2 - use);
           ref[m] = nm;
+          n[m] = n[m] * a1 + n2 * a2;
           l[m] = l[m] * a1 + l2 * a2;
 #pragma unroll
           for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[m][dt][e] = o[m][dt][e] * a1 + w[(2 * MPW + (m * DVT + dt) * 16 + e) * 64] * a2;
+              o[m][dt][e] = o[m][dt][e] * a1 + w[(3 * MPW + (m * DVT + dt) * 16 + e) * 64] * a2;
         }
       }
     }
@@ -274,8 +284,9 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 #pragma unroll
     for (int m = 0; m < MPW; ++m) {
       if (h == 0) {
-        w[2 * (m + mw)] = ref[m];
-        w[2 * (m + mw) + 1] = l[m];
+        w[3 * (m + mw)] = ref[m];
+        w[3 * (m + mw) + 1] = n[m];
+        w[3 * (m + mw) + 2] = l[m];
       }
 #pragma unroll
       for (int dt = 0; dt < DVT; ++dt)
@@ -285,7 +296,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
           if (col < 2 * A.d) {
             f32x4 v = {o[m][dt][4 * q4], o[m][dt][4 * q4 + 1], o[m][dt][4 * q4 + 2], o[m][dt][4 * q4 + 3]};
             if (DaT<T>::NP == 2) v *= vscale;
-            *reinterpret_cast<f32x4*>(w + 4 + 2 * (m + mw) * A.d + col) = v;
+            *reinterpret_cast<f32x4*>(w + 8 + 2 * (m + mw) * A.d + col) = v;
           }
         }
     }
@@ -293,7 +304,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   }
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    const float inv = da_inv(l[m]) * (DaT<T>::NP == 2 ? vscale : 1.f);
+    const float inv = da_inv(n[m]) * (DaT<T>::NP == 2 ? vscale : 1.f);
 #pragma unroll
     for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 // LPR lanes per row.  A lane takes four columns.
 template <typename T, int NW, int LPR>
 __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaArgs A) {
-  __shared__ float red[NW == 1 ? 1 : NW][2][NW == 1 ? 4 : 256 + 4];
+  __shared__ __attribute__((aligned(16))) float red[NW == 1 ? 1 : NW][2][NW == 1 ? 4 : 256 + 4];
   const unsigned rows = (unsigned)A.Nq * A.G;
   const long all = (long)rows * A.B * A.Hkv;
   const int lane = threadIdx.x % LPR, wave = NW == 1 ? 0 : da_uni(threadIdx.x >> 6), cols = 2 * A.d;
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
     for (int s = NW == 1 ? 0 : lane; s < A.splits; s += NW == 1 ? 1 : 64) {
       const f32x4 t = *reinterpret_cast<const f32x4*>(w + s * step);
       m[0] = fmaxf(m[0], t[0]);
-      m[1] = fmaxf(m[1], t[2]);
+      m[1] = fmaxf(m[1], t[3]);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -362,16 +373,18 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
     }
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
     f32x4 acc[2] = {none, none};
-    float l[2] = {0.f, 0.f};
+    float l[2] = {0.f, 0.f}, n[2] = {0.f, 0.f};
     const int c4 = 4 * lane < cols ? 4 * lane : 0;      // (lanes behind the last column: the first ones again, not used)
 #pragma unroll kAtOnce
     for (int s = NW == 1 ? 0 : wave; s < A.splits; s += NW) {
       const float* p = w + s * step;
-      const f32x4 t = *reinterpret_cast<const f32x4*>(p), x = *reinterpret_cast<const f32x4*>(p + 4 + c4);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p + 4 + cols + c4);
-      const float a0 = __builtin_amdgcn_exp2f(t[0] - m[0]), a1 = __builtin_amdgcn_exp2f(t[2] - m[1]);
-      l[0] = fmaf(t[1], a0, l[0]);
-      l[1] = fmaf(t[3], a1, l[1]);
+      const f32x4 t = *reinterpret_cast<const f32x4*>(p), t2 = *reinterpret_cast<const f32x4*>(p + 4);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + 8 + c4), y = *reinterpret_cast<const f32x4*>(p + 8 + cols + c4);
+      const float a0 = __builtin_amdgcn_exp2f(t[0] - m[0]), a1 = __builtin_amdgcn_exp2f(t[3] - m[1]);
+      n[0] = fmaf(t[1], a0, n[0]);
+      l[0] = fmaf(t[2], a0, l[0]);
+      n[1] = fmaf(t2[0], a1, n[1]);
+      l[1] = fmaf(t2[1], a1, l[1]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         acc[0][e] = fmaf(x[e], a0, acc[0][e]);
@@ -382,7 +395,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         *reinterpret_cast<f32x4*>(&red[wave][k][4 * lane]) = acc[k];
-        if (lane == 0) red[wave][k][256] = l[k];
+        if (lane == 0) {
+          red[wave][k][256] = n[k];
+          red[wave][k][257] = l[k];
+        }
       }
       __syncthreads();
       if (wave == 0) {
@@ -390,14 +406,15 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
         for (int i = 1; i < NW; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            l[k] += red[i][k][256];
+            n[k] += red[i][k][256];
+            l[k] += red[i][k][257];
             acc[k] += *reinterpret_cast<const f32x4*>(&red[i][k][4 * lane]);
           }
       }
     }
     if (NW == 1 || wave == 0) {
       if (4 * lane < cols) {
-        const float i1 = da_inv(l[0]), i2 = da_inv(l[1]), lam = da_lam<T>(A, head);
+        const float i1 = da_inv(n[0]), i2 = da_inv(n[1]), lam = da_lam<T>(A, head);
         const long o = (((long)b * A.Nq + qi) * A.H + head) * cols + 4 * lane;
         typedef T vec __attribute__((ext_vector_type(4)));
         vec a, z;
@@ -448,12 +465,13 @@ static int fwd_go(const DaArgs& A, hipStream_t s) {
   const long rows = (long)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = blocks * A.splits * A.B * A.Hkv, grid = (units + 7) / 8 * 8;
   if (grid * Cfg::NT >= (1ll << 32)) return -22;
-  const void* f = reinterpret_cast<const void*>(diff_fwd_kernel<T, DP, RW, KW, DW>);
+  constexpr bool kAlways = DaT<T>::NP == 2;
+  const auto f = A.lse ? diff_fwd_kernel<T, DP, RW, KW, DW, true> : diff_fwd_kernel<T, DP, RW, KW, DW, kAlways>;
   if (Cfg::kLds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::kLds);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::kLds);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL((diff_fwd_kernel<T, DP, RW, KW, DW>), dim3((unsigned)grid), dim3(Cfg::NT), Cfg::kLds, s, A);
+  hipLaunchKernelGGL(f, dim3((unsigned)grid), dim3(Cfg::NT), Cfg::kLds, s, A);
   return (int)hipGetLastError();
 }
 
@@ -491,7 +509,7 @@ using namespace samble;
 
 extern "C" size_t samble_diff_fwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d) {
   const FwdPlan p = fwd_plan(type == 0, B, Nq, Nk, H, Hkv, d);
-  return p.splits == 1 ? 0 : (size_t)p.splits * B * H * Nq * (4 + 4l * d) * sizeof(float);
+  return p.splits == 1 ? 0 : (size_t)p.splits * B * H * Nq * da_part_floats(d) * sizeof(float);
 }
 
 extern "C" int samble_launch_diff_fwd(int type, const DaArgs* args, hipStream_t s) {

@@ -420,6 +420,19 @@ struct Feed {
   __device__ __forceinline__ unsigned word(int row0) const { return da_uni(words(DMA ? cur : 0)[row0 >> 5]); }
 };
 
+// c + the sum of eight operands (of one plane)
+template <typename E>
+__device__ __forceinline__ float da_sum8(const vec8<E>& v, float c) {
+  const vec2<E> one = {(E)1.f, (E)1.f};
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const vec2<E> x = {v[e], v[e + 1]};
+    if constexpr (__is_same(E, bf16)) c = __builtin_amdgcn_fdot2_f32_bf16(x, one, c, false);
+    else c = __builtin_amdgcn_fdot2(x, one, c, false);
+  }
+  return c;
+}
+
 // whether row j + 4 h of a tile's 32 is visible, h the lane's half: the comparison's result made on the scalar unit
 __device__ __forceinline__ bool da_bit(unsigned word, int j) {
   const unsigned lo = (unsigned)((int)(word << (31 - j)) >> 31), hi = (unsigned)((int)(word << (27 - j)) >> 31);
