@@ -12,7 +12,7 @@
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
 // are operands of the sums over rows as they stand.
 // P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, the type of the matrix instructions' operands (two
-// planes would double their number): against float64 dq is off by 2.8e-3 and dk by 2.4e-3 of its norm in bf16, where rounding
+// planes would double their number): against float64 dq is off by 2.7e-3 and dk by 2.3e-3 of its norm in bf16, where rounding
 // the results alone is 1.7e-3; sums are fp32.
 //
 // Bound: as the forward's, matrix instructions (24 and 32 to a 32 x 32 block of d = 64) and vector ones of a wave in turn.

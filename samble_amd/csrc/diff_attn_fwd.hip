@@ -15,7 +15,7 @@
 // the other.  8 x 2048 x 16 heads of 64, bf16, no mask: 460 us, 900 TFLOP/s with both value products counted (a large matrix
 // product reaches 1175); causal on 4 key heads 238 us; fp32, 8 heads: 670 us, 310 TFLOP/s of three products each.
 // Single tokens: the cache's bytes.  16 sequences of up to 8192 keys, 8 key heads of 64, bf16: 77 + 5 us, 4.6 TB/s; one
-// sequence of 128-deep heads: 54 + 8 us, 4.9 TB/s.  A causal call whose blocks all start at once (2 x 2048, 4 key heads: 88 us)
+// sequence of 128-deep heads: 54 + 8 us, 4.9 TB/s.  A causal call whose blocks all start at once (2 x 2048, 4 key heads, for training: 93 us)
 // lasts as long as the longest row block, alone on its CU at the end.
 #include "diff_dev.h"
 
