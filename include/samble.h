@@ -735,9 +735,9 @@ int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const
                      query's position do not exist
    A row that sees no key gives zeros and takes no part in the gradients.  Values of keys that do not exist are never used.
      samble_diff_attn_fwd   out (B, Nq, H, 2 d) contiguous; out2 (sum_j P_1 v, same shape) and lse (B, H, 2, Nq) for the
-                            backward, both or neither null; workspace: samble_diff_attn_fwd_workspace_bytes (may be 0)
+                            backward, both or neither null; workspace (on 16 bytes): samble_diff_attn_fwd_workspace_bytes (may be 0)
      samble_diff_attn_bwd   dq (B, Nq, H, 2, d), dk (B, Nk, Hkv, 2, d), dv (B, Nk, Hkv, 2 d), dlam (H), contiguous, every
-                            element written; workspace: samble_diff_attn_bwd_workspace_bytes.  No atomics */
+                            element written; workspace (on 16 bytes): samble_diff_attn_bwd_workspace_bytes.  No atomics */
 size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* shape);
 int samble_diff_attn_fwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
                          const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,

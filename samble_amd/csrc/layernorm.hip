@@ -10,7 +10,8 @@
 //   inner == 1  rows of C contiguous values.  TPR threads own a row and keep it in registers, in P pieces of 16 bytes each:
 //               TPR = 8 .. 64 inside a wave for narrow rows, 256 and 512 above.  Workgroups walk the rows and read the next
 //               one ahead.  8192 x 4096 bf16: forward 24 us (5.6 TB/s, part of it from the caches), backward 38 + 4 us.
-//   inner > 1   channel-major (B, C, N) tensors: 16 lanes stand along N (16 bytes each), the other threads along C.
+//   inner > 1   channel-major (B, C, N) tensors: 16 lanes (above 256 channels 8, above 512 4) stand along N (16 bytes each), the
+//               other threads along C.
 //               32 x 128 x 2048 fp32 with residual: forward 27 us (5.0 TB/s), backward 24.5 + 4 us (4.1 TB/s).
 // Pieces are loaded at the alignment of one element, with one short piece at the end of an odd row (4099 x 5001 fp16 with
 // residual: forward 36 us, 4.6 TB/s, backward 39 + 5 us; rows of 5000 take 3 % less).  Rows beyond what registers hold (16 384
@@ -770,6 +771,9 @@ static LnPlan ln_plan(int C, int V) {
   if (pieces <= 2048) return {512, 4};
   return {0, 0};
 }
+// Lanes along N: at most 512 threads in a workgroup, whose waves then have 256 registers (8 x 512 x 2048, backward: fp32 29 us, bf16
+// 52 us; 1024 threads of 128 registers spill: 160 us, 176 us).
+constexpr int ln_chan_lanes(int tc) { return tc > 32 ? 512 / tc : 16; }
 static LnPlan ln_chan_plan(int C) {   // threads along C, pieces per thread
   if (C <= 16) return {16, 1};
   if (C <= 32) return {16, 2};
@@ -805,7 +809,7 @@ template <typename T> static long ln_lines(int C, long outer, long inner) {
     const long need = (outer * inner + 63) / 64;
     return need < kLnLoopLines ? need : kLnLoopLines;
   }
-  const int tn = pl.tpr == 128 ? 8 : 16;
+  const int tn = ln_chan_lanes(pl.tpr);
   return ln_even(outer * ((inner + tn * LnT<T>::V - 1) / (tn * LnT<T>::V)), kLnLines);
 }
 
@@ -868,8 +872,8 @@ static int ln_launch(const LnArgs& A, bool bwd, hipStream_t s) {
     case 16 * 8 + 4: return ln_chan<T, 16, 16, 4>(A, bwd, s);
     case 16 * 8 + 8: return ln_chan<T, 16, 16, 8>(A, bwd, s);
     case 32 * 8 + 8: return ln_chan<T, 16, 32, 8>(A, bwd, s);
-    case 64 * 8 + 8: return ln_chan<T, 16, 64, 8>(A, bwd, s);
-    case 128 * 8 + 8: return ln_chan<T, 8, 128, 8>(A, bwd, s);
+    case 64 * 8 + 8: return ln_chan<T, ln_chan_lanes(64), 64, 8>(A, bwd, s);
+    case 128 * 8 + 8: return ln_chan<T, ln_chan_lanes(128), 128, 8>(A, bwd, s);
   }
   const unsigned grid = ln_grid((A.outer * A.inner + 255) / 256);
   if (!bwd) {
