@@ -858,10 +858,11 @@ static int ln_launch(const LnArgs& A, bool bwd, hipStream_t s) {
     if (!bwd) {
       hipLaunchKernelGGL((ln_rows_fwd_loop_kernel<T>), dim3(ln_grid(A.outer)), dim3(1024), 0, s, A);
     } else {
-      hipLaunchKernelGGL((ln_rows_bwd_loop_kernel<T>), dim3(ln_grid(A.outer)), dim3(1024), 0, s, A);
+      // (the weight gradients first: the input's gradient may stand in dy's place)
       if (A.part)
         hipLaunchKernelGGL((ln_rows_wgrad_loop_kernel<T>), dim3((A.C + 255) / 256, (unsigned)ln_lines<T>(A.C, A.outer, 1)),
                            dim3(256), 0, s, A);
+      hipLaunchKernelGGL((ln_rows_bwd_loop_kernel<T>), dim3(ln_grid(A.outer)), dim3(1024), 0, s, A);
     }
     return (int)hipGetLastError();
   }
@@ -879,10 +880,10 @@ static int ln_launch(const LnArgs& A, bool bwd, hipStream_t s) {
   if (!bwd) {
     hipLaunchKernelGGL((ln_chan_fwd_loop_kernel<T>), dim3(grid), dim3(256), 0, s, A);
   } else {
-    hipLaunchKernelGGL((ln_chan_bwd_loop_kernel<T>), dim3(grid), dim3(256), 0, s, A);
-    if (A.part)
+    if (A.part)      // (first, as above)
       hipLaunchKernelGGL((ln_chan_wgrad_loop_kernel<T>), dim3((A.C + 3) / 4, (unsigned)ln_lines<T>(A.C, A.outer, A.inner)),
                          dim3(256), 0, s, A);
+    hipLaunchKernelGGL((ln_chan_bwd_loop_kernel<T>), dim3(grid), dim3(256), 0, s, A);
   }
   return (int)hipGetLastError();
 }

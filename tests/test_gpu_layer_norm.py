@@ -270,3 +270,35 @@ def test_c_entries_refuse_bad_arguments():
     assert _lib.query("samble_layer_norm_workspace_bytes", 5, 128, 10, 1) == 0
     with pytest.raises(_lib.SambleError, match="workspace"):
         _lib.call("samble_layer_norm_bwd", 0, 0, 64, 4, 1, 64, 4, 1, None, 0, 0, None, 64, 64, 2, 4, 1, 64, 64, 64, None, 0, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("shape", [(5, 300, 1), (9, 4099, 1), (3, 8200, 1), (3, 16390, 1), (2, 64, 37), (2, 700, 40), (2, 1030, 50)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_input_gradient_in_the_place_of_another_gradient(shape, dtype):
+    """The C entry allows dx = dy and dx = extra where those are contiguous: the same bits as into a tensor of its own."""
+    outer, C, inner = shape
+    gen = torch.Generator(device=DEV).manual_seed(C)
+    rnd = lambda *s: torch.randn(s, generator=gen, device=DEV)  # noqa: E731
+    x, dy, extra = ((rnd(*shape) + 0.3).to(dtype) for _ in range(3))
+    w, mean, rstd = 1 + 0.3 * rnd(C), 0.1 * rnd(outer * inner), 0.5 + rnd(outer * inner).abs()
+    kind = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    nbytes = _lib.query("samble_layer_norm_workspace_bytes", kind, C, outer, inner)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(dy, extra, dx):
+        dw, db = torch.empty((2, C), device=DEV)
+        _lib.call("samble_layer_norm_bwd", kind, 0, x.data_ptr(), C * inner, inner, dy.data_ptr(), C * inner, inner,
+                  extra.data_ptr(), C * inner, inner, w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), outer, C, inner,
+                  dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), nbytes, stream)
+        return dx, dw, db
+
+    apart = run(dy, extra, torch.empty_like(x))
+    over_dy = dy.clone()
+    for a, b in zip(apart, run(over_dy, extra, over_dy)):
+        assert torch.equal(a, b), "dx = dy"
+    over_extra = extra.clone()
+    for a, b in zip(apart, run(dy, over_extra, over_extra)):
+        assert torch.equal(a, b), "dx = extra"
