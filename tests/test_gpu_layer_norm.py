@@ -302,3 +302,19 @@ def test_input_gradient_in_the_place_of_another_gradient(shape, dtype):
     over_extra = extra.clone()
     for a, b in zip(apart, run(dy, over_extra, over_extra)):
         assert torch.equal(a, b), "dx = extra"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_more_channel_slices_than_workgroups_of_a_launch(dtype):
+    """A slice of few columns is one workgroup's work, and a launch holds at most 2^20 workgroups: the rest is walked to."""
+    from samble_amd.norm import layer_norm
+    B, C, N = (1 << 20) + 77, 5, 2
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    x, r = ((torch.randn((B, C, N), generator=gen, device=DEV) + 0.4).to(dtype) for _ in range(2))
+    w, b = (torch.randn(C, generator=gen, device=DEV) for _ in range(2))
+    with torch.no_grad():
+        y, s = layer_norm(x, w, b, dim=1, residual=r)
+    assert torch.equal(s, (x.float() + r.float()).to(dtype))
+    for part in (slice(0, 200), slice((1 << 20) - 50, (1 << 20) + 50), slice(B - 200, B)):
+        _close(y[part], *_ref(s[part], w, b, 1e-5, 1), 128, str(part))
