@@ -563,7 +563,7 @@ def _per_item(name: str, t, B: int, device):
 def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam, *, scale=None, causal: bool = False,
                            lengths=None, q_start=None, key_mask=None) -> torch.Tensor:
     """Attention by the difference of two softmax maps: out = (softmax(scale q_1 k_1^T) - lam softmax(scale q_2 k_2^T)) v,
-    differentiable in q, k, v and lam.
+    differentiable in q, k, v and lam (reverse mode; dual tensors of forward mode are refused).
 
     q (B, Nq, H, 2, d), k (B, Nk, Hkv, 2, d): two maps per head; v (B, Nk, Hkv, 2 d) -> (B, Nq, H, 2 d).  fp32, fp16 or
     bf16, one type, softmax statistics and sums in fp32; Hkv divides H (query head h reads key head h // (H // Hkv)); d a
@@ -615,7 +615,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
         return torch.zeros((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device) + torch.nan_to_num(tie)
     if lam.shape != (H,) or lam.stride(0) != 1:
         lam = lam.expand(H).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad):
+    if ops._differentiated(q, k, v, lam):
         return _DiffAttn.apply(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)
     return ops.stage_diff_attn_fwd(q, k, v, lam, scale, bool(causal), lengths, q_start, key_mask)[0]
 

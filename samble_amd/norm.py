@@ -11,7 +11,7 @@ from torch import nn
 
 from . import _lib
 from .ops import ELEMENT_TYPES as TYPES
-from .ops import _need_gpu, _on, _p
+from .ops import _differentiated, _need_gpu, _on, _p
 
 
 def _slices(t: torch.Tensor, dim: int):
@@ -127,7 +127,8 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                dim: int = -1, residual: Optional[torch.Tensor] = None):
-    """(x - mean) / sqrt(var + eps) * weight + bias over axis `dim` (biased variance), differentiable in every tensor.
+    """(x - mean) / sqrt(var + eps) * weight + bias over axis `dim` (biased variance), differentiable in every tensor (reverse
+    mode; dual tensors of forward mode are refused).
 
     x: fp32, fp16 or bf16, any shape; weight / bias (C,) of x's type or fp32, of one type, either may be None.  residual: x's
     shape and type; then s = x + residual (rounded to x's type) is what is normalised, and (y, s) is returned -- gradients
@@ -156,7 +157,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         raise ValueError(f"layer_norm: eps must not be negative, got {eps}")
     _need_gpu(x, weight, bias, residual)
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _differentiated(x, weight, bias, residual):
         return _LayerNorm.apply(x, weight, bias, residual, float(eps), dim)
     y, s, _, _ = stage_layer_norm_fwd(x, weight, bias, eps, dim, residual, stats=False)
     return y if residual is None else (y, s)

@@ -14,6 +14,7 @@ import os
 from typing import List, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -46,6 +47,16 @@ class _on:
         if self.guard is not None:
             self.guard.__exit__(*exc)
         return False
+
+
+def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call has to go through its autograd node: for a gradient, or (a level of forward mode is open) for the node's
+    own refusal of dual tensors, whose tangents a plain call would drop."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0
 
 
 def _need_gpu(*tensors: torch.Tensor) -> None:

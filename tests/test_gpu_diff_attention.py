@@ -650,3 +650,20 @@ def test_c_entries_refuse_bad_arguments():
         call("samble_diff_attn_fwd", fwd_tail, shape=(1, 1, 60000, 4, 2, 16))
     assert _lib.query("samble_diff_attn_fwd_workspace_bytes", 2, (ctypes.c_int64 * 6)(1, 1, 60000, 4, 2, 16)) > 0
     assert _lib.query("samble_diff_attn_fwd_workspace_bytes", 2, None) == 0
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is not dropped without a word."""
+    from torch.autograd import forward_ad
+
+    from samble_amd.attention import differential_attention
+    args = list(_inputs(1, 5, 9, 2, 1, 16, torch.float32, 3)[:4])
+    with forward_ad.dual_level():
+        plain = differential_attention(*args)
+        for n in range(4):
+            dual = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError):
+                    differential_attention(*args[:n], dual, *args[n + 1:])
+    assert torch.equal(plain, differential_attention(*args))

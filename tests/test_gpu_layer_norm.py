@@ -318,3 +318,20 @@ def test_more_channel_slices_than_workgroups_of_a_launch(dtype):
     assert torch.equal(s, (x.float() + r.float()).to(dtype))
     for part in (slice(0, 200), slice((1 << 20) - 50, (1 << 20) + 50), slice(B - 200, B)):
         _close(y[part], *_ref(s[part], w, b, 1e-5, 1), 128, str(part))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is not dropped without a word."""
+    from torch.autograd import forward_ad
+
+    from samble_amd.norm import layer_norm
+    x, t, w = torch.randn(3, 8, device=DEV), torch.randn(3, 8, device=DEV), torch.randn(8, device=DEV)
+    with forward_ad.dual_level():
+        plain = layer_norm(x, w)
+        for kw in (dict(x=forward_ad.make_dual(x, t), weight=w), dict(x=x, weight=forward_ad.make_dual(w, w)),
+                   dict(x=x, residual=forward_ad.make_dual(x, t))):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(RuntimeError):
+                    layer_norm(**kw)
+    assert torch.equal(plain, layer_norm(x, w))
