@@ -629,7 +629,8 @@ class DifferentialAttention(nn.Module):
 
     Constructor fields as Point2PointAttention's (q_in .. v_out equal, C = 2 d H with d a multiple of 8 up to 64), plus an
     optional `lambda_init` list (default 0.8 - 0.6 exp(-0.3 layer)).  forward(x, lengths=None, key_mask=None): ragged clouds
-    padded to N points -- the points that do not exist are seen by nobody (their own outputs mean nothing)."""
+    padded to N points -- the points that do not exist are seen by nobody (their own outputs mean nothing).  Parameters and x in
+    fp32, fp16 or bf16, of one type, or fp32 under torch.autocast; the result has x's type."""
 
     def __init__(self, config_attention, layer):
         super().__init__()
@@ -656,28 +657,29 @@ class DifferentialAttention(nn.Module):
         self.norm1 = LayerNorm(C, dim=1)
         self.norm2 = LayerNorm(C, dim=1)
 
-    def lam(self) -> torch.Tensor:
-        return (torch.exp((self.lambda_q1 * self.lambda_k1).sum(-1)) - torch.exp((self.lambda_q2 * self.lambda_k2).sum(-1))
-                + self.lambda_init)
+    def lam(self) -> torch.Tensor:      # (fp32 whatever the parameters' type)
+        q1, k1, q2, k2 = (p.float() for p in (self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2))
+        return torch.exp((q1 * k1).sum(-1)) - torch.exp((q2 * k2).sum(-1)) + self.lambda_init
 
     def forward(self, x, lengths=None, key_mask=None):
         if not x.is_cuda:
             raise ops._lib.SambleError("samble_amd.DifferentialAttention runs on the GPU only (no CPU fallback)")
         B, C, N = x.shape
         H, d = self.num_heads, self.depth
-        if C == 128:
+        if C == 128:      # (fp32 kernels, also under autocast; a 16-bit layer's rows are rounded to its type behind them)
             from .downsample import _Projection
             no_tokens = self.q_conv.weight.new_zeros((1, C, 0))
-            qkv = _Projection.apply(x, no_tokens, self.q_conv.weight, self.k_conv.weight, self.v_conv.weight)
-        else:      # (the projection kernels are built for 128 channels)
+            qkv = _Projection.apply(x, no_tokens, self.q_conv.weight, self.k_conv.weight, self.v_conv.weight).to(x.dtype)
+        else:      # (the projection kernels are built for 128 channels; one product of two matrices, not a batch of them)
             w = torch.cat((self.q_conv.weight, self.k_conv.weight, self.v_conv.weight)).reshape(3 * C, C)
-            qkv = torch.matmul(x.transpose(1, 2), w.t())
+            qkv = nn.functional.linear(x.transpose(1, 2).reshape(B * N, C), w).view(B, N, 3 * C)
         q, k, v = qkv.split(C, dim=2)          # rows [Q | K | V]: read where they stand
         out = differential_attention(q.view(B, N, H, 2, d), k.view(B, N, H, 2, d), v.view(B, N, H, 2 * d), self.lam(),
                                      lengths=lengths, key_mask=key_mask)
         out = self.head_norm(out) * (1.0 - self.lambda_init)
-        x, _ = self.norm1(out.reshape(B, N, C).transpose(1, 2).contiguous(), residual=x)
-        x, _ = self.norm2(_feed_forward(self.ff, x), residual=x)
+        # (under autocast the products come back in its type: the branches join the residual in the residual's)
+        x, _ = self.norm1(out.reshape(B, N, C).transpose(1, 2).to(x.dtype).contiguous(), residual=x)
+        x, _ = self.norm2(_feed_forward(self.ff, x).to(x.dtype), residual=x)
         return x
 
 

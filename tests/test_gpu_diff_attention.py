@@ -667,3 +667,63 @@ def test_forward_mode_is_refused():
                 with mode(), pytest.raises(RuntimeError):
                     differential_attention(*args[:n], dual, *args[n + 1:])
     assert torch.equal(plain, differential_attention(*args))
+
+
+def _layer_and_input(C, H, ff, N):
+    from samble_amd.attention import DifferentialAttention
+    torch.manual_seed(C + H + ff)
+    layer = DifferentialAttention(_layer_config(C, H, ff), 0).to(DEV)
+    return layer, torch.randn(2, C, N, device=DEV), torch.randn(2, C, N, device=DEV)
+
+
+def _layer_step(layer, x, g):
+    x = x.detach().requires_grad_(True)
+    y = layer(x)
+    grads = torch.autograd.grad(y.float(), [x, *layer.parameters()], g)
+    return [y.detach(), *grads]
+
+
+LAYERS = [(64, 2, 96, 65), (128, 4, 96, 70), (128, 4, 512, 100), (128, 1, 512, 33)]
+
+
+def _layer_tolerance(dtype, gradient):
+    """Relative to the norm of each tensor.  On the way from the input to the loss and back a value passes at most 16 roundings to
+    the 16-bit type (input, weight and result of four products in a row, and the same of their gradients, half of them on either
+    way), each of eps / 2, and the result's own; softmax and the three norms pass on up to twice that.  A gradient also jumps where
+    a rounding moves a hidden value over the kink of the LeakyReLU (slopes 1 and 0.2).  For normal values with an error of r times
+    their norm, r <= 8 eps (the 16 on the way there), signs differ with probability arctan(r) / pi <= r / pi; such an entry is off by 0.8
+    beside a slope of sqrt((1 + 0.04) / 2) = 0.72 in the mean square: 1.11 sqrt(r / pi) of the norm."""
+    eps = torch.finfo(dtype).eps
+    return (2 * 16 + 1) * eps / 2 + (1.11 * math.sqrt(8 * eps / math.pi) if gradient else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H,ff,N", LAYERS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_layer_under_autocast(C, H, ff, N, dtype):
+    """Every width that the constructor takes."""
+    layer, x, g = _layer_and_input(C, H, ff, N)
+    ref = _layer_step(layer, x, g)
+    with torch.autocast("cuda", dtype=dtype):
+        got = _layer_step(layer, x, g)
+    for name, a, b in zip(["y", "x", *dict(layer.named_parameters())], got, ref):
+        assert bool(torch.isfinite(a).all()), name
+        err = ((a.double() - b.double()).norm() / b.double().norm()).item()
+        assert err <= _layer_tolerance(dtype, name != "y"), f"{name}: {err:.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,H,ff,N", LAYERS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_layer_in_sixteen_bits(C, H, ff, N, dtype):
+    """Parameters and tensors of a 16-bit type, against the same values in fp32."""
+    layer, x, g = _layer_and_input(C, H, ff, N)
+    layer = layer.to(dtype)
+    x = x.to(dtype)
+    got = _layer_step(layer, x, g)
+    assert all(t.dtype == dtype for t in got)
+    ref = _layer_step(layer.float(), x.float(), g)
+    for name, a, b in zip(["y", "x", *dict(layer.named_parameters())], got, ref):
+        assert bool(torch.isfinite(a).all()), name
+        err = ((a.double() - b.double()).norm() / b.double().norm()).item()
+        assert err <= _layer_tolerance(dtype, name != "y"), f"{name}: {err:.2e}"
