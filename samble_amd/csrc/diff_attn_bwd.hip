@@ -26,7 +26,7 @@ namespace samble {
 // 128, bf16: one wave with 512 registers 604 us, a wave for each map, both forming dA, 1194 us).
 template <typename T, int DP>
 struct DqCfg {
-  static constexpr int RW = 4, NT = 64 * RW, WPS = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 1 : 2;
+  static constexpr int RW = 4, NT = 64 * RW, WPS = DP == 128 || (DaT<T>::NP > 1 && DP == 64) ? 1 : 2;
   static constexpr int SUB = 2, KT = 32 * SUB;
   typedef Feed<T, DP, KT, NT> Fd;
   static constexpr int DT = DP < 32 ? 1 : DP / 32;     // 32-column pieces of a map's gradient (16 columns: both maps on one)
@@ -65,18 +65,18 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
 
   Lane<DP> L(lane, 0);
   Frag<T> qf[2][KS], gf[2 * KS];
-  float c[2], gscale;
+  const float c = A.scale * kLog2e;
   {
     const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
+    for (int m = 0; m < 2; ++m) da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
   }
   const float lam = da_lam<T>(A, head);
-  float dot[2] = {0.f, 0.f}, norm = 0.f;      // t_1, t_2, |g|^2
+  float dot[2] = {0.f, 0.f};      // t_1, t_2
   {
     const T* gp = (const T*)A.dout + b * A.g_bs + qi * A.g_rs + head * A.g_hs;
     const long at = (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
-    gscale = da_row<T, 2 * KS>(gp, 2 * A.d, live, h, gf);
+    da_row<T, 2 * KS>(gp, 2 * A.d, live, h, gf);
 #pragma unroll
     for (int s = 0; s < 2 * KS; ++s) {
       const int o = 16 * s + 8 * h;
@@ -93,13 +93,11 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
       for (int e = 0; e < 8; ++e) {
         dot[0] = fmaf(g[e], u[e], dot[0]);
         dot[1] = fmaf(g[e], w[e], dot[1]);
-        norm = fmaf(g[e], g[e], norm);
       }
     }
     dot[0] = da_xor32_sum(dot[0]);
     dot[1] = da_xor32_sum(dot[1]);
     dot[0] = fmaf(lam, dot[1], dot[0]);
-    if (DaT<T>::NP == 2) norm = da_xor32_sum(norm);
   }
   float lse[2], tm[2], lack[2];
 #pragma unroll
@@ -109,34 +107,15 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
     tm[m] = dot[m];
     lack[m] = 0.f;
   }
-  if (DaT<T>::NP == 2 && live && h == 0)
-    A.delta[2l * A.B * A.H * A.Nq + ((long)b * A.H + head) * A.Nq + qi] = sqrtf(norm);
 
   f32x16 acc[2][DT];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[m][t] = zero16();
-  // fp32: the scale of dS (this lane's row: from the largest dA - t so far) and of the keys in the sums
-  float fscale = 1.f, kscale = 1.f;
-  unsigned fbits = 0;
-  if (DaT<T>::NP == 2) {
-    for (int m = 0; m < 2; ++m) fbits = da_max_bits(fbits, tm[m]);
-    fscale = 0.5f * da_scale(fbits);
-  }
 
   for (int t = 0; t < tiles; ++t) {
     feed.next(L);
-    if (DaT<T>::NP == 2 && kscale != feed.sx) {       // uniform, rare
-      const float f = t == 0 ? 1.f : feed.sx / kscale;
-      kscale = feed.sx;
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[m][dt][e] *= f;
-    }
     if (t + 1 < tiles) feed.issue(keys, (t + 1) * Cfg::KT);
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
@@ -146,35 +125,14 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
       f32x16 da = zero16();
 #pragma unroll
       for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(L, 1, row0, ks), gf[ks], da);
-      float a1 = 1.f;
-      if (DaT<T>::NP == 2) {
-        a1 = 1.f / gscale / feed.sy;
-        float top = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(da[e]));
-        const unsigned now = __float_as_uint(xor32_max(top) * a1);
-        if (__any(now > (fbits | 0x007fffffu))) {     // a larger power of two than so far
-          fbits = max(fbits, now);
-          const float n = 0.5f * da_scale(fbits), f = n / fscale;
-          fscale = n;
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) acc[m][dt][e] *= f;
-        }
-        a1 *= fscale;
-      }
       Frag<T> ds[2][2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         f32x16 s = zero16();
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) s = da_mma<T>(Tl::rows(L, 0, row0, m * KS + ks), qf[m][ks], s);
-        const float cm = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cm, -lse[m]));
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], c, -lse[m]));
         if (word != 0xffffffffu) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[e] = da_bit(word, crow(e, 0)) ? s[e] : 0.f;
@@ -189,8 +147,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
         for (int u = 0; u < 2; ++u) {
           float p[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            p[e] = s[8 * u + e] * (DaT<T>::NP == 2 ? fmaf(da[8 * u + e], a1, -tm[m] * fscale) : da[8 * u + e] - tm[m]);
+          for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e] * (da[8 * u + e] - tm[m]);
           if (DaT<T>::NP == 1) lack[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           ds[m][u] = da_pack<T>(p);
         }
@@ -217,7 +174,7 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float f = A.scale * (m ? -lam : 1.f) / fscale / kscale;      // dS_2 = -lam P_2 (dA - t_2)
+    const float f = A.scale * (m ? -lam : 1.f);      // dS_2 = -lam P_2 (dA - t_2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -236,14 +193,14 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
 // KBW waves along the keys, RWW along the rows of a tile (their sums meet in LDS).  `mirror`: half of a workgroup's keys are
 // taken from the front and half from the back, so that under a causal mask, where the first keys are seen by all rows and the
 // last ones by few, every workgroup has the same work; the four waves of a key block stand on the four SIMDs.  VL: the values, a
-// stationary operand like the keys, stay in LDS instead of registers (64-deep heads: room for a second wave on the SIMD;
-// 128-deep: room at all).
+// stationary operand like the keys, stay in LDS instead of registers (64-deep heads and 32-deep ones of fp32: room for a second
+// wave on the SIMD; fp32 of 64 and 128-deep heads: room at all).
 template <typename T, int DP, int KBW, int RWW>
 struct DkvCfg {
   static constexpr int NW = KBW * RWW, NT = 64 * NW, KB = 32 * KBW;
-  static constexpr bool VL = DP >= 64;
-  static constexpr int WPS = DP == 128 || (DaT<T>::NP == 2 && DP == 64) ? 1 : 2;      // waves per SIMD the registers allow
-  static constexpr int SUB = RWW == 1 && DP <= 32 ? 2 : 1, RT = 32 * RWW * SUB;       // rows of a tile
+  static constexpr bool VL = DP >= 64 || (DaT<T>::NP > 1 && DP == 32);
+  static constexpr int WPS = DP == 128 || (DaT<T>::NP > 1 && DP == 64) ? 1 : 2;      // waves per SIMD the registers allow
+  static constexpr int SUB = RWW == 1 && !VL ? 2 : 1, RT = 32 * RWW * SUB;       // rows of a tile
   typedef Feed<T, DP, RT, NT> Fd;
   typedef Tile<T, DP, KB> Vt;
   static constexpr int DT = DP < 32 ? 1 : DP / 32, DVT = 2 * DP / 32;
@@ -332,9 +289,9 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   const T* gb = (const T*)A.dout + b * A.g_bs + (long)hk * A.G * A.g_hs;
   Fd feed(smem, tid);
   Lane<DP> L(lane, 32 * rww);
-  // the rows' statistics go with their tile: copied like it (fp16 / bf16; rows behind the last: zeros), or through registers,
-  // where they take on the scales (fp32; rows behind the last: P = 0)
-  float sv[4] = {0.f, 0.f, 0.f, 0.f}, gn = 0.f;
+  // the rows' statistics go with their tile: copied like it (fp16 / bf16; rows behind the last: zeros), or through registers
+  // (fp32; rows behind the last: P = 0)
+  float sv[4] = {0.f, 0.f, 0.f, 0.f};
   int buf = 1;               // the statistics that are current; issue() fills the other ones
   auto issue = [&](int g, int t) {
     src.x = qb + g * A.q_hs;
@@ -361,70 +318,29 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       sv[1] = ok ? (ls + A.Nq)[i] : __builtin_huge_valf();
       sv[2] = ok ? tt[i] : 0.f;
       sv[3] = ok ? (tt + A.Nq)[i] : 0.f;
-      gn = ok ? A.delta[2l * A.B * A.H * A.Nq + hd * A.Nq + i] : 0.f;
     }
   };
   if (left) issue(g, t);
 
   Frag<T> kf[2][KS], vf[Cfg::VL ? 1 : 2 * KS];
-  float c[2], vscale = 1.f;     // logits' base-2 exponents per unit of the products; scale of this lane's values
-  // fp32: the largest |v_j| of the workgroup's keys; scale 2^kA of the probabilities, which leaves room for P_1 - lam P_2
-  float vnorm = 0.f;
-  int kA = 0;
+  const float c = A.scale * kLog2e;      // logits' base-2 exponents per unit of the products
   {
     const T* kp = (const T*)A.k + b * A.k_bs + hk * A.k_hs + (long)(valid ? key : 0) * A.k_rs;
     const T* vp = (const T*)A.v + b * A.v_bs + hk * A.v_hs;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(kp + m * A.k_ms, A.d, valid, h, kf[m]);
-    if constexpr (DaT<T>::NP == 2) {
-      unsigned bits = 0;
-#pragma unroll
-      for (int s = 0; s < 2 * KS; ++s) {
-        const int o = 16 * s + 8 * h;
-        Raw8<T> raw;
-        raw.load(vp + (long)(valid ? key : 0) * A.v_rs + o, valid && o < 2 * A.d);
-        float w[8];
-        raw.widen(w);
-        bits = raw.bits(bits);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vnorm = fmaf(w[e], w[e], vnorm);
-      }
-      vnorm = wave_max64(sqrtf(da_xor32_sum(vnorm)));
-      bits = da_wave_max(bits);
-      float* red = stats;      // (the waves' maxima meet here before the first tile's statistics)
-      if (lane == 0) {
-        red[2 * wave] = vnorm;
-        red[2 * wave + 1] = __uint_as_float(bits);
-      }
-      __syncthreads();
-      for (int w = 0; w < Cfg::NW; ++w) {
-        vnorm = fmaxf(vnorm, red[2 * w]);
-        bits = max(bits, __float_as_uint(red[2 * w + 1]));
-      }
-      __syncthreads();
-      vscale = da_scale(__builtin_amdgcn_readfirstlane(bits));
-      float lm = 0.f;
-      for (int g = 0; g < A.G; ++g) lm = fmaxf(lm, fabsf(da_lam<T>(A, hk * A.G + g)));
-      kA = 13 - min(max((int)((__float_as_uint(1.f + lm) >> 23) & 255) - 127, 0), 100);
-    }
+    for (int m = 0; m < 2; ++m) da_row<T, KS>(kp + m * A.k_ms, A.d, valid, h, kf[m]);
     if constexpr (Cfg::VL) {
       for (int e = tid; e < Cfg::KB * DP / 4; e += NT) {
         const int row = e / (DP / 4), pc = e % (DP / 4), kk = block_key(row >> 5) + (row & 31);
         Raw8<T> raw;
         raw.load(vp + (long)kk * A.v_rs + pc * 8, kk < len && (!km || km[kk]) && pc * 8 < 2 * A.d);
-        const Frag<T> f = raw.frag(vscale);
+        const Frag<T> f = raw.frag();
 #pragma unroll
         for (int p = 0; p < Tl::NP; ++p)
           *reinterpret_cast<vec8<typename Tl::E>*>(val + p * Cfg::Vt::kPlane + da_off<DP>(row, pc)) = f.p[p];
       }
     } else {
-#pragma unroll
-      for (int s = 0; s < 2 * KS; ++s) {
-        const int o = 16 * s + 8 * h;
-        Raw8<T> raw;
-        raw.load(vp + (long)(valid ? key : 0) * A.v_rs + o, valid && o < 2 * A.d);
-        vf[s] = raw.frag(vscale);
-      }
+      da_row<T, 2 * KS>(vp + (long)(valid ? key : 0) * A.v_rs, 2 * A.d, valid, h, vf);
     }
   }
   f32x16 dk[2][DT], dv[DVT];
@@ -432,41 +348,12 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   for (int t = 0; t < DT; ++t) dk[0][t] = dk[1][t] = zero16();
 #pragma unroll
   for (int t = 0; t < DVT; ++t) dv[t] = zero16();
-  // fp32: scale of dA - t (|dA| and |t| are at most |g| |v|), of the queries in dk's sums and of the gradients in dv's
-  float fscale = 1.f, qscale = 1.f, gscale = 1.f;
-  bool fresh = true;
 
   while (left) {
     const float lam = da_lam<T>(A, hk * A.G + g);
     buf ^= 1;
     float* stat = stats + buf * Cfg::kStat;
-    feed.next(L, __float_as_uint(gn), [&] {
-      if (DaT<T>::NP == 2) {
-        const float f = 0.5f * da_scale(__float_as_uint(__uint_as_float(feed.uz) * vnorm));
-        sv[0] -= (float)kA;
-        sv[1] -= (float)kA;
-        const float u = f * 0x1p-14f;        // |dA - t| u <= 1
-        if (u != fscale || feed.sx != qscale || feed.sy != gscale) {      // uniform, rare
-          const float a = fresh ? 1.f : (u / fscale) * (feed.sx / qscale), z = fresh ? 1.f : feed.sy / gscale;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              dk[0][dt][e] *= a;
-              dk[1][dt][e] *= a;
-            }
-#pragma unroll
-          for (int dt = 0; dt < DVT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dv[dt][e] *= z;
-          fscale = u;
-          qscale = feed.sx;
-          gscale = feed.sy;
-          fresh = false;
-        }
-        sv[2] *= fscale;
-        sv[3] *= fscale;
-      }
+    feed.next(L, [&] {
       if (!Fd::DMA && tid < RT) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) stat[e * RT + tid] = sv[e];
@@ -479,7 +366,6 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       ++g;
     }
     if (--left) issue(g, t);
-    const float a1 = DaT<T>::NP == 2 ? fscale / vscale / feed.sy : 1.f;
 #pragma unroll
     for (int sub = 0; sub < Cfg::SUB; ++sub) {
         const int row0 = 32 * (rww + sub);
@@ -517,9 +403,6 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
             for (int m = 0; m < 2; ++m) s[m][e] = see ? s[m][e] : kNegInf;
           }
         }
-        float cm[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) cm[m] = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
         // half of the rows at a time: their products run under the other half's exponentials
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -532,11 +415,11 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i = 8 * u + 4 * q4 + e, j = 4 * q4 + e;
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], cm[0], -l1[e]));
-              const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][i], cm[1], -l2[e]));
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], c, -l1[e]));
+              const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][i], c, -l2[e]));
               a[j] = p1 - p2;
-              d1[j] = p1 * (DaT<T>::NP == 2 ? fmaf(da[i], a1, -t1[e]) : da[i] - t1[e]);
-              d2[j] = p2 * (DaT<T>::NP == 2 ? fmaf(da[i], -a1, t2[e]) : t2[e] - da[i]);
+              d1[j] = p1 * (da[i] - t1[e]);
+              d2[j] = p2 * (t2[e] - da[i]);
             }
           }
           const Frag<T> af = da_pack<T>(a), f1 = da_pack<T>(d1), f2 = da_pack<T>(d2);
@@ -552,8 +435,6 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         }
     }
   }
-  const float back = DaT<T>::NP == 2 ? __uint_as_float((unsigned)(127 - kA) << 23) : 1.f;      // 2^-kA
-  const float kback = A.scale * back / fscale / qscale, vback = back / gscale;
   if constexpr (RWW > 1) {      // the waves along the rows: one after the other onto the first
     float* w = reinterpret_cast<float*>(smem) + kb * Cfg::kState + lane;
     for (int from = 1; from < RWW; ++from) {
@@ -606,7 +487,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         vec v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = valid ? kback * dk[m][dt][reg + e] : 0.f;
+          x[e] = valid ? A.scale * dk[m][dt][reg + e] : 0.f;
           v[e] = (T)x[e];
         }
         if (part) *reinterpret_cast<f32x4*>(pp + m * A.d + col) = x;
@@ -622,7 +503,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       vec v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = valid ? vback * dv[dt][4 * q4 + e] : 0.f;
+        x[e] = valid ? dv[dt][4 * q4 + e] : 0.f;
         v[e] = (T)x[e];
       }
       if (part) *reinterpret_cast<f32x4*>(pp + 2 * A.d + col) = x;
@@ -680,7 +561,7 @@ static size_t dkv_part_floats(bool wide, int B, int Nq, int Nk, int H, int Hkv, 
   const int s = dkv_plan(wide, B, Nq, Nk, H, Hkv, true).splits, t = dkv_plan(wide, B, Nq, Nk, H, Hkv, false).splits;
   return s > 1 || t > 1 ? (size_t)(s > t ? s : t) * B * Nk * Hkv * 4 * d : 0;
 }
-static size_t bwd_row_floats(int B, int Nq, int H) { return ((size_t)B * H * 3 * Nq + 3) / 4 * 4; }      // t_1, t_2, |dout|
+static size_t bwd_row_floats(int B, int Nq, int H) { return ((size_t)B * H * 2 * Nq + 3) / 4 * 4; }      // t_1, t_2
 
 template <typename T, int DP, int KBW, int RWW>
 static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
@@ -698,7 +579,7 @@ static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
 template <typename T, int DP>
 static int bwd_go(DaArgs& A, hipStream_t s) {
   typedef DqCfg<T, DP> Q;
-  constexpr bool kWide = DP == 128 || (DaT<T>::NP == 2 && DP == 64);
+  constexpr bool kWide = DP == 128 || (DaT<T>::NP > 1 && DP == 64);
   const long rows = (long)A.Nq * A.G, pairs = (long)A.B * A.Hkv;
   const long grid = ((rows + 127) / 128 * pairs + 7) / 8 * 8, blocks = ((long)A.Nk + 127) / 128 * pairs;
   if (grid * Q::NT >= (1ll << 32) || (blocks + 8 + A.H) * 256 >= (1ll << 32)) return -22;      // (both launches, before the first)

@@ -89,11 +89,11 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 
   Lane<DP> L(lane, 32 * kw * Cfg::SUB);
   Frag<T> qf[MPW][KS];
-  float c[MPW];             // logits' base-2 exponents per unit of the products
+  const float c = A.scale * kLog2e;      // logits' base-2 exponents per unit of the products
   {
     const T* qp = (const T*)A.q + b * A.q_bs + qi * A.q_rs + head * A.q_hs + mw * A.q_ms;
 #pragma unroll
-    for (int m = 0; m < MPW; ++m) c[m] = A.scale * kLog2e / da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
+    for (int m = 0; m < MPW; ++m) da_row<T, KS>(qp + m * A.q_ms, A.d, live, h, qf[m]);
   }
 
   f32x16 o[MPW][DVT];
@@ -110,7 +110,6 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 #pragma unroll
     for (int t = 0; t < DVT; ++t) o[m][t] = zero16();
   }
-  float vscale = 1.f;       // scale of the outputs' sums (fp32: the values')
 
   Frag<T> pf[MPW][2];       // the step's probabilities, operands of the value products
   // logits of the 32 keys at L + off
@@ -133,7 +132,6 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         for (int m = 0; m < MPW; ++m) o[m][dt] = da_mma<T>(vf, pf[m][u], o[m][dt]);
       }
   };
-  float cm[MPW];
   auto hide = [&](f32x16 (&s)[MPW], int k0, unsigned word) {       // what the rows do not see
     if (word != 0xffffffffu) {
 #pragma unroll
@@ -164,12 +162,12 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
       top[m] = s[m][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top[m] = fmaxf(top[m], s[m][e]);      // (of this half of the keys: enough for the question)
-      more = more || top[m] * cm[m] > more_at[m];
+      more = more || top[m] * c > more_at[m];
     }
     if (__any(more)) {
 #pragma unroll
       for (int m = 0; m < MPW; ++m) {
-        const float mx = fmaxf(more_at[m] == kNegInf ? kNegInf : ref[m], xor32_max(top[m]) * cm[m]);
+        const float mx = fmaxf(more_at[m] == kNegInf ? kNegInf : ref[m], xor32_max(top[m]) * c);
         const float now = mx == kNegInf ? 0.f : mx;
         const float al = more_at[m] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ref[m] - now);      // (first: sums of zero)
         l[m] *= al;
@@ -192,7 +190,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(s[m][8 * u + e], cm[m], -sub));
+          p[e] = __builtin_amdgcn_exp2f(fmaf(s[m][8 * u + e], c, -sub));
           if (BOTH) l[m] += p[e];
         }
         f[m][u] = da_pack<T>(p);
@@ -203,18 +201,6 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
 
   for (int t = t0; t < t1; ++t) {
     feed.next(L);
-    if (DaT<T>::NP == 2 && vscale != feed.sy) {       // uniform, rare
-      const float f = t == t0 ? 1.f : feed.sy / vscale;
-      vscale = feed.sy;
-#pragma unroll
-      for (int m = 0; m < MPW; ++m)
-#pragma unroll
-        for (int dt = 0; dt < DVT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[m][dt][e] *= f;
-    }
-#pragma unroll
-    for (int m = 0; m < MPW; ++m) cm[m] = DaT<T>::NP == 2 ? da_per(c[m], feed.sx) : c[m];
     if (t + 1 < t1) feed.issue(keys, (t + 1) * Cfg::KT);
     f32x16 s[2][MPW];
     logits(L, 0, s[0]);
@@ -277,7 +263,6 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
     }
   }
 
-  if (DaT<T>::NP == 2) vscale = 1.f / vscale;
   if (A.splits > 1) {
     if (kw || !live) return;
     float* w = A.part + (((long)split * A.B * A.Hkv + pair) * rows + r) * da_part_floats(A.d);
@@ -294,8 +279,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
         for (int q4 = 0; q4 < 4; ++q4) {
           const int col = 32 * dt + 8 * q4 + 4 * h;
           if (col < 2 * A.d) {
-            f32x4 v = {o[m][dt][4 * q4], o[m][dt][4 * q4 + 1], o[m][dt][4 * q4 + 2], o[m][dt][4 * q4 + 3]};
-            if (DaT<T>::NP == 2) v *= vscale;
+            const f32x4 v = {o[m][dt][4 * q4], o[m][dt][4 * q4 + 1], o[m][dt][4 * q4 + 2], o[m][dt][4 * q4 + 3]};
             *reinterpret_cast<f32x4*>(w + 8 + 2 * (m + mw) * A.d + col) = v;
           }
         }
@@ -304,7 +288,7 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   }
 #pragma unroll
   for (int m = 0; m < MPW; ++m) {
-    const float inv = da_inv(n[m]) * (DaT<T>::NP == 2 ? vscale : 1.f);
+    const float inv = da_inv(n[m]);
 #pragma unroll
     for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
@@ -450,7 +434,7 @@ static FwdPlan fwd_plan(bool wide, int B, int Nq, int Nk, int H, int Hkv, int d)
   FwdPlan p;
   p.few = rows <= 32;
   p.blocks = p.few ? 1 : (rows + 127) / 128;
-  const long have = p.blocks * pairs, room = p.few || (d <= (wide ? 32 : 64) && Nk >= 4096) ? 512 : 256;
+  const long have = p.blocks * pairs, room = p.few || (d <= (wide ? 16 : 64) && Nk >= 4096) ? 512 : 256;
   long s = room / have;
   const long most = Nk / 512;
   if (s > most) s = most;
@@ -465,7 +449,7 @@ static int fwd_go(const DaArgs& A, hipStream_t s) {
   const long rows = (long)A.Nq * A.G, blocks = (rows + 32 * RW - 1) / (32 * RW);
   const long units = blocks * A.splits * A.B * A.Hkv, grid = (units + 7) / 8 * 8;
   if (grid * Cfg::NT >= (1ll << 32)) return -22;
-  constexpr bool kAlways = DaT<T>::NP == 2;
+  constexpr bool kAlways = DaT<T>::NP > 1;
   const auto f = A.lse ? diff_fwd_kernel<T, DP, RW, KW, DW, true> : diff_fwd_kernel<T, DP, RW, KW, DW, kAlways>;
   if (Cfg::kLds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, Cfg::kLds);
@@ -477,12 +461,12 @@ static int fwd_go(const DaArgs& A, hipStream_t s) {
 
 template <typename T>
 static int fwd_type(DaArgs& A, hipStream_t s) {
-  const FwdPlan p = fwd_plan(DaT<T>::NP == 2, A.B, A.Nq, A.Nk, A.H, A.Hkv, A.d);
+  const FwdPlan p = fwd_plan(DaT<T>::NP > 1, A.B, A.Nq, A.Nk, A.H, A.Hkv, A.d);
   A.splits = p.splits;
-  constexpr bool F = DaT<T>::NP == 2;
+  constexpr bool F = DaT<T>::NP > 1;
   int rc = -22;
   if (A.d <= 16) rc = p.few ? fwd_go<T, 16, 1, 4, 1>(A, s) : fwd_go<T, 16, 4, 1, 1>(A, s);
-  else if (A.d <= 32) rc = p.few ? fwd_go<T, 32, 1, 2, 2>(A, s) : fwd_go<T, 32, 4, 1, 1>(A, s);
+  else if (A.d <= 32) rc = p.few ? fwd_go<T, 32, 1, 2, 2>(A, s) : fwd_go<T, 32, 4, 1, F ? 2 : 1>(A, s);
   else if (A.d <= 64) {
     if constexpr (F) rc = p.few ? fwd_go<T, 64, 1, 2, 2>(A, s) : fwd_go<T, 64, 4, 1, 2>(A, s);
     else rc = p.few ? fwd_go<T, 64, 1, 2, 2>(A, s) : fwd_go<T, 64, 4, 1, 1>(A, s);

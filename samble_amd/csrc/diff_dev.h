@@ -6,11 +6,13 @@
 // r / G of head hk G + r % G.  A key head's tiles are then read once for all its query heads, and the sums of shared heads'
 // gradients are ordinary sums over rows.
 //
-// Products.  v_mfma_f32_32x32x16 on fp16 or bf16 operands, fp32 sums.  fp16 / bf16 tensors are operands as they are; an fp32
-// tensor is split into two fp16 planes of its scaled values (x s = h + l, 22 bits) and a product takes three partial products.
-// The scales are powers of two: one per row where a row is a lane's own, one for the whole tile (the largest value so far over
-// a workgroup's tiles) where rows stream through LDS; sums are rescaled in the few steps where that one changes.  What is 2^15
-// below the largest value of the tiles loses bits below 2^-37 of that value.
+// Products.  v_mfma_f32_32x32x16 on fp16 or bf16 operands, fp32 sums.  fp16 / bf16 tensors are operands as they are.  An fp32
+// value is three bf16 planes, x = h + m + l, each the rounding of what the ones before it leave: 24 bits, none lost, at fp32's
+// own exponents, so that no value depends on the size of its neighbours.  A product takes the six partial products down to
+// 2^-16 of the first; the three left out are below 2^-23 of it.  (Two fp16 planes of scaled values take three products: 440
+// instead of 600 us for the training step of 32 x 1024 x 4 heads of 16.  But a scale is shared, and what stands 2^20 below
+// the largest value that shares it keeps 2^-18 of itself, nothing at 2^40.)  An infinity's or NaN's lower planes are NaN: all sums
+// that it enters are NaN.
 // Lane l holds
 //     A: A[row = l & 31][k = 8 (l >> 5) + e],  B: B[k = 8 (l >> 5) + e][col = l & 31],  e = 0 .. 7
 //     D: register r: D[row = crow(r, l >> 5)][col = l & 31]
@@ -36,7 +38,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <typename T> struct DaT;      // operand type, planes; kP: the probabilities' scale 2^kP (fp16 operands: off the subnormals)
-template <> struct DaT<float> { typedef f16 E; static constexpr int NP = 2, kP = 6; };
+template <> struct DaT<float> { typedef bf16 E; static constexpr int NP = 3, kP = 0; };
 template <> struct DaT<f16> { typedef f16 E; static constexpr int NP = 1, kP = 6; };
 template <> struct DaT<bf16> { typedef bf16 E; static constexpr int NP = 1, kP = 0; };
 
@@ -63,6 +65,9 @@ __device__ __forceinline__ f32x16 da_mma(const Frag<T>& a, const Frag<T>& b, f32
   if constexpr (DaT<T>::NP == 1) {
     return da_mfma(a.p[0], b.p[0], c);
   } else {   // the small products first
+    c = da_mfma(a.p[2], b.p[0], c);
+    c = da_mfma(a.p[0], b.p[2], c);
+    c = da_mfma(a.p[1], b.p[1], c);
     c = da_mfma(a.p[1], b.p[0], c);
     c = da_mfma(a.p[0], b.p[1], c);
     return da_mfma(a.p[0], b.p[0], c);
@@ -70,48 +75,27 @@ __device__ __forceinline__ f32x16 da_mma(const Frag<T>& a, const Frag<T>& b, f32
 }
 
 // eight fp32 values as an operand.  fp16 / bf16: one rounding to the tensors' own type (half a step of the value; the sums
-// that these factors enter stay in fp32); fp32 (values scaled into fp16's range): two planes, 22 bits.
+// that these factors enter stay in fp32); fp32: three planes, no bit lost.
 template <typename T>
 __device__ __forceinline__ Frag<T> da_pack(const float (&v)[8]) {
   typedef typename DaT<T>::E E;
+  constexpr int NP = DaT<T>::NP;
   Frag<T> f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const f32x2 x = {v[e], v[e + 1]};
-    const vec2<E> h = __builtin_convertvector(x, vec2<E>);
-    f.p[0][e] = h[0];
-    f.p[0][e + 1] = h[1];
-    if constexpr (DaT<T>::NP == 2) {
-      // what the first plane leaves, exactly; v_fma_mix widens the fp16 factor itself (the compiler takes two instructions).
-      // The asm reads vector results only, and v[] not before the conversion above did.
-      f32x2 r;
-      float r0, r1;
-      const unsigned hh = __builtin_bit_cast(unsigned, h);
-      asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hh), "v"(v[e]));
-      asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hh), "v"(v[e + 1]));
-      r[0] = r0;
-      r[1] = r1;
-      const vec2<E> l = __builtin_convertvector(r, vec2<E>);
-      f.p[1][e] = l[0];
-      f.p[1][e + 1] = l[1];
+    f32x2 x = {v[e], v[e + 1]};
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const vec2<E> h = __builtin_convertvector(x, vec2<E>);
+      f.p[p][e] = h[0];
+      f.p[p][e + 1] = h[1];
+      if (p + 1 < NP) {
+        x[0] -= (float)h[0];
+        x[1] -= (float)h[1];
+      }
     }
   }
   return f;
-}
-
-// the power of two that takes a value with these absolute bits to 2^13 .. 2^14 (0: left alone as far as it goes; infinities
-// and NaN stay what they are)
-__device__ __forceinline__ float da_scale(unsigned abs_bits) {
-  const unsigned e = max(abs_bits >> 23, 14u);
-  return __uint_as_float((267u - e) << 23);
-}
-// c / scale, never 0: what is masked stands for minus infinity times it
-__device__ __forceinline__ float da_per(float c, float scale) { return fmaxf(c / scale, 0x1p-126f); }
-__device__ __forceinline__ unsigned da_max_bits(unsigned a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
-__device__ __forceinline__ unsigned da_wave_max(unsigned x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, o, 64));
-  return x;
 }
 
 // eight contiguous values of a tensor, as they are read (held across a tile's computation); ok = false: zeros
@@ -123,18 +107,14 @@ template <> struct Raw8<float> {
     v[0] = ok ? *reinterpret_cast<const f32x4*>(p) : z;
     v[1] = ok ? *reinterpret_cast<const f32x4*>(p + 4) : z;
   }
-  __device__ __forceinline__ Frag<float> frag(float s) const {
-    const float t[8] = {v[0][0] * s, v[0][1] * s, v[0][2] * s, v[0][3] * s, v[1][0] * s, v[1][1] * s, v[1][2] * s, v[1][3] * s};
+  __device__ __forceinline__ Frag<float> frag() const {
+    float t[8];
+    widen(t);
     return da_pack<float>(t);
   }
   __device__ __forceinline__ void widen(float (&t)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = v[e >> 2][e & 3];
-  }
-  __device__ __forceinline__ unsigned bits(unsigned a) const {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a = da_max_bits(a, v[e >> 2][e & 3]);
-    return a;
   }
 };
 template <typename T> struct Raw8 {
@@ -143,30 +123,21 @@ template <typename T> struct Raw8 {
     const u32x4 z = {0, 0, 0, 0};
     v = __builtin_bit_cast(vec8<T>, ok ? *reinterpret_cast<const u32x4*>(p) : z);
   }
-  __device__ __forceinline__ Frag<T> frag(float) const { return Frag<T>{{v}}; }
+  __device__ __forceinline__ Frag<T> frag() const { return Frag<T>{{v}}; }
   __device__ __forceinline__ void widen(float (&t)[8]) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (float)v[e];
   }
-  __device__ __forceinline__ unsigned bits(unsigned a) const { return a; }
 };
 
-// a lane's own row as KS operands (elements 16 s + 8 h .. of a row of n live ones) and the scale they carry: the row's own
-// power of two for fp32, 1 otherwise
+// a lane's own row as KS operands (elements 16 s + 8 h .. of a row of n live ones)
 template <typename T, int KS>
-__device__ __forceinline__ float da_row(const T* p, int n, bool live, int h, Frag<T> (&f)[KS]) {
+__device__ __forceinline__ void da_row(const T* p, int n, bool live, int h, Frag<T> (&f)[KS]) {
   Raw8<T> raw[KS];
-  unsigned bits = 0;
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    raw[s].load(p + 16 * s + 8 * h, live && 16 * s + 8 * h < n);
-    bits = raw[s].bits(bits);
-  }
-  float sc = 1.f;
-  if constexpr (DaT<T>::NP == 2) sc = da_scale(max(bits, (unsigned)__shfl_xor((int)bits, 32, 64)));
+  for (int s = 0; s < KS; ++s) raw[s].load(p + 16 * s + 8 * h, live && 16 * s + 8 * h < n);
 #pragma unroll
-  for (int s = 0; s < KS; ++s) f[s] = raw[s].frag(sc);
-  return sc;
+  for (int s = 0; s < KS; ++s) f[s] = raw[s].frag();
 }
 
 // byte offset of piece c of a row of 2 DP 16-bit elements, and back from the e-th piece in LDS
@@ -271,7 +242,7 @@ struct Rows {
 // Tiles on their way from memory to LDS, NT threads together, at LDS address 0.
 //   fp16 / bf16: memory to LDS without registers (global_load_lds_dwordx4), two tiles: while one is computed on, the next
 //   lands.  The 64 pieces of a wave's copy stand one behind the other in LDS, so the lane picks the piece that belongs there.
-//   fp32: through registers, where the values are scaled and split into planes; one tile.
+//   fp32: through registers, where the values are split into planes; one tile.
 // use:  feed.issue(first, row0);  for each tile: { feed.next(L);  [feed.issue(following, row0)];  compute }
 // next() is a barrier of the workgroup.
 template <typename T, int DP, int KT, int NT>
@@ -279,9 +250,9 @@ struct Feed {
   typedef Tile<T, DP, KT> Tl;
   static constexpr bool DMA = Tl::NP == 1;
   static constexpr int kPieces = KT * DP / 4;                    // of X, and of Y
-  static constexpr int kPer = (kPieces + NT - 1) / NT, NW = NT / 64;
+  static constexpr int kPer = (kPieces + NT - 1) / NT;
   static constexpr int kBufs = Tl::kBytes * (DMA ? 2 : 1);
-  static constexpr int kLds = kBufs + 32 + (DMA ? 0 : 16 * NW);  // the tiles, their visible rows (a bit each), the waves' maxima
+  static constexpr int kLds = kBufs + 32;                        // the tiles, their visible rows (a bit each)
   static_assert(!DMA || kPieces % 64 == 0, "whole waves copy");
   static_assert(!DMA || NT % 256 == 0, "a thread's pieces stand at one place of their rows");
   static_assert(KT <= 128, "room for the visible rows");
@@ -289,12 +260,10 @@ struct Feed {
   char* lds;
   int tid, wave, cur;       // cur: the buffer that next() left current
   bool bit;
-  unsigned ux, uy, uz;      // fp32: absolute bits of the largest value so far in X, in Y, and of next()'s third value
-  float sx, sy;             // the scales of X and Y in LDS
   Raw8<T> x[DMA ? 1 : kPer], y[DMA ? 1 : kPer];
 
   __device__ __forceinline__ Feed(char* l, int t)
-      : lds(l), tid(t), wave(da_uni(t >> 6)), cur(0), bit(false), ux(0), uy(0), uz(0), sx(1.f), sy(1.f) {}
+      : lds(l), tid(t), wave(da_uni(t >> 6)), cur(0), bit(false) {}
 
   __device__ __forceinline__ int after() const { return cur ^ 1; }      // the buffer that issue() fills
   __device__ __forceinline__ unsigned* words(int buf) const { return reinterpret_cast<unsigned*>(lds + kBufs) + 4 * buf; }
@@ -357,11 +326,10 @@ struct Feed {
       }
     }
   }
-  // the tile issued last, in LDS for every wave; every wave is done with the tile before it.  fp32: its scales are sx, sy,
-  // never above those of the tiles before; `third`: a value of each thread whose largest so far joins uz; between(): run by
-  // every thread before the second barrier, with the new scales
+  // the tile issued last, in LDS for every wave; every wave is done with the tile before it.  between(): run by every thread
+  // before the last barrier
   template <typename F>
-  __device__ __forceinline__ void next(Lane<DP>& L, unsigned third, F between) {
+  __device__ __forceinline__ void next(Lane<DP>& L, F between) {
     if constexpr (DMA) {
       between();
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -369,39 +337,13 @@ struct Feed {
       cur = after();
       L.move((cur - was) * Tl::kBytes);
     } else {
-      unsigned mx = 0, my = 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        mx = x[i].bits(mx);
-        my = y[i].bits(my);
-      }
-      mx = da_wave_max(mx);
-      my = da_wave_max(my);
-      third = da_wave_max(third);
-      u32x4* red = reinterpret_cast<u32x4*>(lds + kBufs + 32);
-      if ((tid & 63) == 0) {
-        const u32x4 m = {mx, my, third, 0u};
-        red[wave] = m;
-      }
       __syncthreads();
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const u32x4 m = red[w];
-        ux = max(ux, m[0]);
-        uy = max(uy, m[1]);
-        uz = max(uz, m[2]);
-      }
-      ux = da_uni(ux);
-      uy = da_uni(uy);
-      uz = da_uni(uz);
-      sx = da_scale(ux);
-      sy = da_scale(uy);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int e = tid + NT * i;
         if (kPieces % NT && e >= kPieces) break;
         const int o = da_off<DP>(e / (DP / 4), e % (DP / 4));
-        const Frag<T> fx = x[i].frag(sx), fy = y[i].frag(sy);
+        const Frag<T> fx = x[i].frag(), fy = y[i].frag();
 #pragma unroll
         for (int p = 0; p < Tl::NP; ++p) {
           *reinterpret_cast<vec8<typename Tl::E>*>(lds + p * Tl::kPlane + o) = fx.p[p];
@@ -414,7 +356,7 @@ struct Feed {
     }
   }
   __device__ __forceinline__ void next(Lane<DP>& L) {
-    next(L, 0u, [] {});
+    next(L, [] {});
   }
   // visible rows row0 .. row0 + 31 of the current tile, a bit each
   __device__ __forceinline__ unsigned word(int row0) const { return da_uni(words(DMA ? cur : 0)[row0 >> 5]); }

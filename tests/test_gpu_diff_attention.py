@@ -727,3 +727,87 @@ def test_layer_in_sixteen_bits(C, H, ff, N, dtype):
         assert bool(torch.isfinite(a).all()), name
         err = ((a.double() - b.double()).norm() / b.double().norm()).item()
         assert err <= _layer_tolerance(dtype, name != "y"), f"{name}: {err:.2e}"
+
+
+# ---- ranges ---------------------------------------------------------------------------------------------------------------
+def _exact(q, k, v, lam, g, causal=False):
+    """float64 out, dq, dk, dv, dlam of the formulas (no key masks; causal: the queries are the last positions)"""
+    leaves = [t.detach().double().requires_grad_(True) for t in (q, k, v, lam)]
+    B, Nq, H, _, d = q.shape
+    Nk, Hkv = k.shape[1:3]
+    qq, kk, vv, lm = leaves
+    kk, vv = kk.repeat_interleave(H // Hkv, 2), vv.repeat_interleave(H // Hkv, 2)
+    s = torch.matmul(qq.permute(0, 2, 3, 1, 4), kk.permute(0, 2, 3, 4, 1).contiguous()) / math.sqrt(d)
+    if causal:
+        s = s.masked_fill(~_visible(B, Nq, Nk, True, None, None, None, DEV)[:, None, None], -math.inf)
+    p = torch.softmax(s, -1)
+    out = torch.matmul(p[:, :, 0] - lm[None, :, None, None] * p[:, :, 1], vv.transpose(1, 2)).transpose(1, 2)
+    return (out.detach(), *torch.autograd.grad(out, leaves, g.double()))
+
+
+def _step(q, k, v, lam, g, **kw):
+    from samble_amd.attention import differential_attention
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, **kw)
+    return (out.detach(), *torch.autograd.grad(out, leaves, g))
+
+
+FP32 = [(2, 70, 130, 4, 2, 16), (1, 150, 333, 2, 2, 32), (1, 65, 200, 2, 1, 64), (2, 1, 1500, 4, 2, 64), (1, 300, 40, 2, 2, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", FP32, ids=lambda c: "-".join(map(str, c)))
+def test_fp32_columns_and_keys_of_different_magnitude(case):
+    """Columns of v from 2^-40 to 2^40, channels of q and k whose product alone is of order one, keys of v from 2^-20 to 2^20:
+    the bound of each element is a few roundings of the magnitudes that the formula itself adds up for it."""
+    q, k, v, lam, g, gen = _inputs(*case, torch.float32, 5)
+    B, Nq, Nk, H, Hkv, d = case
+    power = lambda n, most: torch.exp2(torch.randint(-most, most + 1, (n,), generator=gen, device=DEV).float())  # noqa: E731
+    c = power(d, 30)
+    q, k = q * c, k / c
+    for scaled in (v * power(2 * d, 40), v * power(Nk, 20)[:, None, None]):
+        _check(q, k, scaled, lam, g, _step(q, k, scaled, lam, g), d ** -0.5, False, None, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", FP32, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_an_infinity_in_a_visible_value_stays_in_its_column(case, dtype):
+    from samble_amd.attention import differential_attention
+    q, k, v, lam, _, _ = _inputs(*case, TYPES[dtype], 7)
+    plain = differential_attention(q, k, v, lam)
+    for bad in (math.inf, -math.inf, math.nan):
+        other = v.clone()
+        other[0, 3, 0, 5] = bad
+        out = differential_attention(q, k, other, lam)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit[0, :, : case[3] // case[4], 5] = True
+        assert torch.equal(out[~hit], plain[~hit]) and not torch.isfinite(out[hit]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", FP32, ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("exponent", [-100, -80, -60, 60, 80])
+def test_fp32_gradients_of_any_size(case, exponent):
+    """The gradients are linear in dout, and dq, dk and dlam in v: times a power of two they are the same numbers, as far as
+    neither side leaves fp32's range (sums of 2^-24 steps of the largest term, which is far from either end)."""
+    q, k, v, lam, g, _ = _inputs(*case, torch.float32, 9)
+    one = _step(q, k, v, lam, g)
+    for scaled, powers in ((_step(q, k, v, lam, g * 2.0 ** exponent), (0, exponent, exponent, exponent, exponent)),
+                           (_step(q, k, v * 2.0 ** exponent, lam, g), (exponent, exponent, exponent, 0, exponent))):
+        for name, a, b, e in zip(("out", "dq", "dk", "dv", "dlam"), one, scaled, powers):
+            assert bool(torch.isfinite(b).all()), name
+            err = (b.double() * 2.0 ** -e - a.double()).norm() / a.double().norm()
+            assert err.item() <= 64 * U, f"{name}: {err.item():.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("small", [2.0 ** -86, 2.0 ** -30])
+@pytest.mark.parametrize("causal", [False, True])
+def test_fp32_rows_of_small_gradient_before_ordinary_ones(small, causal):
+    q, k, v, lam, g, _ = _inputs(1, 400, 400, 2, 2, 32, torch.float32, 13)
+    g[:, :128] *= small
+    got = _step(q, k, v, lam, g, causal=causal)
+    _check(q, k, v, lam, g, got, 32 ** -0.5, causal, None, None, None)
+    alone = _step(q, k, v, lam, g[:, :128].repeat(1, 4, 1, 1)[:, :400], causal=causal)
+    assert torch.equal(alone[1][:, :128], got[1][:, :128])
