@@ -7,8 +7,11 @@
 //                    sum_j P = 1, sum_j P (dA - t) is what it lacks, and t plus that sum is kept for the second launch
 //                    (dlam adds t over all rows: there the roundings of 2^-9 or 2^-12 would not be small beside a sum of
 //                    both signs)
+//                    fp16: dS is held times a power of two of the row, from the largest dA and t so far
 //   diff_dkv_kernel  a wave owns 32 keys and sweeps over the rows of all query heads that share the key head, or over a part
 //                    of them (`splits`, added by diff_dkv_join_kernel); workgroups behind the last one sum dlam
+//                    fp16: P and dS are held times powers of two from the largest |lam| and the largest dA and t of all
+//                    rows, which the first launch leaves
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
 // are operands of the sums over rows as they stand.
 // P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, the type of the matrix instructions' operands (two
@@ -32,6 +35,9 @@ struct DqCfg {
   static constexpr int DT = DP < 32 ? 1 : DP / 32;     // 32-column pieces of a map's gradient (16 columns: both maps on one)
   static constexpr int kLds = Fd::kLds;
 };
+
+// the waves' largest values (fp16) in the row statistics, behind t_1 and t_2
+__host__ __device__ __forceinline__ long da_bound_at(const DaArgs& A) { return 2l * A.B * A.H * A.Nq; }
 
 template <typename T, int DP>
 __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_dq_kernel(DaArgs A) {
@@ -114,6 +120,14 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[m][t] = zero16();
 
+  // fp16: dS is held times fscale, a power of two for this lane's row: |dA| and |t| times it are below 2^13
+  float fscale = 1.f;
+  unsigned fbits = 0;
+  if (kDaScaled<T>) {
+    fbits = da_max_bits(da_max_bits(0u, tm[0]), tm[1]);
+    fscale = da_scale(fbits);
+  }
+
   for (int t = 0; t < tiles; ++t) {
     feed.next(L);
     if (t + 1 < tiles) feed.issue(keys, (t + 1) * Cfg::KT);
@@ -125,6 +139,25 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
       f32x16 da = zero16();
 #pragma unroll
       for (int ks = 0; ks < 2 * KS; ++ks) da = da_mma<T>(Tl::rows(L, 1, row0, ks), gf[ks], da);
+      if (kDaScaled<T>) {
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(da[e]));
+        const unsigned now = da_max_bits(0u, xor32_max(top));
+        if (__any(now > (fbits | 0x007fffffu))) {     // a larger power of two than so far: few steps
+          fbits = max(fbits, now);
+          const float to = da_scale(fbits), f = to / fscale;
+          fscale = to;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            lack[m] *= f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[m][dt][e] *= f;
+          }
+        }
+      }
       Frag<T> ds[2][2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -147,7 +180,8 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
         for (int u = 0; u < 2; ++u) {
           float p[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = s[8 * u + e] * (da[8 * u + e] - tm[m]);
+          for (int e = 0; e < 8; ++e)
+            p[e] = s[8 * u + e] * (kDaScaled<T> ? fmaf(da[8 * u + e], fscale, -tm[m] * fscale) : da[8 * u + e] - tm[m]);
           if (DaT<T>::NP == 1) lack[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
           ds[m][u] = da_pack<T>(p);
         }
@@ -167,14 +201,20 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (DaT<T>::NP == 1) tm[m] += da_xor32_sum(lack[m]);
+    if (DaT<T>::NP == 1) tm[m] += da_xor32_sum(lack[m]) / fscale;
     if (live && h == 0) A.delta[(((long)b * A.H + head) * 2 + m) * A.Nq + qi] = tm[m];
+  }
+  if (kDaScaled<T>) {      // the wave's largest, for the second launch
+    fbits = max(fbits, da_max_bits(da_max_bits(0u, tm[0]), tm[1]));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) fbits = max(fbits, (unsigned)__shfl_xor((int)fbits, o, 64));
+    if (lane == 0) reinterpret_cast<unsigned*>(A.delta)[da_bound_at(A) + ((long)pair * blocks + blk) * RW + rw] = fbits;
   }
   if (!live) return;
   T* dq = (T*)A.dq + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float f = A.scale * (m ? -lam : 1.f);      // dS_2 = -lam P_2 (dA - t_2)
+    const float f = A.scale * (m ? -lam : 1.f) / fscale;      // dS_2 = -lam P_2 (dA - t_2)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -343,6 +383,26 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       da_row<T, 2 * KS>(vp + (long)(valid ? key : 0) * A.v_rs, 2 * A.d, valid, h, vf);
     }
   }
+  // fp16: P_1, lam P_2 and their difference are held times 2^kA (below 2^14), dS times 2^kA us (|dA - t| us <= 1)
+  float us = 1.f, up = 1.f;      // up = 2^kA
+  if constexpr (kDaScaled<T>) {
+    const unsigned rows = (unsigned)A.Nq * A.G, waves = (rows + 127) / 128 * 4;
+    const unsigned* at = reinterpret_cast<const unsigned*>(A.delta) + da_bound_at(A) + (long)pair * waves;
+    unsigned bits = 0;
+    for (unsigned e = tid; e < waves; e += NT) bits = max(bits, at[e]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) bits = max(bits, (unsigned)__shfl_xor((int)bits, o, 64));
+    unsigned* red = reinterpret_cast<unsigned*>(stats + Cfg::kStat);      // (the first tile's statistics land in the other half)
+    if (lane == 0) red[wave] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < Cfg::NW; ++w) bits = max(bits, red[w]);
+    float lm = 0.f;
+    for (int g = 0; g < A.G; ++g) lm = fmaxf(lm, fabsf(da_lam<T>(A, hk * A.G + g)));
+    const int kA = 13 - min(max((int)((__float_as_uint(1.f + lm) >> 23) & 255) - 127, 0), 100);
+    us = da_scale(da_uni(bits)) * 0x1p-14f;
+    up = __uint_as_float((unsigned)(127 + kA) << 23);
+  }
   f32x16 dk[2][DT], dv[DVT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[0][t] = dk[1][t] = zero16();
@@ -350,7 +410,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
   for (int t = 0; t < DVT; ++t) dv[t] = zero16();
 
   while (left) {
-    const float lam = da_lam<T>(A, hk * A.G + g);
+    const float lam = da_lam<T>(A, hk * A.G + g) * (kDaScaled<T> ? up * us : 1.f);
     buf ^= 1;
     float* stat = stats + buf * Cfg::kStat;
     feed.next(L, [&] {
@@ -415,9 +475,9 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int i = 8 * u + 4 * q4 + e, j = 4 * q4 + e;
-              const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], c, -l1[e]));
+              const float p1 = __builtin_amdgcn_exp2f(fmaf(s[0][i], c, -l1[e])) * (kDaScaled<T> ? up * us : 1.f);
               const float p2 = lam * __builtin_amdgcn_exp2f(fmaf(s[1][i], c, -l2[e]));
-              a[j] = p1 - p2;
+              a[j] = (p1 - p2) * (kDaScaled<T> ? 1.f / us : 1.f);
               d1[j] = p1 * (da[i] - t1[e]);
               d2[j] = p2 * (t2[e] - da[i]);
             }
@@ -435,6 +495,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         }
     }
   }
+  const float kback = A.scale / (up * us), vback = 1.f / up;
   if constexpr (RWW > 1) {      // the waves along the rows: one after the other onto the first
     float* w = reinterpret_cast<float*>(smem) + kb * Cfg::kState + lane;
     for (int from = 1; from < RWW; ++from) {
@@ -487,7 +548,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
         vec v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = valid ? A.scale * dk[m][dt][reg + e] : 0.f;
+          x[e] = valid ? kback * dk[m][dt][reg + e] : 0.f;
           v[e] = (T)x[e];
         }
         if (part) *reinterpret_cast<f32x4*>(pp + m * A.d + col) = x;
@@ -503,7 +564,7 @@ __global__ __launch_bounds__((DkvCfg<T, DP, KBW, RWW>::NT), (DkvCfg<T, DP, KBW, 
       vec v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = valid ? dv[dt][4 * q4 + e] : 0.f;
+        x[e] = valid ? vback * dv[dt][4 * q4 + e] : 0.f;
         v[e] = (T)x[e];
       }
       if (part) *reinterpret_cast<f32x4*>(pp + 2 * A.d + col) = x;
@@ -561,7 +622,10 @@ static size_t dkv_part_floats(bool wide, int B, int Nq, int Nk, int H, int Hkv, 
   const int s = dkv_plan(wide, B, Nq, Nk, H, Hkv, true).splits, t = dkv_plan(wide, B, Nq, Nk, H, Hkv, false).splits;
   return s > 1 || t > 1 ? (size_t)(s > t ? s : t) * B * Nk * Hkv * 4 * d : 0;
 }
-static size_t bwd_row_floats(int B, int Nq, int H) { return ((size_t)B * H * 2 * Nq + 3) / 4 * 4; }      // t_1, t_2
+// t_1, t_2 of the rows, and the largest values of a pair's waves of 32 rows
+static size_t bwd_row_floats(int B, int Nq, int H, int Hkv) {
+  return ((size_t)B * H * 2 * Nq + ((size_t)Nq * (H / Hkv) + 127) / 128 * 4 * B * Hkv + 3) / 4 * 4;
+}
 
 template <typename T, int DP, int KBW, int RWW>
 static int dkv_go(const DaArgs& A, bool mirror, hipStream_t s) {
@@ -589,7 +653,7 @@ static int bwd_go(DaArgs& A, hipStream_t s) {
   if (e != hipSuccess) return (int)e;
   const DkvPlan p = dkv_plan(kWide, A.B, A.Nq, A.Nk, A.H, A.Hkv, A.causal);
   A.splits = p.splits;
-  A.part = A.delta + bwd_row_floats(A.B, A.Nq, A.H);
+  A.part = A.delta + bwd_row_floats(A.B, A.Nq, A.H, A.Hkv);
   if constexpr (!kWide) {
     if (p.half) return dkv_go<T, DP, 2, 4>(A, p.mirror, s);
   }
@@ -612,7 +676,7 @@ static int bwd_type(DaArgs& A, hipStream_t s) {
 using namespace samble;
 
 extern "C" size_t samble_diff_bwd_ws_bytes(int type, int B, int Nq, int Nk, int H, int Hkv, int d) {
-  return (bwd_row_floats(B, Nq, H) + dkv_part_floats(d > (type == 0 ? 32 : 64), B, Nq, Nk, H, Hkv, d)) * sizeof(float);
+  return (bwd_row_floats(B, Nq, H, Hkv) + dkv_part_floats(d > (type == 0 ? 32 : 64), B, Nq, Nk, H, Hkv, d)) * sizeof(float);
 }
 
 extern "C" int samble_launch_diff_bwd(int type, const DaArgs* args, hipStream_t s) {

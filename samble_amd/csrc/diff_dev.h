@@ -98,6 +98,20 @@ __device__ __forceinline__ Frag<T> da_pack(const float (&v)[8]) {
   return f;
 }
 
+// fp16 operands of the backward, P and dS, are held times powers of two (2^11 steps at 2^13, 2^-25 at the low end: half a step is
+// 2^-12 of a term as long as that is above 2^-27 of the largest one).
+template <typename T> constexpr bool kDaScaled = __is_same(T, f16);
+// the power of two that takes a value with these absolute bits to 2^12 .. 2^13 (0: far up)
+__device__ __forceinline__ float da_scale(unsigned abs_bits) {
+  const unsigned e = max(abs_bits >> 23, 13u);
+  return __uint_as_float((266u - e) << 23);
+}
+// larger of two absolute bits, the second one only if it is finite (an infinity or NaN is one in all its sums, at any scale)
+__device__ __forceinline__ unsigned da_max_bits(unsigned a, float x) {
+  const unsigned u = __float_as_uint(x) & 0x7fffffffu;
+  return u < 0x7f800000u && u > a ? u : a;
+}
+
 // eight contiguous values of a tensor, as they are read (held across a tile's computation); ok = false: zeros
 template <typename T> struct Raw8;
 template <> struct Raw8<float> {

@@ -811,3 +811,38 @@ def test_fp32_rows_of_small_gradient_before_ordinary_ones(small, causal):
     _check(q, k, v, lam, g, got, 32 ** -0.5, causal, None, None, None)
     alone = _step(q, k, v, lam, g[:, :128].repeat(1, 4, 1, 1)[:, :400], causal=causal)
     assert torch.equal(alone[1][:, :128], got[1][:, :128])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** -10, 1.0, 2.0 ** 10])
+@pytest.mark.parametrize("case", [(1, 600, 1000, 8, 1, 16), (2, 500, 700, 4, 2, 32), (1, 257, 900, 8, 2, 64), (1, 200, 2000, 4, 1, 128),
+                                  (1, 40, 4000, 2, 2, 64)], ids=lambda c: "-".join(map(str, c)))
+def test_fp16_gradients_of_any_size(case, size):
+    """dS of a thousand keys is a thousandth of a gradient: as an operand of the type it is held where it has all its bits.
+    Bound, against the norm of each gradient in float64: P and dS rounded once each, t from outputs that were rounded once, each
+    2^-11 of the terms, whose norm is at most four times the result's (independent signs); the result's own rounding comes on top."""
+    q, k, v, lam, g, _ = _inputs(*case, torch.float16, 4)
+    g = (g.float() * size).half()
+    want = _exact(q, k, v, lam, g)
+    for name, a, b in zip(("dq", "dk", "dv", "dlam"), _step(q, k, v, lam, g)[1:], want[1:]):
+        assert bool(torch.isfinite(a).all()), name
+        own = (b.to(a.dtype).double() - b).norm()
+        err = (a.double() - b).norm()
+        assert err <= own + 3 * 4 * 2.0 ** -11 * b.norm(), f"{name}: {(err / b.norm()).item():.2e}, rounding alone {(own / b.norm()).item():.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lam_value", [0.4, 300.0])
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_fp16_terms_beyond_the_type(d, lam_value):
+    """Few keys and large gradients: P (dA - t) is beyond 65504, the gradients are not."""
+    q, k, v, _, g, _ = _inputs(1, 90, 4, 2, 1, d, torch.float16, 6)
+    k, v, g = (0.02 * k.float()).half(), (16 * v.float() / math.sqrt(d / 16)).half(), (4000 * g.float() / max(1.0, lam_value)).half()
+    q = (0.02 * q.float()).half()
+    lam = torch.full((2,), lam_value, device=DEV)
+    want = _exact(q, k, v, lam, g)
+    got = _step(q, k, v, lam, g)
+    for name, a, b in zip(("out", "dq", "dk"), got, want):
+        assert bool(torch.isfinite(a).all()) and float(b.abs().max()) < 60000, name
+        err = ((a.double() - b).norm() / b.norm()).item()
+        assert err <= 4 * 4 * 2.0 ** -11, f"{name}: {err:.2e}"
