@@ -737,7 +737,11 @@ int samble_amax_bwd_f32(const float* x, int64_t x_bs, int B, int C, int N, const
      samble_diff_attn_fwd   out (B, Nq, H, 2 d) contiguous; out2 (sum_j P_1 v, same shape) and lse (B, H, 2, Nq) for the
                             backward, both or neither null; workspace (on 16 bytes): samble_diff_attn_fwd_workspace_bytes (may be 0)
      samble_diff_attn_bwd   dq (B, Nq, H, 2, d), dk (B, Nk, Hkv, 2, d), dv (B, Nk, Hkv, 2 d), dlam (H), contiguous, every
-                            element written; workspace (on 16 bytes): samble_diff_attn_bwd_workspace_bytes.  No atomics */
+                            element written; workspace (on 16 bytes): samble_diff_attn_bwd_workspace_bytes.  No atomics
+     ..._rest               the same with what the roundings of out and out2 to a 16-bit type leave, a byte each: rest (B, Nq, H,
+                            2 d, 2) on 16 bytes, written by the forward, read by the backward of the same call (null: as the
+                            entries without it; fp32 has none).  dq then comes from row sums of 15 bits or more instead of
+                            the rounded outputs' */
 size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* shape);
 int samble_diff_attn_fwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
                          const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
@@ -748,6 +752,15 @@ int samble_diff_attn_bwd(int type, int lam_type, const void* q, const void* k, c
                          const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
                          const uint8_t* key_mask, int causal, float scale, const void* out, const void* out2, const float* lse,
                          const void* dout, void* dq, void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream);
+int samble_diff_attn_fwd_rest(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                              const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                              const uint8_t* key_mask, int causal, float scale, void* out, void* out2, float* lse, int8_t* rest,
+                              void* ws, size_t ws_bytes, void* stream);
+int samble_diff_attn_bwd_rest(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                              const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
+                              const uint8_t* key_mask, int causal, float scale, const void* out, const void* out2,
+                              const float* lse, const int8_t* rest, const void* dout, void* dq, void* dk, void* dv, void* dlam,
+                              void* ws, size_t ws_bytes, void* stream);
 /* Layer normalisation over the middle axis of (outer, C, inner): inner = 1 for rows of C contiguous values (a row every x_os
    elements; x_cs unused), otherwise channel-major slices as this library's layers hold them, (B, C, N) with channel stride
    x_cs and contiguous columns.  type / w_type: SAMBLE_TYPE_* of the tensors / of weight and bias (w_type = type or F32; either

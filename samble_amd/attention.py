@@ -537,16 +537,18 @@ class _DiffAttn(torch.autograd.Function):
     # (no autocast decorators: no torch arithmetic runs in either direction, the kernels take the types they are given)
     @staticmethod
     def forward(ctx, q, k, v, lam, scale, causal, lengths, q_start, key_mask):
-        out, out2, lse = ops.stage_diff_attn_fwd(q, k, v, lam, scale, causal, lengths, q_start, key_mask, for_backward=True)
-        ctx.save_for_backward(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse)
+        # (16-bit types: a byte beside each saved value, for row sums in the backward that are not those of rounded outputs)
+        rest = q.new_empty((*q.shape[:3], v.shape[3], 2), dtype=torch.int8) if q.dtype != torch.float32 else None
+        out, out2, lse = ops.stage_diff_attn_fwd(q, k, v, lam, scale, causal, lengths, q_start, key_mask, for_backward=True, rest=rest)
+        ctx.save_for_backward(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, rest)
         ctx.cfg = (scale, causal)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, lam, lengths, q_start, key_mask, out, out2, lse = ctx.saved_tensors
-        grads = ops.stage_diff_attn_bwd(q, k, v, lam, *ctx.cfg, lengths, q_start, key_mask, out, out2, lse, g.to(q.dtype))
+        q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, rest = ctx.saved_tensors
+        grads = ops.stage_diff_attn_bwd(q, k, v, lam, *ctx.cfg, lengths, q_start, key_mask, out, out2, lse, g.to(q.dtype), rest)
         return tuple(d if need else None for d, need in zip(grads, ctx.needs_input_grad)) + (None,) * 5
 
 

@@ -1491,10 +1491,22 @@ SAMBLE_API size_t samble_diff_attn_fwd_workspace_bytes(int type, const int64_t* 
   return diff_shape_ok(type, n) ? samble_diff_fwd_ws_bytes(type, (int)n[0], (int)n[1], (int)n[2], (int)n[3], (int)n[4], (int)n[5]) : 0;
 }
 
+static bool rest_ok(int type, const void* rest, const void* out2) {
+  return !rest || (type != SAMBLE_TYPE_F32 && out2 && (reinterpret_cast<uintptr_t>(rest) & 15) == 0);
+}
+
 SAMBLE_API int samble_diff_attn_fwd(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
                                     const int64_t* shape, const int64_t* strides, const int32_t* lengths, const int32_t* q_start,
                                     const uint8_t* key_mask, int causal, float scale, void* out, void* out2, float* lse, void* ws,
                                     size_t ws_bytes, void* stream) {
+  return samble_diff_attn_fwd_rest(type, lam_type, q, k, v, lam, shape, strides, lengths, q_start, key_mask, causal, scale, out, out2,
+                                   lse, nullptr, ws, ws_bytes, stream);
+}
+
+SAMBLE_API int samble_diff_attn_fwd_rest(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                                         const int64_t* shape, const int64_t* strides, const int32_t* lengths,
+                                         const int32_t* q_start, const uint8_t* key_mask, int causal, float scale, void* out,
+                                         void* out2, float* lse, int8_t* rest, void* ws, size_t ws_bytes, void* stream) {
   samble::DaArgs A;
   if (int rc = diff_args("samble_diff_attn_fwd" SAMBLE_DIFF_NEEDS, type, lam_type, q, k, v, lam, shape, strides, lengths, q_start,
                          key_mask, causal, scale, &A))
@@ -1502,10 +1514,12 @@ SAMBLE_API int samble_diff_attn_fwd(int type, int lam_type, const void* q, const
   const int64_t none = 0;
   if (!rows16(type, out, &none, 1) || (out2 && !rows16(type, out2, &none, 1)) || (!out2) != (!lse))
     return fail(SAMBLE_E_INVALID, "samble_diff_attn_fwd: out on 16 bytes, out2 with lse or neither");
+  if (!rest_ok(type, rest, out2))
+    return fail(SAMBLE_E_INVALID, "samble_diff_attn_fwd: rest with out2 of a 16-bit type only, on 16 bytes");
   const size_t need = samble_diff_attn_fwd_workspace_bytes(type, shape);
   if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 15)))
     return fail(SAMBLE_E_WORKSPACE, "samble_diff_attn_fwd: workspace too small (samble_diff_attn_fwd_workspace_bytes)");
-  A.out = out; A.out2 = out2; A.lse = lse; A.part = (float*)ws;
+  A.out = out; A.out2 = out2; A.lse = lse; A.rest = rest; A.part = (float*)ws;
   const int rc = samble_launch_diff_fwd(type, &A, (hipStream_t)stream);
   if (rc == -22) return fail(SAMBLE_E_INVALID, "samble_diff_attn_fwd: more rows and heads than one launch holds");
   return done(rc, "samble_diff_attn_fwd");
@@ -1520,6 +1534,15 @@ SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const
                                     const uint8_t* key_mask, int causal, float scale, const void* out, const void* out2,
                                     const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dlam, void* ws,
                                     size_t ws_bytes, void* stream) {
+  return samble_diff_attn_bwd_rest(type, lam_type, q, k, v, lam, shape, strides, lengths, q_start, key_mask, causal, scale, out, out2,
+                                   lse, nullptr, dout, dq, dk, dv, dlam, ws, ws_bytes, stream);
+}
+
+SAMBLE_API int samble_diff_attn_bwd_rest(int type, int lam_type, const void* q, const void* k, const void* v, const void* lam,
+                                         const int64_t* shape, const int64_t* strides, const int32_t* lengths,
+                                         const int32_t* q_start, const uint8_t* key_mask, int causal, float scale, const void* out,
+                                         const void* out2, const float* lse, const int8_t* rest, const void* dout, void* dq,
+                                         void* dk, void* dv, void* dlam, void* ws, size_t ws_bytes, void* stream) {
   samble::DaArgs A;
   if (int rc = diff_args("samble_diff_attn_bwd" SAMBLE_DIFF_NEEDS, type, lam_type, q, k, v, lam, shape, strides, lengths, q_start,
                          key_mask, causal, scale, &A))
@@ -1529,9 +1552,12 @@ SAMBLE_API int samble_diff_attn_bwd(int type, int lam_type, const void* q, const
       !rows16(type, dq, &none, 1) || !rows16(type, dk, &none, 1) || !rows16(type, dv, &none, 1) || !lse || !dlam ||
       !aligned_for(lam_type, dlam))
     return fail(SAMBLE_E_INVALID, "samble_diff_attn_bwd: out, out2, lse, dout, dq, dk, dv, dlam are needed, rows on 16 bytes");
+  if (!rest_ok(type, rest, out2))
+    return fail(SAMBLE_E_INVALID, "samble_diff_attn_bwd: rest with out2 of a 16-bit type only, on 16 bytes");
   if (!ws || ws_bytes < samble_diff_attn_bwd_workspace_bytes(type, shape) || (reinterpret_cast<uintptr_t>(ws) & 15))
     return fail(SAMBLE_E_WORKSPACE, "samble_diff_attn_bwd: workspace too small (samble_diff_attn_bwd_workspace_bytes)");
   A.out = const_cast<void*>(out); A.out2 = const_cast<void*>(out2); A.lse = const_cast<float*>(lse); A.dout = dout;
+  A.rest = const_cast<int8_t*>(rest);
   A.g_bs = strides[12]; A.g_rs = strides[13]; A.g_hs = strides[14];
   A.dq = dq; A.dk = dk; A.dv = dv; A.dlam = dlam; A.delta = (float*)ws;
   const int rc = samble_launch_diff_bwd(type, &A, (hipStream_t)stream);

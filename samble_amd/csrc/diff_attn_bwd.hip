@@ -3,10 +3,11 @@
 //     dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dv = (P_1 - lam P_2)^T g,  dlam = - sum_i t_2
 // The logits are formed again from q and k; P = exp2(logit - lse) with the forward's row statistics.  No atomics:
 //   diff_dq_kernel   a wave owns 32 rows (layout of the forward): first t_1 = g . out + lam t_2 and t_2 = g . out2 from the
-//                    saved outputs, then one sweep over the keys.  16-bit outputs are rounded, and so is a t of them; since
-//                    sum_j P = 1, sum_j P (dA - t) is what it lacks, and t plus that sum is kept for the second launch
-//                    (dlam adds t over all rows: there the roundings of 2^-9 or 2^-12 would not be small beside a sum of
-//                    both signs)
+//                    saved outputs, then one sweep over the keys.  16-bit outputs are rounded, and t of them is off by as much
+//                    in all keys of a row: where the row sees one key almost alone, by more than dA - t itself (19 keys, bf16:
+//                    dq off by 2.4 times its own rounding; 1.5 times with a whole t).  So the forward leaves a byte beside
+//                    each (`rest`), and t has 15 bits at least.  Since sum_j P = 1, sum_j P (dA - t) is what still lacks; t
+//                    plus that sum is kept for the second launch, whose dlam adds t over all rows
 //                    fp16: dS is held times a power of two of the row, from the largest dA and t so far
 //   diff_dkv_kernel  a wave owns 32 keys and sweeps over the rows of all query heads that share the key head, or over a part
 //                    of them (`splits`, added by diff_dkv_join_kernel); workgroups behind the last one sum dlam
@@ -83,7 +84,8 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
     const T* gp = (const T*)A.dout + b * A.g_bs + qi * A.g_rs + head * A.g_hs;
     const long at = (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
     da_row<T, 2 * KS>(gp, 2 * A.d, live, h, gf);
-#pragma unroll
+    // (four steps' loads in flight, and no branch around them: all of them take registers that the sweep then spills)
+#pragma unroll 4
     for (int s = 0; s < 2 * KS; ++s) {
       const int o = 16 * s + 8 * h;
       const bool ok = live && o < 2 * A.d;
@@ -95,6 +97,15 @@ __global__ __launch_bounds__((DqCfg<T, DP>::NT), (DqCfg<T, DP>::WPS)) void diff_
       raw.widen(g);
       o1.widen(u);
       o2.widen(w);
+      if constexpr (DaT<T>::NP == 1) {
+        const u32x4 none = {0, 0, 0, 0}, pairs = ok && A.rest ? *reinterpret_cast<const u32x4*>(A.rest + 2 * (at + o)) : none;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int pair = (int)(pairs[e >> 1] << (16 * (1 - (e & 1)))) >> 16;
+          u[e] = da_whole<T>(u[e], (int)((unsigned)pair << 24) >> 24);
+          w[e] = da_whole<T>(w[e], pair >> 8);
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         dot[0] = fmaf(g[e], u[e], dot[0]);

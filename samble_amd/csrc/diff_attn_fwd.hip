@@ -309,25 +309,54 @@ __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A
   }
   if (kw || !live) return;
   const float lam = da_lam<T>(A, head);
-  T* out = (T*)A.out + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
-  T* out2 = A.out2 ? (T*)A.out2 + (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d : nullptr;
+  const long at = (((long)b * A.Nq + qi) * A.H + head) * 2 * A.d;
+  auto second = [&](int dt, int i) { return MW > 1 ? f[(dt * 16 + i) * 64] : o[MPW - 1][dt][i]; };
+  if constexpr (DaT<T>::NP > 1) {
 #pragma unroll
-  for (int dt = 0; dt < DVT; ++dt)
+    for (int dt = 0; dt < DVT; ++dt)
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int col = 32 * dt + 8 * q4 + 4 * h;
-      if (col >= 2 * A.d) continue;
-      typedef T vec __attribute__((ext_vector_type(4)));
-      vec a, z;
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int col = 32 * dt + 8 * q4 + 4 * h;
+        if (col >= 2 * A.d) continue;
+        f32x4 a, z;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v2 = MW > 1 ? f[(dt * 16 + 4 * q4 + e) * 64] : o[MPW - 1][dt][4 * q4 + e];
-        a[e] = (T)fmaf(-lam, v2, o[0][dt][4 * q4 + e]);
-        z[e] = (T)v2;
+        for (int e = 0; e < 4; ++e) {
+          z[e] = second(dt, 4 * q4 + e);
+          a[e] = fmaf(-lam, z[e], o[0][dt][4 * q4 + e]);
+        }
+        *reinterpret_cast<f32x4*>((float*)A.out + at + col) = a;
+        if (A.out2) *reinterpret_cast<f32x4*>((float*)A.out2 + at + col) = z;
       }
-      *reinterpret_cast<vec*>(out + col) = a;
-      if (out2) *reinterpret_cast<vec*>(out2 + col) = z;
-    }
+  } else {      // two groups of four columns, one of them the other half's: 16 bytes
+#pragma unroll
+    for (int dt = 0; dt < DVT; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; q4 += 2) {
+        const int col = 32 * dt + 8 * (q4 + h);
+        if (32 * dt + 8 * q4 >= 2 * A.d) continue;
+        u32x4 a, z, r = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          vec4<T> x, y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 4 * (q4 + k) + e;
+            const float v2 = second(dt, i), v = fmaf(-lam, v2, o[0][dt][i]);
+            x[e] = (T)v;
+            y[e] = (T)v2;
+            if (BOTH) r[2 * k + (e >> 1)] |= da_rests<T>(v, x[e], v2, y[e]) << (16 * (e & 1));
+          }
+          const u32x2 xw = __builtin_bit_cast(u32x2, x), yw = __builtin_bit_cast(u32x2, y);
+          a[2 * k] = xw[0], a[2 * k + 1] = xw[1];
+          z[2 * k] = yw[0], z[2 * k + 1] = yw[1];
+        }
+        *reinterpret_cast<u32x4*>((T*)A.out + at + col) = da_halves(a);
+        if (BOTH) {
+          if (A.out2) *reinterpret_cast<u32x4*>((T*)A.out2 + at + col) = da_halves(z);
+          if (A.rest) *reinterpret_cast<u32x4*>(A.rest + 2 * (at + col)) = da_halves(r);
+        }
+      }
+  }
 }
 
 // adds the splits of a row.  NW = 16: a workgroup per row, a wave takes every sixteenth split (many splits, few rows); NW = 1:
@@ -402,14 +431,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
         const long o = (((long)b * A.Nq + qi) * A.H + head) * cols + 4 * lane;
         typedef T vec __attribute__((ext_vector_type(4)));
         vec a, z;
+        u32x2 r = {0, 0};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v2 = acc[1][e] * i2;
-          a[e] = (T)fmaf(-lam, v2, acc[0][e] * i1);
+          const float v2 = acc[1][e] * i2, v = fmaf(-lam, v2, acc[0][e] * i1);
+          a[e] = (T)v;
           z[e] = (T)v2;
+          if constexpr (DaT<T>::NP == 1) r[e >> 1] |= da_rests<T>(v, a[e], v2, z[e]) << (16 * (e & 1));
         }
         *reinterpret_cast<vec*>((T*)A.out + o) = a;
         if (A.out2) *reinterpret_cast<vec*>((T*)A.out2 + o) = z;
+        if (DaT<T>::NP == 1 && A.rest) *reinterpret_cast<u32x2*>(A.rest + 2 * o) = r;
       }
       if (A.lse && lane == 0) {
         float* ls = A.lse + ((long)b * A.H + head) * 2 * A.Nq + qi;

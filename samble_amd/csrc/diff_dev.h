@@ -31,6 +31,7 @@
 
 namespace samble {
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16;
 typedef __bf16 bf16;
@@ -393,6 +394,31 @@ __device__ __forceinline__ float da_sum8(const vec8<E>& v, float c) {
 __device__ __forceinline__ bool da_bit(unsigned word, int j) {
   const unsigned lo = (unsigned)((int)(word << (31 - j)) >> 31), hi = (unsigned)((int)(word << (27 - j)) >> 31);
   return __builtin_amdgcn_inverse_ballot_w64(((unsigned long long)hi << 32) | lo);
+}
+
+// What rounding x to r leaves, in 2^-7 of half a step of the type: the difference of their fp32 encodings, which counts steps of
+// fp32 (of the same sign; fp16's subnormals and infinity: 0).  r and this byte give x to 2^-15 (bf16) or 2^-18 of itself.
+template <typename T> constexpr int kDaRest = __is_same(T, bf16) ? 9 : 6;
+template <typename T>
+__device__ __forceinline__ int da_rest(float x, T r) {
+  const int off = (int)(__float_as_uint(x) - __float_as_uint((float)r)), most = 64 << kDaRest<T>;
+  return off < -most || off > most ? 0 : (off + (1 << (kDaRest<T> - 1))) >> kDaRest<T>;
+}
+template <typename T>
+__device__ __forceinline__ float da_whole(float r, int rest) {
+  return __uint_as_float(__float_as_uint(r) + ((unsigned)rest << kDaRest<T>));
+}
+// the pair of them of an element of out and one of out2
+template <typename T>
+__device__ __forceinline__ unsigned da_rests(float x, T rx, float y, T ry) {
+  return (unsigned)((da_rest<T>(x, rx) & 255) | (da_rest<T>(y, ry) & 255) << 8);
+}
+// words 0, 1 and 2, 3 of the wave's lower half and of its upper half -> words 0, 1 of both in the lower lane, words 2, 3 of both in
+// the upper one
+__device__ __forceinline__ u32x4 da_halves(u32x4 w) {
+  const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+  const u32x4 r = {a[0], b[0], a[1], b[1]};
+  return r;
 }
 
 template <typename T>

@@ -469,10 +469,20 @@ def _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask):
     return (q, k, v), head, shape, strides, [_p(lengths), _p(q_start), _p(key_mask)]
 
 
-def stage_diff_attn_fwd(q, k, v, lam, scale: float, causal: bool, lengths=None, q_start=None, key_mask=None, for_backward=False):
+def _rest_shape(q, rest) -> None:
+    if rest is not None:
+        B, Nq, H, _, d = q.shape
+        if rest.shape != (B, Nq, H, 2 * d, 2) or rest.dtype != torch.int8 or not rest.is_contiguous() or rest.device != q.device:
+            raise ValueError(f"rest must be a contiguous ({B},{Nq},{H},{2 * d},2) int8 tensor on {q.device}")
+
+
+def stage_diff_attn_fwd(q, k, v, lam, scale: float, causal: bool, lengths=None, q_start=None, key_mask=None, for_backward=False,
+                        rest=None):
     """q (B,Nq,H,2,d), k (B,Nk,Hkv,2,d), v (B,Nk,Hkv,2d), lam (H) -> (out (B,Nq,H,2d), out2, lse): csrc/diff_attn_fwd.hip.
-    out2 (the second map's output) and lse (B,H,2,Nq) are what the backward needs (None unless for_backward)."""
-    _need_gpu(q, k, v, lam, lengths, q_start, key_mask)
+    out2 (the second map's output) and lse (B,H,2,Nq) are what the backward needs (None unless for_backward); `rest`, an int8
+    tensor (B,Nq,H,2d,2) for 16-bit types, is filled with what the roundings of out and out2 leave."""
+    _need_gpu(q, k, v, lam, lengths, q_start, key_mask, rest)
+    _rest_shape(q, rest)
     B, Nq, H, _, d = q.shape
     with _on(q.device) as stream:
         out = torch.empty((B, Nq, H, 2 * d), dtype=q.dtype, device=q.device)
@@ -481,22 +491,24 @@ def stage_diff_attn_fwd(q, k, v, lam, scale: float, causal: bool, lengths=None, 
         keep, head, shape, strides, masks = _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask)
         nbytes = _lib.query("samble_diff_attn_fwd_workspace_bytes", head[0], shape)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _lib.call("samble_diff_attn_fwd", *head, (ctypes.c_int64 * 12)(*strides), *masks, causal, scale, out.data_ptr(), _p(out2),
-                  _p(lse), _p(ws), nbytes, stream)
+        _lib.call("samble_diff_attn_fwd_rest", *head, (ctypes.c_int64 * 12)(*strides), *masks, causal, scale, out.data_ptr(),
+                  _p(out2), _p(lse), _p(rest), _p(ws), nbytes, stream)
     return out, out2, lse
 
 
-def stage_diff_attn_bwd(q, k, v, lam, scale: float, causal: bool, lengths, q_start, key_mask, out, out2, lse, g):
-    """-> (dq, dk, dv, dlam), contiguous, in the shapes and types of q, k, v, lam: csrc/diff_attn_bwd.hip."""
-    _need_gpu(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, g)
+def stage_diff_attn_bwd(q, k, v, lam, scale: float, causal: bool, lengths, q_start, key_mask, out, out2, lse, g, rest=None):
+    """-> (dq, dk, dv, dlam), contiguous, in the shapes and types of q, k, v, lam: csrc/diff_attn_bwd.hip.  `rest`: the
+    forward's; without it the row sums of dq come from the rounded outputs."""
+    _need_gpu(q, k, v, lam, lengths, q_start, key_mask, out, out2, lse, g, rest)
+    _rest_shape(q, rest)
     with _on(q.device) as stream:
         dq, dk, dv, dlam = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam)]
         keep, head, shape, strides, masks = _diff_attn_args(q, k, v, lam, lengths, q_start, key_mask)
         g, gs = _rows16(g)
         nbytes = _lib.query("samble_diff_attn_bwd_workspace_bytes", head[0], shape)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.call("samble_diff_attn_bwd", *head, (ctypes.c_int64 * 15)(*strides, *gs), *masks, causal, scale, out.data_ptr(),
-                  out2.data_ptr(), lse.data_ptr(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(),
+        _lib.call("samble_diff_attn_bwd_rest", *head, (ctypes.c_int64 * 15)(*strides, *gs), *masks, causal, scale, out.data_ptr(),
+                  out2.data_ptr(), lse.data_ptr(), _p(rest), g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(),
                   ws.data_ptr(), nbytes, stream)
     return dq, dk, dv, dlam
 

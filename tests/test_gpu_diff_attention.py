@@ -846,3 +846,44 @@ def test_fp16_terms_beyond_the_type(d, lam_value):
         assert bool(torch.isfinite(a).all()) and float(b.abs().max()) < 60000, name
         err = ((a.double() - b).norm() / b.norm()).item()
         assert err <= 4 * 4 * 2.0 ** -11, f"{name}: {err:.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0.0, 64.0])
+@pytest.mark.parametrize("case", [(2, 1, 40, 4, 2, 16), (1, 150, 90, 2, 2, 32), (1, 200, 300, 4, 1, 64), (2, 3, 2100, 4, 2, 64),
+                                  (1, 70, 130, 2, 1, 128), (1, 2, 3000, 1, 1, 128), (1, 60, 50, 2, 2, 24)],
+                         ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_dq_is_not_that_of_rounded_outputs(dtype, case, offset):
+    """Keys and values with a large common part: dq is a difference of terms far larger than itself, and a row sum t from outputs
+    that were rounded to 16 bits would be off in all of them alike.  Bound of an element, h = eps / 2: half a step of it, dS
+    rounded once, P relative (see above), and t off by 2^-7 h of the magnitudes that it sums over (a byte beside each saved value),
+    by h of how far the values stand from the output (P is rounded once in the forward's sums and in their divisor alike) and by
+    fp32 sums over 2 d columns."""
+    B, Nq, Nk, H, Hkv, d = case
+    q, k, v, lam, g, _ = _inputs(*case, TYPES[dtype], 4)
+    k, v = (1.5 + 0.2 * k.float()).to(k.dtype), (offset + v.float()).to(v.dtype)
+    got = _step(q, k, v, lam, g)[1].double()
+    h = torch.finfo(TYPES[dtype]).eps / 2
+    sub = 2.0 ** -25 if dtype == "fp16" else 0.0
+    scale = d ** -0.5
+    for b in range(B):
+        for hq in range(H):
+            kk, vv, gg, lm = k[b, :, hq // (H // Hkv)].double(), v[b, :, hq // (H // Hkv)].double(), g[b, :, hq].double(), float(lam[hq])
+            dA, adA = gg @ vv.T, gg.abs() @ vv.abs().T
+            P = [torch.softmax(q[b, :, hq, m].double() @ kk[:, m].T * scale, -1) for m in range(2)]
+            t2 = (P[1] * dA).sum(-1, keepdim=True)
+            t1 = (P[0] * dA).sum(-1, keepdim=True)
+            o = [p @ vv for p in P]
+            et2 = (gg.abs() * (2.0 ** -7 * h + (2 * d + 32) * U) * o[1].abs()).sum(-1, keepdim=True)
+            et1 = (gg.abs() * (2.0 ** -7 * h + (2 * d + 32) * U) * (o[0] - lm * o[1]).abs()).sum(-1, keepdim=True) + lm * et2
+            for m, (t, et, sign) in enumerate(((t1, et1, 1.0), (t2, et2, -lm))):
+                L = (q[b, :, hq, m].double().abs() @ kk[:, m].abs().T * scale).amax(-1, keepdim=True)
+                dP = 2 * ((d + 32) * U * L + 16 * U) + Nk * U
+                spread = (P[m] * (gg.abs().T[:, :, None] * (vv.T[:, None] - o[m].T[:, :, None]).abs()).sum(0)).sum(-1, keepdim=True)
+                dS = sign * P[m] * (dA - t)
+                edS = abs(sign) * P[m] * (et + h * spread + (2 * d + 32) * U * adA + (dP + 4 * U) * (dA - t).abs()) + h * dS.abs()
+                ref = scale * dS @ kk[:, m]
+                tol = scale * (edS + Nk * U * dS.abs()) @ kk[:, m].abs() * (1 + 1e-3) + h * ref.abs() + sub
+                err = (got[b, :, hq, m] - ref).abs()
+                assert bool((err <= tol).all()), f"b{b} h{hq} m{m}: {(err - tol).max():.3e} over, error {err.max():.3e}"
