@@ -772,7 +772,7 @@ int samble_diff_attn_bwd_rest(int type, int lam_type, const void* q, const void*
                              g = dy weight, plus `extra` (may be null: the gradient that reaches the sum from elsewhere),
                              contiguous; dweight / dbias (both or neither null) of type w_type, sums in fp32 in a fixed order.
                              workspace: samble_layer_norm_workspace_bytes, needed for dweight / dbias only
-   outputs do not overlap inputs, except dx = dy or dx = extra where those are contiguous */
+   C at most 2^30, with weight gradients below 2^26.  Outputs do not overlap inputs, except dx = dy or dx = extra where those are contiguous */
 size_t samble_layer_norm_workspace_bytes(int type, int C, int64_t outer, int64_t inner);
 int samble_layer_norm_fwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* residual, int64_t r_os,
                           int64_t r_cs, const void* weight, const void* bias, int64_t outer, int C, int64_t inner, float eps,

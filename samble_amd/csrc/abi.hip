@@ -1399,7 +1399,8 @@ static bool aligned_for(int type, const void* p) { return (reinterpret_cast<uint
 
 static int ln_args_ok(const char* who, int type, int w_type, const void* x, const void* w, int64_t outer, int C, int64_t inner) {
   if (!type_ok(type) || (w_type != type && w_type != SAMBLE_TYPE_F32)) return fail(SAMBLE_E_INVALID, who);
-  if (outer <= 0 || inner <= 0 || C <= 0 || outer > (int64_t)1 << 40 || inner > (int64_t)1 << 40) return fail(SAMBLE_E_INVALID, who);
+  if (outer <= 0 || inner <= 0 || C <= 0 || C > 1 << 30 || outer > (int64_t)1 << 40 || inner > (int64_t)1 << 40)      // (the kernels step
+    return fail(SAMBLE_E_INVALID, who);                                                     // over C in 32 bits, past its end)
   if (!x || !aligned_for(type, x) || !aligned_for(w_type, w)) return fail(SAMBLE_E_INVALID, who);
   return 0;
 }
@@ -1411,8 +1412,8 @@ SAMBLE_API size_t samble_layer_norm_workspace_bytes(int type, int C, int64_t out
 SAMBLE_API int samble_layer_norm_fwd(int type, int w_type, const void* x, int64_t x_os, int64_t x_cs, const void* residual,
                                      int64_t r_os, int64_t r_cs, const void* weight, const void* bias, int64_t outer, int C,
                                      int64_t inner, float eps, void* y, void* sum, float* mean, float* rstd, void* stream) {
-  if (int rc = ln_args_ok("samble_layer_norm_fwd: need a known type (weights: the same or fp32), outer, C, inner > 0 and "
-                          "element-aligned tensors", type, w_type, x, weight, outer, C, inner))
+  if (int rc = ln_args_ok("samble_layer_norm_fwd: need a known type (weights: the same or fp32), outer, inner > 0, C in "
+                          "1 .. 2^30 and element-aligned tensors", type, w_type, x, weight, outer, C, inner))
     return rc;
   if (!y || (!mean) != (!rstd) || (residual && !sum) || !aligned_for(type, y) || !aligned_for(type, residual) ||
       !aligned_for(type, sum) || !aligned_for(w_type, bias))
@@ -1427,12 +1428,14 @@ SAMBLE_API int samble_layer_norm_bwd(int type, int w_type, const void* x, int64_
                                      const void* weight, const float* mean, const float* rstd, int64_t outer, int C,
                                      int64_t inner, void* dx, void* dweight, void* dbias, void* ws, size_t ws_bytes,
                                      void* stream) {
-  if (int rc = ln_args_ok("samble_layer_norm_bwd: need a known type (weights: the same or fp32), outer, C, inner > 0 and "
-                          "element-aligned tensors", type, w_type, x, weight, outer, C, inner))
+  if (int rc = ln_args_ok("samble_layer_norm_bwd: need a known type (weights: the same or fp32), outer, inner > 0, C in "
+                          "1 .. 2^30 and element-aligned tensors", type, w_type, x, weight, outer, C, inner))
     return rc;
   if (!dy || !mean || !rstd || !dx || !aligned_for(type, dy) || !aligned_for(type, dx) || !aligned_for(type, extra) ||
       (!dweight) != (!dbias) || !aligned_for(w_type, dweight) || !aligned_for(w_type, dbias))
     return fail(SAMBLE_E_INVALID, "samble_layer_norm_bwd: dy, mean, rstd, dx, and dweight with dbias or neither, element-aligned");
+  if (dweight && C >= 1 << 26)      // (64 threads a channel, in a launch of fewer than 2^32)
+    return fail(SAMBLE_E_INVALID, "samble_layer_norm_bwd: weight gradients of fewer than 2^26 channels");
   if (dweight && (!ws || ws_bytes < samble_ln_ws_bytes(type, C, outer, inner)))
     return fail(SAMBLE_E_WORKSPACE, "samble_layer_norm_bwd: workspace too small (samble_layer_norm_workspace_bytes)");
   return done(samble_launch_ln_bwd(type, w_type == SAMBLE_TYPE_F32, x, x_os, x_cs, dy, dy_os, dy_cs, extra, e_os, e_cs, weight,

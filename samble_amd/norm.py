@@ -132,7 +132,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x: fp32, fp16 or bf16, any shape; weight / bias (C,) of x's type or fp32, of one type, either may be None.  residual: x's
     shape and type; then s = x + residual (rounded to x's type) is what is normalised, and (y, s) is returned -- gradients
-    that reach s join in the backward pass.  Statistics and sums are fp32.  Rows of any width and any number of channels;
+    that reach s join in the backward pass.  Statistics and sums are fp32.  Rows of any width and any number of channels
+    (to 2^30; gradients of weight and bias below 2^26);
     leading axes may be strided.  A NaN or infinity stays in its own row."""
     if not isinstance(x, torch.Tensor) or x.dim() == 0:
         raise ValueError("layer_norm: x must be a tensor with at least one axis")
@@ -144,6 +145,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     C = x.shape[dim]
     if C == 0:
         raise ValueError("layer_norm: the normalised axis is empty")
+    if C > 1 << 30:
+        raise ValueError(f"layer_norm: at most 2^30 values in a slice, got {C}")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -151,6 +154,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             raise ValueError(f"layer_norm: {name} must be ({C},) of type {x.dtype} or float32 on {x.device}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("layer_norm: weight and bias must share one type")
+    if C >= 1 << 26 and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (weight, bias)):
+        raise ValueError(f"layer_norm: gradients of weight and bias below 2^26 channels, got {C}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("layer_norm: residual must have x's shape, type and device")
     if not eps >= 0.0:

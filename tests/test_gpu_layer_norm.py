@@ -335,3 +335,23 @@ def test_forward_mode_is_refused():
                 with mode(), pytest.raises(RuntimeError):
                     layer_norm(**kw)
     assert torch.equal(plain, layer_norm(x, w))
+
+
+def test_slices_beyond_the_kernels_indices_are_refused():
+    """2^32 + 5 values are not 5, and a 32-bit index does not step past 2^31."""
+    from samble_amd.norm import layer_norm
+    for n in ((1 << 30) + 1, (1 << 31) - 1, (1 << 32) + 5):
+        for shape, dim in (((n,), 0), ((1, n, 2), 1)):
+            with pytest.raises(ValueError, match="layer_norm"):
+                layer_norm(torch.zeros(()).expand(shape), dim=dim)
+    wide = torch.zeros(()).expand(1 << 26)
+    with pytest.raises(ValueError, match="2\\^26"):
+        layer_norm(wide, wide.clone().requires_grad_(True))
+    fwd = [0, 0, 64, 4, 1, None, 0, 0, None, None, 2, 4, 1, 1e-5, 64, None, None, None, None]
+    bwd = [0, 0, 64, 4, 1, 64, 4, 1, None, 0, 0, None, 64, 64, 2, 4, 1, 64, 64, 64, 64, 1 << 50, None]
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        for name, args, at in (("samble_layer_norm_fwd", fwd, 11), ("samble_layer_norm_bwd", bwd, 15)):
+            with pytest.raises(_lib.SambleError, match=name):
+                _lib.call(name, *args[:at], n, *args[at + 1:])
+    with pytest.raises(_lib.SambleError, match="2\\^26"):
+        _lib.call("samble_layer_norm_bwd", *bwd[:15], 1 << 26, *bwd[16:])
