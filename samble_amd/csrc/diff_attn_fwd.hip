@@ -457,16 +457,17 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void diff_join_kernel(DaAr
 struct FwdPlan { bool few; long blocks; int splits; };
 
 // Few rows (at most 32 of a key head) take the kernels whose waves stand along the keys.  Splits: as many as fill the CUs and no
-// more, since a part of a second round costs a whole one (8 clouds of 1999 points, one head, fp32, d 64: 2 splits 113 us, 3
-// splits 138 us); each split has at least four tiles of 128 keys, since its partial results go through memory, at most 128.
-// Where two workgroups of four waves fit on a CU: as many as fill both places for few rows, and for keys so long that the parts
+// more, since a part of a second round costs a whole one (8 clouds of 1999 points, one head, fp32, d 64, joins included: 2 splits 155 us, 3
+// splits 189 us); each split has at least four tiles of 128 keys, since its partial results go through memory, at most 128.
+// Where two workgroups of four waves fit on a CU (not fp32 of 64-deep heads, 98 KB of tiles: 4 x 5 queries, 8 heads of 48, 5000 keys
+// 82 us for two places, 54 us for one): as many as fill both places for few rows, and for keys so long that the parts
 // are small beside them (4 x 1024 rows, 8 heads of 64, bf16: 2048 keys 85 us, in 2 splits 74 + 18; 4096 keys 163 us, 131 + 18).
 static FwdPlan fwd_plan(bool wide, int B, int Nq, int Nk, int H, int Hkv, int d) {
   const long rows = (long)Nq * (H / Hkv), pairs = (long)B * Hkv;
   FwdPlan p;
   p.few = rows <= 32;
   p.blocks = p.few ? 1 : (rows + 127) / 128;
-  const long have = p.blocks * pairs, room = p.few || (d <= (wide ? 16 : 64) && Nk >= 4096) ? 512 : 256;
+  const long have = p.blocks * pairs, room = (p.few && !(wide && d > 32)) || (d <= (wide ? 16 : 64) && Nk >= 4096) ? 512 : 256;
   long s = room / have;
   const long most = Nk / 512;
   if (s > most) s = most;
