@@ -16,18 +16,19 @@
 // Layout, operands and tiles: diff_dev.h.  The second kernel holds S with the row index on the registers, so that P and dS
 // are operands of the sums over rows as they stand.
 // P, P_1 - lam P_2 and dS of 16-bit tensors are rounded to the tensors' type, the type of the matrix instructions' operands (two
-// planes would double their number): against float64 dq is off by 2.7e-3 and dk by 2.3e-3 of its norm in bf16, where rounding
-// the results alone is 1.7e-3; sums are fp32.
+// planes would double their number): against float64 dq is off by 2.5e-3 and dk by 2.3e-3 of its norm in bf16, where rounding
+// the results alone is 1.7e-3 (fp16: 3.2e-4, 2.1e-4); sums are fp32.
 //
 // Bound: as the forward's, matrix instructions (24 and 32 to a 32 x 32 block of d = 64) and vector ones of a wave in turn.
-// 8 x 2048 x 16 heads of 64, bf16, no mask: dq 510 us (810 TFLOP/s), dk and dv 660 us (835); causal on 4 key heads 281 and
-// 430 us; fp32, 32 x 1024 x 4 heads of 16: 166 and 190 us (the vector unit: two planes of P and dS).
+// 8 x 2048 x 16 heads of 64, bf16, no mask: dq 516 us (800 TFLOP/s), dk and dv 654 us (840); causal on 4 key heads dk and dv
+// 418 us; fp32, 32 x 1024 x 4 heads of 16: 198 and 245 us (vector unit 0.6 of the busy cycles, matrix unit 0.5), 8 x 2048 x 8
+// heads of 64: 1200 and 1516 us (1030 and 1090 TFLOP/s of the matrix unit's).
 #include "diff_dev.h"
 
 namespace samble {
 
 // WPS: waves per SIMD.  Two, but where both maps' operands and gradients need more than 256 registers (8 x 2048 x 8 heads of
-// 128, bf16: one wave with 512 registers 604 us, a wave for each map, both forming dA, 1194 us).
+// 128, bf16: one wave with 512 registers 639 us, a wave for each map, both forming dA, 1194 us).
 template <typename T, int DP>
 struct DqCfg {
   static constexpr int RW = 4, NT = 64 * RW, WPS = DP == 128 || (DaT<T>::NP > 1 && DP == 64) ? 1 : 2;

@@ -7,16 +7,19 @@
 //   RW  waves along the rows, each its own 32
 //   KW  waves along the keys of a tile, each its own 32: for few rows (single tokens); their results meet in LDS
 //   MW  waves along the maps: 1 = both in one wave, which share every value read; 2 where the outputs of two maps would
-//       leave no registers (8 x 2048 x 8 heads of 128, bf16: 515 us; both maps in one wave of 512 registers 4.5 ms)
+//       leave no registers (8 x 2048 x 8 heads of 128, bf16: 430 us, with its spills at the ends of the sweep; both maps in
+//       one wave of 512 registers 4.5 ms), and for fp32 of 32-deep heads (557 us either way, without spills)
 // Few rows against many keys are also split over workgroups (`splits`); diff_join_kernel adds the parts.
 //
 // Bound.  Many rows: a 32 x 32 block of both maps is 24 matrix instructions (d = 64; 768 cycles) and about 250 vector ones
 // (1100 cycles: exponential, sum, maximum, conversion), which two waves of a SIMD can overlap but one wave issues one after
-// the other.  8 x 2048 x 16 heads of 64, bf16, no mask: 460 us, 900 TFLOP/s with both value products counted (a large matrix
-// product reaches 1175); causal on 4 key heads 238 us; fp32, 8 heads: 670 us, 310 TFLOP/s of three products each.
-// Single tokens: the cache's bytes.  16 sequences of up to 8192 keys, 8 key heads of 64, bf16: 77 + 5 us, 4.6 TB/s; one
-// sequence of 128-deep heads: 54 + 8 us, 4.9 TB/s.  A causal call whose blocks all start at once (2 x 2048, 4 key heads, for training: 93 us)
-// lasts as long as the longest row block, alone on its CU at the end.
+// the other.  8 x 2048 x 16 heads of 64, bf16, no mask: 412 us, 1000 TFLOP/s with both value products counted (a large matrix
+// product reaches 1175), 493 us with what the backward needs; causal on 4 key heads 219 us.  fp32, 8 heads: 1000 us, 206
+// TFLOP/s of six products each, all that the matrix unit gives.  Single tokens: the cache's bytes.  16 sequences of up to 8192
+// keys, 8 key heads of 64, bf16: 80 + 5 us, 4.5 TB/s (fp32, all of 8192: 262 + 5 us, 4.1 TB/s; a tile's planes leave room for one
+// workgroup a CU, and none of its loads is in flight while it splits them); one sequence of 128-deep heads: 52 + 9 us, 5.1 TB/s.
+// A causal call whose blocks all start at once (2 x 2048, 4 key heads, for training: 95 us) lasts as long as the longest row
+// block, alone on its CU at the end.
 #include "diff_dev.h"
 
 namespace samble {
@@ -42,7 +45,8 @@ __device__ __forceinline__ float da_lse(float m, float l, int shift) {      // l
 }
 
 // (Registers are held to two waves per SIMD, so that one wave's matrix instructions run under the other's exponentials; the
-// whole file of 512 would put every accumulator into the half that the vector unit cannot read.)
+// whole file of 512 would put every accumulator into the half that the vector unit cannot read.  128-deep heads spill 22 .. 55
+// registers, before and behind the sweep, not in it.)
 // (BOTH: the backward comes.)
 template <typename T, int DP, int RW, int KW, int MW, bool BOTH>
 __global__ __launch_bounds__(64 * RW * KW * MW, 2) void diff_fwd_kernel(DaArgs A) {

@@ -772,7 +772,8 @@ static LnPlan ln_plan(int C, int V) {
   return {0, 0};
 }
 // Lanes along N: at most 512 threads in a workgroup, whose waves then have 256 registers (8 x 512 x 2048, backward: fp32 29 us, bf16
-// 52 us; 1024 threads of 128 registers spill: 160 us, 176 us).
+// 52 us; 1024 threads of 128 registers spill: 160 us, 176 us).  That is room for fp32; the backward of the 16-bit types, eight
+// columns a thread, still spills 115 .. 126 registers in all three forms above 128 channels.
 constexpr int ln_chan_lanes(int tc) { return tc > 32 ? 512 / tc : 16; }
 static LnPlan ln_chan_plan(int C) {   // threads along C, pieces per thread
   if (C <= 16) return {16, 1};
