@@ -568,8 +568,9 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     differentiable in q, k, v and lam (reverse mode; dual tensors of forward mode are refused).
 
     q (B, Nq, H, 2, d), k (B, Nk, Hkv, 2, d): two maps per head; v (B, Nk, Hkv, 2 d) -> (B, Nq, H, 2 d).  fp32, fp16 or
-    bf16, one type, softmax statistics and sums in fp32 (fp32 tensors enter the products whole, 24 bits at any magnitude); Hkv divides H (query head h reads key head h // (H // Hkv)); d a
-    multiple of 8 up to 128 (fp32: 64).  Any strides (copied unless rows start on 16 bytes and the last axis is contiguous).
+    bf16, one type, softmax statistics and sums in fp32 (fp32 tensors enter the products
+    whole, 24 bits from 2^-100 to 2^100); Hkv divides H (query head h reads key head h // (H // Hkv)); d a multiple of 8 up to 128
+    (fp32: 64).  Any strides (copied unless rows start on 16 bytes and the last axis is contiguous).
     lam: (H,) or one value, of q's type or fp32.  scale: 1 / sqrt(d) unless given, positive.
     lengths (B,): item b has that many keys (out of 0 .. Nk: the nearest); key_mask (B, Nk) bool: False = the key does not
     exist.  Whatever stands at keys that do not exist, NaN included, is not used and gets gradient 0.

@@ -45,7 +45,7 @@ __device__ __forceinline__ float da_lse(float m, float l, int shift) {      // l
 }
 
 // (Registers are held to two waves per SIMD, so that one wave's matrix instructions run under the other's exponentials; the
-// whole file of 512 would put every accumulator into the half that the vector unit cannot read.  128-deep heads spill 22 .. 55
+// whole file of 512 would put every accumulator into the half that the vector unit cannot read.  128-deep heads spill 22 .. 57
 // registers, before and behind the sweep, not in it.)
 // (BOTH: the backward comes.)
 template <typename T, int DP, int RW, int KW, int MW, bool BOTH>

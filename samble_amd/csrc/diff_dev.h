@@ -397,16 +397,21 @@ __device__ __forceinline__ bool da_bit(unsigned word, int j) {
 }
 
 // What rounding x to r leaves, in 2^-7 of half a step of the type: the difference of their fp32 encodings, which counts steps of
-// fp32 (of the same sign; fp16's subnormals and infinity: 0).  r and this byte give x to 2^-15 (bf16) or 2^-18 of itself.
+// fp32 (x and r have one sign), or where fp16's own steps end, 2^-24 apart, that of their values; an infinity leaves 0.  r and this
+// byte give x to 2^-15 (bf16) or 2^-18 of itself, or to 2^-32.
 template <typename T> constexpr int kDaRest = __is_same(T, bf16) ? 9 : 6;
+template <typename T> __device__ __forceinline__ bool da_fixed(float r) { return __is_same(T, f16) && fabsf(r) < 0x1p-14f; }
 template <typename T>
 __device__ __forceinline__ int da_rest(float x, T r) {
-  const int off = (int)(__float_as_uint(x) - __float_as_uint((float)r)), most = 64 << kDaRest<T>;
-  return off < -most || off > most ? 0 : (off + (1 << (kDaRest<T> - 1))) >> kDaRest<T>;
+  const float f = (float)r;
+  const int off = (int)(__float_as_uint(x) - __float_as_uint(f)), most = 64 << kDaRest<T>;
+  const int steps = off < -most || off > most ? 0 : (off + (1 << (kDaRest<T> - 1))) >> kDaRest<T>;
+  return da_fixed<T>(f) ? (int)rintf((x - f) * 0x1p31f) : steps;
 }
 template <typename T>
 __device__ __forceinline__ float da_whole(float r, int rest) {
-  return __uint_as_float(__float_as_uint(r) + ((unsigned)rest << kDaRest<T>));
+  const float x = __uint_as_float(__float_as_uint(r) + ((unsigned)rest << kDaRest<T>));
+  return da_fixed<T>(r) ? fmaf((float)rest, 0x1p-31f, r) : x;
 }
 // the pair of them of an element of out and one of out2
 template <typename T>

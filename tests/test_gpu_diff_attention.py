@@ -887,3 +887,43 @@ def test_dq_is_not_that_of_rounded_outputs(dtype, case, offset):
                 tol = scale * (edS + Nk * U * dS.abs()) @ kk[:, m].abs() * (1 + 1e-3) + h * ref.abs() + sub
                 err = (got[b, :, hq, m] - ref).abs()
                 assert bool((err <= tol).all()), f"b{b} h{hq} m{m}: {(err - tol).max():.3e} over, error {err.max():.3e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** -18, 2.0 ** -21])
+@pytest.mark.parametrize("case", [(2, 150, 90, 2, 2, 32), (1, 200, 300, 4, 1, 64), (2, 3, 2100, 4, 2, 64), (1, 70, 130, 2, 1, 128)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_fp16_outputs_below_the_types_normal_numbers(case, size):
+    """Values of few steps of 2^-24: the outputs stand among fp16's last steps, but dS, dq and dk do not (gradients of 2^12).  Bound against the norm of each gradient in float64, as above: dS and what t is made of rounded once each."""
+    q, k, v, lam, g, _ = _inputs(*case, torch.float16, 8)
+    v, g = (v.float() * size).half(), (4096 * g.float()).half()
+    want = _exact(q, k, v, lam, g)
+    for name, a, b in zip(("dq", "dk", "dv", "dlam"), _step(q, k, v, lam, g)[1:], want[1:]):
+        own, err = (b.to(a.dtype).double() - b).norm(), (a.double() - b).norm()
+        assert err <= own + 2 * 2.0 ** -11 * b.norm(), f"{name}: {(err / b.norm()).item():.2e}, rounding alone {(own / b.norm()).item():.2e}"
+
+
+def test_the_rest_of_the_outputs_is_refused_where_there_is_none():
+    import ctypes
+
+    from samble_amd import ops
+    shape, st = (ctypes.c_int64 * 6)(1, 2, 3, 4, 2, 16), (ctypes.c_int64 * 15)(256, 128, 32, 16, 192, 64, 32, 16, 192, 64, 32, 0, 256, 128, 32)
+
+    def fwd(kind, out2, rest):
+        _lib.call("samble_diff_attn_fwd_rest", kind, kind, 256, 256, 256, 256, shape, st, None, None, None, 0, 0.25, 256, out2, out2,
+                  rest, None, 0, None)
+
+    def bwd(kind, rest):
+        _lib.call("samble_diff_attn_bwd_rest", kind, kind, 256, 256, 256, 256, shape, st, None, None, None, 0, 0.25, 256, 256, 256, rest,
+                  256, 256, 256, 256, 256, 256, 1 << 20, None)
+
+    for call in (lambda: fwd(0, 256, 256), lambda: fwd(1, 256, 264), lambda: fwd(2, None, 256), lambda: bwd(0, 256), lambda: bwd(2, 260)):
+        with pytest.raises(_lib.SambleError, match="rest"):
+            call()
+    q = torch.zeros(1, 2, 4, 2, 16, dtype=torch.float16)
+    good = torch.zeros(1, 2, 4, 32, 2, dtype=torch.int8)
+    ops._rest_shape(q, good)
+    ops._rest_shape(q, None)
+    for bad in (good.float(), good[..., :1], good.transpose(1, 2), torch.zeros(1, 2, 4, 32, 4, dtype=torch.int8)[..., ::2]):
+        with pytest.raises(ValueError, match="rest"):
+            ops._rest_shape(q, bad)
