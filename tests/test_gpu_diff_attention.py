@@ -927,3 +927,24 @@ def test_the_rest_of_the_outputs_is_refused_where_there_is_none():
     for bad in (good.float(), good[..., :1], good.transpose(1, 2), torch.zeros(1, 2, 4, 32, 4, dtype=torch.int8)[..., ::2]):
         with pytest.raises(ValueError, match="rest"):
             ops._rest_shape(q, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(2, 150, 150, 4, 2, 64), (1, 1500, 130, 2, 1, 32), (2, 2, 2100, 4, 2, 48)], ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_training_step_replayed(case, dtype):
+    """Gradients of other sizes at each replay (scales are made anew), the first call of its kind captured where it is the first."""
+    q, k, v, lam, g, gen = _inputs(*case, TYPES[dtype], 12)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        held = _step(q, k, v, lam, g, causal=True)
+    for size in (1.0, 2.0 ** -9, 2.0 ** 7, 1.0):
+        q.copy_(torch.randn(q.shape, generator=gen, device=DEV))
+        g.copy_(size * torch.randn(g.shape, generator=gen, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = _step(q, k, v, lam, g, causal=True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, held)), size
